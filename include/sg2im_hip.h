@@ -26,7 +26,7 @@ extern "C" {
 #define SG2IM_ERR_ARG 1   /* invalid argument (the reference would raise / assert) */
 #define SG2IM_ERR_HIP 2   /* a HIP runtime call failed; see hipGetLastError() */
 
-int sg2im_abi_version(void);   /* 11 (11: + sg2im_csr_build_triples; 10: bfloat16 storage, weight mirror) */
+int sg2im_abi_version(void);   /* 12 (12: + group norm, linear with residual, 8-bit checkpoints; 11: + sg2im_csr_build_triples; 10: bfloat16 storage, weight mirror) */
 
 /* Statistics: kernels this library has launched (or recorded into a stream capture) so far in this process;
  * which = 0: all of them, 1: the implicit-GEMM family incl. its split-K finishes.  bench.py reads it around the
@@ -660,6 +660,65 @@ int sg2im_adam_prepare_guarded(float lr, float beta1, float beta2, float* state,
 int sg2im_adam_apply_guarded(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, long long n,
                              float beta1, float beta2, float eps, float grad_scale, const float* state,
                              hipStream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Group normalisation + LeakyReLU on channels-last maps [batch][hw][channels]; statistics over the hw pixels and
+ * channels / groups channels of a group, biased variance (torch.nn.GroupNorm; the normalisations of sg2im/layers.py:22-31
+ * have no counterpart that is independent of the batch and has parameters).  Types: 0 float, 1 bfloat16.
+ *   forward:  out = leaky_slope(gamma * (x - mean) * rstd + beta); out_dtype = x_dtype, or bfloat16 from float.
+ *             stats: double[batch][groups][2] = mean, rstd, for the backward pass.  gamma / beta may be NULL (1 / 0).
+ *             codes / exps (both or neither): the 8-bit form of x is written too (sg2im_pack8).
+ *   backward: from x, or - codes / exps given - from its 8-bit form; dy has out's type, dx has x_dtype.  dx, dgamma, dbeta may
+ *             be NULL.  accumulate: dgamma / dbeta += .  The side of the LeakyReLU is decided in 64 bits where the
+ *             32-bit value is within its rounding of zero; at exactly zero the gradient takes `slope`.
+ * workspace: sg2im_groupnorm_workspace bytes, used by this call only.  No alignment beyond an element's is assumed.
+ * SG2IM_ERR_ARG: channels % groups, hw < 1, a NULL that is needed, a workspace that is too small. */
+size_t sg2im_groupnorm_workspace(int batch, long long hw, int channels, int groups, int x_dtype, int backward);
+int sg2im_groupnorm_act_forward(const void* x, int x_dtype, int batch, long long hw, int channels, int groups,
+                                const void* gamma, const void* beta, int param_dtype, float slope, float eps, void* out,
+                                int out_dtype, double* stats, signed char* codes, unsigned char* exps, void* workspace,
+                                size_t workspace_bytes, hipStream_t stream);
+int sg2im_groupnorm_act_backward(const void* dy, int dy_dtype, const void* x, int x_dtype, const signed char* codes,
+                                 const unsigned char* exps, int batch, long long hw, int channels, int groups,
+                                 const void* gamma, const void* beta, int param_dtype, float slope, const double* stats,
+                                 void* dx, void* dgamma, void* dbeta, int grad_dtype, int accumulate, void* workspace,
+                                 size_t workspace_bytes, hipStream_t stream);
+
+/* An activation in 8 bits.  Every row's channels are cut into blocks of 32; a block shares the power of two 2^e, the
+ * smallest with max|x| <= 127 * 2^e (e clamped to [-126, 121]), and holds round-to-even(x / 2^e) in [-127, 127].  -128
+ * stands for an element that is not finite and reads back as NaN.  codes: [rows][channels], exps:
+ * [rows][ceil(channels / 32)] = e + 127.  The values are exact in bfloat16 and float; unpack8 writes either type. */
+int sg2im_pack8(const void* x, int dtype, long long rows, int channels, long long ld, signed char* codes,
+                unsigned char* exps, hipStream_t stream);
+int sg2im_unpack8(const signed char* codes, const unsigned char* exps, long long rows, int channels, void* out, int dtype,
+                  long long ld, hipStream_t stream);
+
+/* Linear layer with bias, LeakyReLU and residual in its epilogue (nn.Linear of sg2im/layers.py:216-232 next to the sum of
+ * a ResidualBlock, sg2im/layers.py:117); x [rows][k], weight [n][k] dense, both of `dtype` (0 float, 1 bfloat16 - bfloat16
+ * products accumulate in float).
+ *   forward:          out = leaky_slope(x W^T + bias) + residual; residual has out's type: `dtype`, or float from bfloat16.
+ *                     bias / residual may be NULL.  signs: uint32[rows][ceil(n / 32)], bit j of word w = (z > 0) of column
+ *                     32 w + j, for the backward pass; NULL: not written (slope 1, or no backward pass).
+ *   backward_act:     dz = dy * (sign ? 1 : slope) in dz_dtype, dense, and dbias (+)= column sums of the unrounded dz.
+ *                     signs NULL: dz = dy.  dz NULL: only dbias; dbias NULL: only dz.
+ *   backward_data:    dx = dz W
+ *   backward_weight:  dweight (+)= dz^T x, from x or from its 8-bit form (codes / exps, dense, of x's rows)
+ * workspace: sg2im_linear_workspace bytes for `which` = 0 forward, 1 backward_data, 2 backward_weight, 3 backward_act.
+ * Rows below 2^31 - 256; leading dimensions in elements; no alignment beyond an element's is assumed. */
+size_t sg2im_linear_workspace(long long rows, int k, int n, int dtype, int which);
+int sg2im_linear_forward(const void* x, int dtype, long long ld_x, const void* weight, const void* bias, int bias_dtype,
+                         const void* residual, long long ld_res, float slope, void* out, int out_dtype, long long ld_out,
+                         unsigned* signs, long long rows, int k, int n, void* workspace, size_t workspace_bytes,
+                         hipStream_t stream);
+int sg2im_linear_backward_act(const void* dy, int dy_dtype, long long ld_dy, const unsigned* signs, float slope, void* dz,
+                              int dz_dtype, void* dbias, int bias_dtype, int accumulate, long long rows, int n,
+                              void* workspace, size_t workspace_bytes, hipStream_t stream);
+int sg2im_linear_backward_data(const void* dz, int dtype, long long ld_dz, const void* weight, void* dx, long long ld_dx,
+                               long long rows, int k, int n, void* workspace, size_t workspace_bytes, hipStream_t stream);
+int sg2im_linear_backward_weight(const void* dz, int dtype, long long ld_dz, const void* x, long long ld_x,
+                                 const signed char* codes, const unsigned char* exps, void* dweight, int dweight_dtype,
+                                 int accumulate, long long rows, int k, int n, void* workspace, size_t workspace_bytes,
+                                 hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,71 @@
+// 16-byte pieces of rows whose start has only the alignment of one element.  gfx950 runs with unaligned access on for
+// global memory, so a dwordx4 load or store of a 2-byte aligned address is one instruction; odd widths then need no
+// scalar path, only their last piece of a row does.
+#pragma once
+#include <hip/hip_runtime.h>
+
+namespace sg2im {
+
+typedef __bf16 bf16_s;
+
+template <typename T> struct VecOf { static constexpr int n = 16 / sizeof(T); };
+
+__device__ __forceinline__ float bf16_bits_to_f32(unsigned short b) { return __uint_as_float((unsigned)b << 16); }
+// (round to nearest even; v_cvt_pk_bf16_f32)
+__device__ __forceinline__ unsigned short f32_to_bf16_bits(float v) { return __builtin_bit_cast(unsigned short, (__bf16)v); }
+
+template <typename T> __device__ __forceinline__ float load1(const T* p);
+template <> __device__ __forceinline__ float load1<float>(const float* p) { return *p; }
+template <> __device__ __forceinline__ float load1<bf16_s>(const bf16_s* p) {
+  return bf16_bits_to_f32(*reinterpret_cast<const unsigned short*>(p));
+}
+template <typename T> __device__ __forceinline__ void store1(T* p, float v);
+template <> __device__ __forceinline__ void store1<float>(float* p, float v) { *p = v; }
+template <> __device__ __forceinline__ void store1<bf16_s>(bf16_s* p, float v) {
+  *reinterpret_cast<unsigned short*>(p) = f32_to_bf16_bits(v);
+}
+
+// NV elements of T <-> registers, any element alignment
+template <typename T, int NV> struct RawVec { unsigned short h[NV]; };
+template <int NV> struct RawVec<float, NV> { float h[NV]; };
+
+template <typename T, int NV> __device__ __forceinline__ RawVec<T, NV> load_raw(const T* p) {
+  RawVec<T, NV> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+template <int NV> __device__ __forceinline__ void widen(const RawVec<float, NV>& r, float (&v)[NV]) {
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) v[j] = r.h[j];
+}
+template <int NV> __device__ __forceinline__ void widen(const RawVec<bf16_s, NV>& r, float (&v)[NV]) {
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) v[j] = bf16_bits_to_f32(r.h[j]);
+}
+template <typename T, int NV> __device__ __forceinline__ void load_vec(const T* p, float (&v)[NV]) {
+  widen(load_raw<T, NV>(p), v);
+}
+template <typename T, int NV> __device__ __forceinline__ void store_vec(T* p, const float (&v)[NV]) {
+  RawVec<T, NV> r;
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if constexpr (sizeof(T) == 4) r.h[j] = v[j]; else r.h[j] = f32_to_bf16_bits(v[j]);
+  }
+  __builtin_memcpy(p, &r, sizeof(r));
+}
+
+// the parameters (affine, bias) are float32 or bfloat16: a wave-uniform choice
+__device__ __forceinline__ float load_param(const void* p, int is_bf16, long long i) {
+  return is_bf16 ? load1(reinterpret_cast<const bf16_s*>(p) + i) : reinterpret_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ void store_param(void* p, int is_bf16, long long i, float v, int accumulate) {
+  if (is_bf16) {
+    bf16_s* q = reinterpret_cast<bf16_s*>(p) + i;
+    store1(q, accumulate ? load1(q) + v : v);
+  } else {
+    float* q = reinterpret_cast<float*>(p) + i;
+    *q = accumulate ? *q + v : v;
+  }
+}
+
+}  // namespace sg2im
