@@ -218,6 +218,28 @@ def load():
   return lib
 
 
+NATIVE_PATH = os.path.join(_HERE, 'lib', 'sg2im_native.so')
+_native = None
+
+
+def native():
+  """the host module of csrc/native.cpp, bound to the loaded library (once); raises when it is missing"""
+  global _native
+  if _native is None:
+    if not os.path.exists(NATIVE_PATH):
+      raise Sg2imHipError('sg2im_native.so not found at %s - build it with `python -m sg2im_amd.build` '
+                          '(or __graft_entry__.build()); the HIP path has no fallback' % NATIVE_PATH)
+    import importlib.util
+    lib = load()
+    spec = importlib.util.spec_from_file_location('sg2im_native', NATIVE_PATH)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    mod.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in _SIGNATURES
+              if name.startswith(('sg2im_init', 'sg2im_groupnorm', 'sg2im_linear', 'sg2im_pack8', 'sg2im_unpack8'))})
+    _native = mod
+  return _native
+
+
 _TRACE = os.environ.get('SG2IM_TRACE', '') == '1'
 EAGER_EPOCH = 0      # number of EAGER launches made through this binding (captured ones do not count)
 CAPTURING = False    # set by the Trainer around a stream capture: launches are recorded, not executed
@@ -232,6 +254,14 @@ def init():
     if load().sg2im_init() != SG2IM_OK:
       raise Sg2imHipError('sg2im_init failed')
     _inited = True
+
+
+def eager():
+  """the host module, for a call that launches: counted as eager outside a capture, like those of call()"""
+  global EAGER_EPOCH
+  if not CAPTURING:
+    EAGER_EPOCH += 1
+  return _native or native()
 
 
 def call(name, *args):

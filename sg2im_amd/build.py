@@ -1,5 +1,6 @@
 """Build libsg2im_hip.so (gfx950) in-tree with hipcc.  No torch involved: the library is a
-plain C-ABI shared object (include/sg2im_hip.h) loaded through ctypes."""
+plain C-ABI shared object (include/sg2im_hip.h) loaded through ctypes.  Next to it lib/sg2im_native.so, a host-only
+module against torch: checks, buffers and autograd nodes around some of its entry points (csrc/native.cpp)."""
 import os
 import subprocess
 import sys
@@ -11,6 +12,7 @@ LIBDIR = os.path.join(HERE, 'lib')
 LIB = os.path.join(LIBDIR, 'libsg2im_hip.so')
 SOURCES = ['conv.hip', 'graph.hip', 'gconv.hip', 'gcn_persist.hip', 'heads.hip', 'norm.hip', 'layout.hip', 'loss.hip',
            'groupnorm.hip', 'linear.hip']
+NATIVE = os.path.join(LIBDIR, 'sg2im_native.so')
 INCLUDES = {}      # (.hip files another translation unit includes: none)
 # (packed fp32 arithmetic off: hipcc -O3 forms v_pk_{add,mul,fma}_f32 from ordinary float code, and some of their forms have
 # given wrong results now and then; the host pass does not know the feature and says so, which is harmless)
@@ -23,6 +25,24 @@ def _stale(target, deps):
     return True
   t = os.path.getmtime(target)
   return any(os.path.getmtime(d) > t for d in deps)
+
+
+def build_native(force=False, verbose=True):
+  """lib/sg2im_native.so with the host compiler (csrc/native.cpp holds no device code)"""
+  import sysconfig
+  src = os.path.join(CSRC, 'native.cpp')
+  if not (force or _stale(NATIVE, [src, os.path.join(ROOT, 'include', 'sg2im_hip.h')])):
+    return None
+  import torch
+  inc = os.path.join(os.path.dirname(torch.__file__), 'include')
+  lib = os.path.join(os.path.dirname(torch.__file__), 'lib')
+  cmd = ['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-w', '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM', '-DTORCH_EXTENSION_NAME=sg2im_native',
+         '-D_GLIBCXX_USE_CXX11_ABI=%d' % int(torch._C._GLIBCXX_USE_CXX11_ABI), '-I' + os.path.join(ROOT, 'include'), '-I' + inc,
+         '-I' + os.path.join(inc, 'torch', 'csrc', 'api', 'include'), '-I' + sysconfig.get_paths()['include'],
+         '-I/opt/rocm/include', src, '-o', NATIVE, '-L' + lib, '-ltorch', '-ltorch_cpu', '-ltorch_python', '-lc10', '-lc10_hip']
+  if verbose:
+    print(' '.join(cmd), flush=True)
+  return subprocess.Popen(cmd)
 
 
 def build(force=False, verbose=True, cflags=(), tag=''):
@@ -43,9 +63,12 @@ def build(force=False, verbose=True, cflags=(), tag=''):
       if verbose:
         print(' '.join(cmd), flush=True)
       procs.append((src, subprocess.Popen(cmd)))
+  native = build_native(force, verbose) if not tag else None
   for src, pr in procs:
     if pr.wait() != 0:
       raise RuntimeError('hipcc failed on %s' % src)
+  if native is not None and native.wait() != 0:
+    raise RuntimeError('g++ failed on native.cpp')
   if force or procs or _stale(lib_path, objs):
     cmd = [hipcc, '--offload-arch=gfx950', '-shared', '-fPIC', '-o', lib_path] + objs
     if verbose:

@@ -25,9 +25,9 @@ constexpr int THREADS = 256;
 
 struct Params {
   const void* x;
-  const signed char* codes;          // instead of x in the backward pass (and written by the forward pass)
+  const signed char* codes;          // instead of x in the backward pass
   const unsigned char* exps;
-  signed char* codes_out;
+  signed char* codes_out;            // written by the forward pass
   unsigned char* exps_out;
   const void* dy;
   const void* gamma;
@@ -36,14 +36,15 @@ struct Params {
   float slope, eps;
   void* out;                         // y, or dx
   double* stats;                     // [N][G][2] mean, rstd
-  void* part;                        // [N][chunks][2][L]: double sums of x, x^2 / float sums of dz, dz xh
+  void* part;                        // [N][chunks][2][L]: double sums of x, x^2 / float sums of dz, dz (x - m)
   double* chan;                      // [N][C][2] sums of dz, dz xh over the pixels
   float* coef;                       // [N][G][2] m1, m2
   void* dgamma;
   void* dbeta;
   int grad_bf16, accumulate;
   long long E;
-  int N, C, G, D, L, rows, chunks, rows_per_chunk, slabs, TV, TP, nblk;
+  int N, C, G, D, L, rows, full_rows, chunks, rows_per_chunk, slabs, TV, TP, nblk;
+  int S;                             // resident kernels: positions per workgroup
 };
 
 // the lane's place: position q0 of its piece in a row, the pixel lane, and this workgroup's image / rows
@@ -63,86 +64,153 @@ __device__ __forceinline__ Place place_of(const Params& p, int NV, long long blo
   return w;
 }
 
-// values of one piece; f(j) only for those of the image (all of them but in its last piece)
-template <typename T, int NV>
-__device__ __forceinline__ int load_piece(const T* base, long long at, long long E, float (&v)[NV]) {
-  if (at + NV <= E) { load_vec<T, NV>(base + at, v); return NV; }
-  const int have = at < E ? (int)(E - at) : 0;
+// the first `have` elements of a piece, zeros behind them
+template <typename T, int NV> __device__ __forceinline__ RawVec<T, NV> load_some(const T* p, int have) {
+  if (have >= NV) return load_raw<T, NV>(p);
+  RawVec<T, NV> r;
   #pragma unroll
-  for (int j = 0; j < NV; ++j) v[j] = j < have ? load1(base + at + j) : 0.f;
-  return have;
+  for (int j = 0; j < NV; ++j) r.h[j] = 0;
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) if (j < have) __builtin_memcpy(&r.h[j], p + j, sizeof(T));
+  return r;
 }
-template <typename T, int NV>
-__device__ __forceinline__ void store_piece(T* base, long long at, int have, const float (&v)[NV]) {
-  if (have == NV) { store_vec<T, NV>(base + at, v); return; }
+template <typename T, int NV> __device__ __forceinline__ void store_some(T* p, int have, const float (&v)[NV]) {
+  if (have >= NV) { store_vec<T, NV>(p, v); return; }
   #pragma unroll
-  for (int j = 0; j < NV; ++j) if (j < have) store1(base + at + j, v[j]);
+  for (int j = 0; j < NV; ++j) if (j < have) store1(p + j, v[j]);
 }
 
-// NV decoded values of the 8-bit form; aligned (C % 32 == 0 or C % NV == 0): the piece lies in one block of one pixel
-template <int NV>
-__device__ __forceinline__ int load_codes(const Params& p, int n, long long at, bool one_block, float (&v)[NV]) {
-  const signed char* c = p.codes + (long long)n * p.E;
-  const long long pix0 = (long long)n * (p.E / p.C);
-  if (one_block && at + NV <= p.E) {
-    signed char q[NV];
-    __builtin_memcpy(q, c + at, NV);
-    const long long pix = at / p.C;
-    const float s = c8_scale(p.exps[(pix0 + pix) * p.nblk + (int)(at - pix * p.C) / C8_BLOCK]);
+// ---- where x comes from: itself, or its 8-bit form ------------------------------------------------------------------
+// A source hands out raw pieces (so that several loads are in flight) and turns them into floats.  EVEN: C is a multiple of
+// the piece, so a row is a pixel and a piece lies in one block of 32 channels.
+template <typename T, int NV, bool EVEN> struct Source {
+  typedef RawVec<T, NV> Raw;
+  const T* x;
+  int q0, L;
+  __device__ __forceinline__ Source(const Params& p, int n, int q0_) : x(reinterpret_cast<const T*>(p.x) + (long long)n * p.E + q0_), q0(q0_), L(p.L) {}
+  __device__ __forceinline__ Raw load(const Params&, int row) const { return load_raw<T, NV>(x + (long long)row * L); }
+  __device__ __forceinline__ Raw load_tail(const Params&, int row, int have) const { return load_some<T, NV>(x + (long long)row * L, have); }
+  static __device__ __forceinline__ void values(const Raw& r, float (&v)[NV]) { widen(r, v); }
+};
+template <int NV> struct RawCodes { signed char q[NV]; unsigned char e[NV]; };
+template <int NV> struct RawCodes1 { signed char q[NV]; unsigned char e; };
+template <int NV> struct Source<signed char, NV, true> {
+  typedef RawCodes1<NV> Raw;
+  const signed char* c;
+  const unsigned char* e;
+  int L;
+  __device__ __forceinline__ Source(const Params& p, int n, int q0)
+    : c(p.codes + (long long)n * p.E + q0), e(p.exps + (long long)n * (p.E / p.C) * p.nblk + q0 / C8_BLOCK), L(p.L) {}
+  __device__ __forceinline__ Raw load(const Params& p, int row) const {
+    Raw r;
+    __builtin_memcpy(r.q, c + (long long)row * L, NV);
+    r.e = e[(long long)row * p.nblk];
+    return r;
+  }
+  __device__ __forceinline__ Raw load_tail(const Params& p, int row, int) const { return load(p, row); }    // (no partial piece)
+  static __device__ __forceinline__ void values(const Raw& r, float (&v)[NV]) {
+    const float s = c8_scale(r.e);
     #pragma unroll
-    for (int j = 0; j < NV; ++j) v[j] = c8_decode(q[j], s);
-    return NV;
+    for (int j = 0; j < NV; ++j) v[j] = c8_decode(r.q[j], s);
   }
-  const int have = at + NV <= p.E ? NV : at < p.E ? (int)(p.E - at) : 0;
-  #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    v[j] = 0.f;
-    if (j < have) {
-      const long long pix = (at + j) / p.C;
-      v[j] = c8_decode(c[at + j], c8_scale(p.exps[(pix0 + pix) * p.nblk + (int)(at + j - pix * p.C) / C8_BLOCK]));
-    }
+};
+template <int NV> struct Source<signed char, NV, false> {
+  typedef RawCodes<NV> Raw;
+  const signed char* c;
+  const unsigned char* e;
+  int L, per;                          // pixels per row
+  int at[NV];                          // exponent of position j, from the row's first pixel
+  __device__ __forceinline__ Source(const Params& p, int n, int q0)
+    : c(p.codes + (long long)n * p.E + q0), e(p.exps + (long long)n * (p.E / p.C) * p.nblk), L(p.L), per(p.L / p.C) {
+    #pragma unroll
+    for (int j = 0; j < NV; ++j) { const int pix = (q0 + j) / p.C; at[j] = pix * p.nblk + (q0 + j - pix * p.C) / C8_BLOCK; }
   }
-  return have;
+  __device__ __forceinline__ Raw load(const Params& p, int row) const {
+    Raw r;
+    __builtin_memcpy(r.q, c + (long long)row * L, NV);
+    const unsigned char* er = e + (long long)row * per * p.nblk;
+    #pragma unroll
+    for (int j = 0; j < NV; ++j) r.e[j] = er[at[j]];
+    return r;
+  }
+  __device__ __forceinline__ Raw load_tail(const Params& p, int row, int have) const {
+    if (have >= NV) return load(p, row);
+    Raw r;
+    const unsigned char* er = e + (long long)row * per * p.nblk;
+    #pragma unroll
+    for (int j = 0; j < NV; ++j) { r.q[j] = 0; r.e[j] = 127; }
+    #pragma unroll
+    for (int j = 0; j < NV; ++j) if (j < have) { r.q[j] = c[(long long)row * L + j]; r.e[j] = er[at[j]]; }
+    return r;
+  }
+  static __device__ __forceinline__ void values(const Raw& r, float (&v)[NV]) {
+    #pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = c8_decode(r.q[j], c8_scale(r.e[j]));
+  }
+};
+
+// f over this lane's rows: U at a time where the image has all of a piece, the rest one by one (a partial piece only in the
+// image's last row)
+template <int U, typename F, typename H>
+__device__ __forceinline__ void each_row(const Params& p, const Place& w, int NV, F batch, H tail) {
+  const int end = min(w.row1, p.full_rows);
+  int r = w.row0 + w.pl;
+  for (; r + (U - 1) * p.TP < end; r += U * p.TP) batch(r);
+  for (; r < w.row1; r += p.TP) {
+    const long long left = p.E - (long long)r * p.L - w.q0;
+    if (left > 0) tail(r, left < NV ? (int)left : NV);
+  }
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------
 
+// sums over the pixel lanes of NV values per thread: out(position of the slab, sum); buf: THREADS * NV values
+template <typename V, int NV, typename F>
+__device__ __forceinline__ void sum_pixel_lanes(const V (&s)[NV], V* buf, int TV, int TP, int pl, F out) {
+  if (pl < TP) {
+    #pragma unroll
+    for (int j = 0; j < NV; ++j) buf[threadIdx.x * NV + j] = s[j];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < TV * NV; i += blockDim.x) {
+    double a = 0.0;
+    for (int t = 0; t < TP; ++t) a += buf[t * TV * NV + i];
+    out(i, a);
+  }
+  __syncthreads();
+}
+
 // sums of x and x^2 of every position over a chunk of rows
 template <typename TX>
 __global__ __launch_bounds__(THREADS) void fwd_partial_kernel(const Params p) {
-  constexpr int NV = VecOf<TX>::n;
-  __shared__ double red[THREADS * NV];
+  constexpr int NV = VecOf<TX>::n, U = 4;
+  __shared__ double buf[THREADS * NV];
   const Place w = place_of(p, NV, blockIdx.x);
-  const TX* x = reinterpret_cast<const TX*>(p.x) + (long long)w.n * p.E;
   double s[NV], q[NV];
   #pragma unroll
   for (int j = 0; j < NV; ++j) s[j] = q[j] = 0.0;
   if (w.on) {
-    #pragma unroll 4
-    for (int r = w.row0 + w.pl; r < w.row1; r += p.TP) {
+    const Source<TX, NV, true> src(p, w.n, w.q0);
+    auto add = [&](const RawVec<TX, NV>& raw) {
       float v[NV];
-      load_piece<TX, NV>(x, (long long)r * p.L + w.q0, p.E, v);      // (what is behind the image reads as 0)
+      widen(raw, v);
       #pragma unroll
       for (int j = 0; j < NV; ++j) { const double d = v[j]; s[j] += d; q[j] = fma(d, d, q[j]); }
-    }
+    };
+    each_row<U>(p, w, NV,
+      [&](int r) {
+        RawVec<TX, NV> raw[U];
+        #pragma unroll
+        for (int k = 0; k < U; ++k) raw[k] = src.load(p, r + k * p.TP);
+        #pragma unroll
+        for (int k = 0; k < U; ++k) add(raw[k]);
+      },
+      [&](int r, int have) { add(src.load_tail(p, r, have)); });          // (what is behind the image reads as 0)
   }
   double* out = reinterpret_cast<double*>(p.part) + ((long long)w.n * p.chunks + w.row0 / p.rows_per_chunk) * 2 * p.L;
-  for (int k = 0; k < 2; ++k) {
-    if (k) __syncthreads();
-    if (w.pl < p.TP) {
-      #pragma unroll
-      for (int j = 0; j < NV; ++j) red[threadIdx.x * NV + j] = k ? q[j] : s[j];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < p.TV * NV; i += THREADS) {
-      const int pos = (w.q0 - (int)(threadIdx.x % p.TV) * NV) + i;
-      if (pos < p.L) {
-        double a = 0.0;
-        for (int t = 0; t < p.TP; ++t) a += red[t * p.TV * NV + i];
-        out[(long long)k * p.L + pos] = a;
-      }
-    }
-  }
+  const int base = w.q0 - (int)(threadIdx.x % p.TV) * NV;
+  sum_pixel_lanes<double, NV>(s, buf, p.TV, p.TP, w.pl, [&](int i, double a) { if (base + i < p.L) out[base + i] = a; });
+  sum_pixel_lanes<double, NV>(q, buf, p.TV, p.TP, w.pl, [&](int i, double a) { if (base + i < p.L) out[p.L + base + i] = a; });
 }
 
 __device__ __forceinline__ void block_sum2(double& a, double& b, double (*red)[2]) {
@@ -156,6 +224,14 @@ __device__ __forceinline__ void block_sum2(double& a, double& b, double (*red)[2
   for (int i = 0; i < waves; ++i) { a += red[i][0]; b += red[i][1]; }
 }
 
+__device__ __forceinline__ void write_stats(const Params& p, long long group, double s, double q) {
+  const double cnt = (double)(p.E / p.C) * p.D, mean = s / cnt;
+  double var = q / cnt - mean * mean;
+  if (var < 0.0) var = 0.0;                                        // (a NaN stays one)
+  p.stats[group * 2] = mean;
+  p.stats[group * 2 + 1] = 1.0 / sqrt(var + (double)p.eps);
+}
+
 // one workgroup per (image, group): the chunks' sums joined in a fixed order
 __global__ __launch_bounds__(1024) void fwd_finish_kernel(const Params p) {
   __shared__ double red[16][2];
@@ -165,29 +241,19 @@ __global__ __launch_bounds__(1024) void fwd_finish_kernel(const Params p) {
   const int reps = p.L / p.C, per = reps * p.D;
   const double* part = reinterpret_cast<const double*>(p.part) + n * p.chunks * 2 * p.L;
   double s = 0.0, q = 0.0;
-  for (long long i = threadIdx.x; i < (long long)p.chunks * per; i += blockDim.x) {
-    const long long chunk = i / per;
-    const int k = (int)(i - chunk * per), rep = k / p.D;
-    const long long at = chunk * 2 * p.L + rep * p.C + g * p.D + (k - rep * p.D);
+  for (int i = threadIdx.x; i < p.chunks * per; i += blockDim.x) {
+    const int chunk = i / per, k = i - chunk * per, rep = k / p.D;
+    const long long at = (long long)chunk * 2 * p.L + rep * p.C + g * p.D + (k - rep * p.D);
     s += part[at];
     q += part[at + p.L];
   }
   block_sum2(s, q, red);
-  if (threadIdx.x == 0) {
-    const double cnt = (double)(p.E / p.C) * p.D, mean = s / cnt;
-    double var = q / cnt - mean * mean;
-    if (var < 0.0) var = 0.0;                                        // (a NaN stays one)
-    p.stats[b * 2] = mean;
-    p.stats[b * 2 + 1] = 1.0 / sqrt(var + (double)p.eps);
-  }
+  if (threadIdx.x == 0) write_stats(p, b, s, q);
 }
 
 // a position's affine: z = fma(x - m, a, b) with m = float(mean), the difference of the two means in b
 struct Affine { float m, a, b; };
-__device__ __forceinline__ Affine affine_of(const Params& p, int n, int pos) {
-  const int c = pos % p.C;
-  const double* st = p.stats + ((long long)n * p.G + c / p.D) * 2;
-  const double mean = st[0], rstd = st[1];
+__device__ __forceinline__ Affine affine_of(const Params& p, int c, double mean, double rstd) {
   const double ga = p.gamma ? load_param(p.gamma, p.param_bf16, c) : 1.0;
   const double be = p.beta ? load_param(p.beta, p.param_bf16, c) : 0.0;
   Affine f;
@@ -196,109 +262,158 @@ __device__ __forceinline__ Affine affine_of(const Params& p, int n, int pos) {
   f.b = (float)(be + ((double)f.m - mean) * ga * rstd);
   return f;
 }
+__device__ __forceinline__ Affine affine_at(const Params& p, int n, int pos) {
+  const int c = pos % p.C;
+  const double* st = p.stats + ((long long)n * p.G + c / p.D) * 2;
+  return affine_of(p, c, st[0], st[1]);
+}
 
-template <typename TX, typename TY>
+template <int NV>
+__device__ __forceinline__ void forward_values(float (&v)[NV], const Affine (&f)[NV], float slope) {
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const float z = fmaf(v[j] - f[j].m, f[j].a, f[j].b);
+    v[j] = z > 0.f ? z : z * slope;
+  }
+}
+
+// the 8-bit form of a piece (C % 32 == 0: a block is 32 / NV neighbouring lanes of one wave, all of them active)
+template <int NV>
+__device__ __forceinline__ void write_codes(const Params& p, int n, int row, int q0, const float (&v)[NV]) {
+  float top = 0.f;
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) top = fmaxf(top, c8_magnitude(v[j]));
+  #pragma unroll
+  for (int o = 1; o < C8_BLOCK / NV; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const int e = c8_exponent(top);
+  const float inv = c8_inverse(e);
+  signed char c[NV];
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) c[j] = c8_encode(v[j], inv);
+  const long long pix = (long long)n * p.rows + row;
+  __builtin_memcpy(p.codes_out + pix * p.C + q0, c, NV);
+  if (q0 % C8_BLOCK == 0) p.exps_out[pix * p.nblk + q0 / C8_BLOCK] = (unsigned char)e;
+}
+
+template <typename TX, typename TY, bool PACK>
 __global__ __launch_bounds__(THREADS) void fwd_apply_kernel(const Params p) {
-  constexpr int NV = VecOf<TX>::n;
+  constexpr int NV = VecOf<TX>::n, U = 4;
   const Place w = place_of(p, NV, blockIdx.x);
   if (!w.on) return;
-  const TX* x = reinterpret_cast<const TX*>(p.x) + (long long)w.n * p.E;
-  TY* y = reinterpret_cast<TY*>(p.out) + (long long)w.n * p.E;
+  const Source<TX, NV, true> src(p, w.n, w.q0);
+  TY* y = reinterpret_cast<TY*>(p.out) + (long long)w.n * p.E + w.q0;
   Affine f[NV];
   #pragma unroll
-  for (int j = 0; j < NV; ++j) f[j] = affine_of(p, w.n, w.q0 + j);
-  #pragma unroll 4
-  for (int r = w.row0 + w.pl; r < w.row1; r += p.TP) {
-    const long long at = (long long)r * p.L + w.q0;
-    float v[NV];
-    const int have = load_piece<TX, NV>(x, at, p.E, v);
-    #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const float z = fmaf(v[j] - f[j].m, f[j].a, f[j].b);
-      v[j] = z > 0.f ? z : z * p.slope;
-    }
-    store_piece<TY, NV>(y, at, have, v);
-  }
+  for (int j = 0; j < NV; ++j) f[j] = affine_at(p, w.n, w.q0 + j);
+  each_row<U>(p, w, NV,
+    [&](int r) {
+      RawVec<TX, NV> raw[U];
+      #pragma unroll
+      for (int k = 0; k < U; ++k) raw[k] = src.load(p, r + k * p.TP);
+      #pragma unroll
+      for (int k = 0; k < U; ++k) {
+        float v[NV];
+        widen(raw[k], v);
+        if constexpr (PACK) write_codes<NV>(p, w.n, r + k * p.TP, w.q0, v);
+        forward_values<NV>(v, f, p.slope);
+        store_vec<TY, NV>(y + (long long)(r + k * p.TP) * p.L, v);
+      }
+    },
+    [&](int r, int have) {
+      float v[NV];
+      widen(src.load_tail(p, r, have), v);
+      if constexpr (PACK) write_codes<NV>(p, w.n, r, w.q0, v);
+      forward_values<NV>(v, f, p.slope);
+      store_some<TY, NV>(y + (long long)r * p.L, have, v);
+    });
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
 
-// SRC: the type x is read in - float, bf16_s, or signed char for its 8-bit form
-template <typename SRC, int NV>
-__device__ __forceinline__ int load_x(const Params& p, int n, long long at, bool one_block, float (&v)[NV]) {
-  if constexpr (sizeof(SRC) == 1) return load_codes<NV>(p, n, at, one_block, v);
-  else return load_piece<SRC, NV>(reinterpret_cast<const SRC*>(p.x) + (long long)n * p.E, at, p.E, v);
+// Which side of the kink: z > 0 with z = fma(x - m, a, b) where |z| is above `tol`, else decided in 64 bits.  Near zero the
+// product is as large as b, so 1e-6 |b| covers its three roundings (2^-24 each); a lane uses the largest of its b.
+template <int NV>
+__device__ __forceinline__ float kink_tolerance(const Affine (&f)[NV], float slope) {
+  float t = 0.f;
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) t = fmaxf(t, fabsf(f[j].b));
+  return slope == 1.f ? -1.f : 1e-6f * t;
 }
-
-struct Back { float m, rs, k, a, b, tol; };      // xh = fma(x - m, rs, k);  z = fma(x - m, a, b)
-__device__ __forceinline__ Back back_of(const Params& p, int n, int pos) {
-  const double* st = p.stats + ((long long)n * p.G + pos % p.C / p.D) * 2;
-  const Affine f = affine_of(p, n, pos);
-  Back q;
-  q.m = f.m; q.a = f.a; q.b = f.b;
-  q.rs = (float)st[1];
-  q.k = (float)(((double)f.m - st[0]) * st[1]);
-  // |z| below this: the rounding of the two products (2^-24 each, of terms as large as b where z is near 0) may decide
-  q.tol = p.slope == 1.f ? -1.f : 1e-6f * fabsf(f.b);
-  return q;
-}
-__device__ __forceinline__ bool above_zero(const Params& p, const Back& f, int n, int pos, float x, float z) {
-  if (fabsf(z) > f.tol) return z > 0.f;
+__device__ __forceinline__ bool above_zero_64(const Params& p, int n, int pos, float x) {
   const int c = pos % p.C;
   const double* st = p.stats + ((long long)n * p.G + c / p.D) * 2;
   const double ga = p.gamma ? load_param(p.gamma, p.param_bf16, c) : 1.0;
   const double be = p.beta ? load_param(p.beta, p.param_bf16, c) : 0.0;
   return fma((double)x - st[0], ga * st[1], be) > 0.0;
 }
+// g: dy -> dz, v: x -> x - m
+template <int NV>
+__device__ __forceinline__ void back_values(const Params& p, int n, int q0, float (&v)[NV], float (&g)[NV], const Affine (&f)[NV], float tol) {
+  float z[NV], low = 3.4e38f;
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    z[j] = fmaf(v[j] - f[j].m, f[j].a, f[j].b);
+    low = fminf(low, fabsf(z[j]));
+  }
+  if (low <= tol) {
+    int pos = q0;
+    asm volatile("" : "+v"(pos));          // (keeps what only this rare branch reads from being held through the loop)
+    #pragma unroll
+    for (int j = 0; j < NV; ++j) if (fabsf(z[j]) <= tol) z[j] = above_zero_64(p, n, pos + j, v[j]) ? 1.f : -1.f;
+  }
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    g[j] = z[j] > 0.f ? g[j] : g[j] * p.slope;
+    v[j] -= f[j].m;
+  }
+}
 
-// sums of dz and dz xh of every position over a chunk of rows
-template <typename SRC, typename TX, typename TY>
+// sums of dz and dz (x - m) of every position over a chunk of rows
+template <typename SRC, typename TX, typename TY, bool EVEN>
 __global__ __launch_bounds__(THREADS) void bwd_partial_kernel(const Params p) {
-  constexpr int NV = VecOf<TX>::n;
-  __shared__ float red[THREADS * NV];
+  constexpr int NV = VecOf<TX>::n, U = 2;
+  __shared__ float buf[THREADS * NV];
   const Place w = place_of(p, NV, blockIdx.x);
-  const TY* dy = reinterpret_cast<const TY*>(p.dy) + (long long)w.n * p.E;
-  const bool one_block = p.C % NV == 0;
   float s[NV], q[NV];
   #pragma unroll
   for (int j = 0; j < NV; ++j) s[j] = q[j] = 0.f;
   if (w.on) {
-    Back f[NV];
+    typedef Source<SRC, NV, EVEN> X;
+    const X src(p, w.n, w.q0);
+    const TY* dy = reinterpret_cast<const TY*>(p.dy) + (long long)w.n * p.E + w.q0;
+    Affine f[NV];
     #pragma unroll
-    for (int j = 0; j < NV; ++j) f[j] = back_of(p, w.n, w.q0 + j);
-    #pragma unroll 2
-    for (int r = w.row0 + w.pl; r < w.row1; r += p.TP) {
-      const long long at = (long long)r * p.L + w.q0;
+    for (int j = 0; j < NV; ++j) f[j] = affine_at(p, w.n, w.q0 + j);
+    const float tol = kink_tolerance<NV>(f, p.slope);
+    auto add = [&](const typename X::Raw& rx, const RawVec<TY, NV>& rg) {
       float v[NV], g[NV];
-      const int have = load_x<SRC, NV>(p, w.n, at, one_block, v);
-      load_piece<TY, NV>(dy, at, p.E, g);
+      X::values(rx, v);
+      widen(rg, g);
+      back_values<NV>(p, w.n, w.q0, v, g, f, tol);
       #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (j >= have) break;
-        const float d = v[j] - f[j].m, z = fmaf(d, f[j].a, f[j].b);
-        const float dz = above_zero(p, f[j], w.n, w.q0 + j, v[j], z) ? g[j] : g[j] * p.slope;
-        s[j] += dz;
-        q[j] = fmaf(dz, fmaf(d, f[j].rs, f[j].k), q[j]);
-      }
-    }
+      for (int j = 0; j < NV; ++j) { s[j] += g[j]; q[j] = fmaf(g[j], v[j], q[j]); }
+    };
+    each_row<U>(p, w, NV,
+      [&](int r) {
+        typename X::Raw rx[U];
+        RawVec<TY, NV> rg[U];
+        #pragma unroll
+        for (int k = 0; k < U; ++k) { rx[k] = src.load(p, r + k * p.TP); rg[k] = load_raw<TY, NV>(dy + (long long)(r + k * p.TP) * p.L); }
+        #pragma unroll
+        for (int k = 0; k < U; ++k) add(rx[k], rg[k]);
+      },
+      // (behind the image dy reads as 0, and 0 times a finite x - m adds nothing)
+      [&](int r, int have) { add(src.load_tail(p, r, have), load_some<TY, NV>(dy + (long long)r * p.L, have)); });
   }
   float* out = reinterpret_cast<float*>(p.part) + ((long long)w.n * p.chunks + w.row0 / p.rows_per_chunk) * 2 * p.L;
-  for (int k = 0; k < 2; ++k) {
-    if (k) __syncthreads();
-    if (w.pl < p.TP) {
-      #pragma unroll
-      for (int j = 0; j < NV; ++j) red[threadIdx.x * NV + j] = k ? q[j] : s[j];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < p.TV * NV; i += THREADS) {
-      const int pos = (w.q0 - (int)(threadIdx.x % p.TV) * NV) + i;
-      if (pos < p.L) {
-        double a = 0.0;
-        for (int t = 0; t < p.TP; ++t) a += red[t * p.TV * NV + i];
-        out[(long long)k * p.L + pos] = (float)a;
-      }
-    }
-  }
+  const int base = w.q0 - (int)(threadIdx.x % p.TV) * NV;
+  sum_pixel_lanes<float, NV>(s, buf, p.TV, p.TP, w.pl, [&](int i, double a) { if (base + i < p.L) out[base + i] = (float)a; });
+  sum_pixel_lanes<float, NV>(q, buf, p.TV, p.TP, w.pl, [&](int i, double a) { if (base + i < p.L) out[p.L + base + i] = (float)a; });
+}
+
+// a channel's sum of dz xh from those of dz (x - m) and dz:  xh = (x - m) rstd + (m - mean) rstd
+__device__ __forceinline__ double sum_xh(const double* st, double s, double q) {
+  return st[1] * (q + ((double)(float)st[0] - st[0]) * s);
 }
 
 // one workgroup per (image, run of whole groups of at least 64 channels or one group): 64 channel lanes x 16 chunk lanes
@@ -329,10 +444,14 @@ __global__ __launch_bounds__(FIN_CH * FIN_LANES) void bwd_finish_kernel(const Pa
     if (lane == 0) {
       s = q = 0.0;
       for (int i = 0; i < FIN_LANES; ++i) { s += red[i][cl][0]; q += red[i][cl][1]; }
-      if (c < c1) { p.chan[(n * p.C + c) * 2] = s; p.chan[(n * p.C + c) * 2 + 1] = q; }
-      const double ga = c < c1 ? (p.gamma ? load_param(p.gamma, p.param_bf16, c) : 1.0) : 0.0;
-      sums[cl][0] = ga * s; sums[cl][1] = ga * q;
-      if (c >= c1) sums[cl][0] = sums[cl][1] = 0.0;
+      double ga = 0.0;
+      if (c < c1) {
+        q = sum_xh(p.stats + (n * p.G + c / p.D) * 2, s, q);
+        p.chan[(n * p.C + c) * 2] = s;
+        p.chan[(n * p.C + c) * 2 + 1] = q;
+        ga = p.gamma ? load_param(p.gamma, p.param_bf16, c) : 1.0;
+        sums[cl][0] = ga * s; sums[cl][1] = ga * q;
+      } else sums[cl][0] = sums[cl][1] = 0.0;
     }
     __syncthreads();
     if (p.D <= FIN_CH) {                                 // whole groups in this (only) block of channels
@@ -372,111 +491,153 @@ __device__ __forceinline__ void param_grads(const Params& p, int block) {
 
 __global__ __launch_bounds__(THREADS) void param_grads_kernel(const Params p) { param_grads(p, blockIdx.x); }
 
-template <typename SRC, typename TX, typename TY>
+// dx = rstd (weight dz - m1 - xh m2) = a dz - c0 - c1 (x - m) with c1 = rstd^2 m2, c0 = rstd m1 + (m - mean) c1
+struct DxCoef { float c0, c1; };
+__device__ __forceinline__ DxCoef dx_coef(double mean, double rstd, double m1, double m2) {
+  DxCoef k;
+  const double c1 = rstd * rstd * m2;
+  k.c1 = (float)c1;
+  k.c0 = (float)(rstd * m1 + ((double)(float)mean - mean) * c1);
+  return k;
+}
+
+template <typename SRC, typename TX, typename TY, bool EVEN>
 __global__ __launch_bounds__(THREADS) void bwd_apply_kernel(const Params p, long long main_blocks) {
-  constexpr int NV = VecOf<TX>::n;
+  constexpr int NV = VecOf<TX>::n, U = 2;
   if ((long long)blockIdx.x >= main_blocks) { param_grads(p, (int)(blockIdx.x - main_blocks)); return; }
   const Place w = place_of(p, NV, blockIdx.x);
   if (!w.on) return;
-  const TY* dy = reinterpret_cast<const TY*>(p.dy) + (long long)w.n * p.E;
-  TX* dx = reinterpret_cast<TX*>(p.out) + (long long)w.n * p.E;
-  const bool one_block = p.C % NV == 0;
-  Back f[NV];
-  float ga[NV], m1[NV], m2[NV];
+  typedef Source<SRC, NV, EVEN> X;
+  const X src(p, w.n, w.q0);
+  const TY* dy = reinterpret_cast<const TY*>(p.dy) + (long long)w.n * p.E + w.q0;
+  TX* dx = reinterpret_cast<TX*>(p.out) + (long long)w.n * p.E + w.q0;
+  Affine f[NV];
+  DxCoef k[NV];
   #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = (w.q0 + j) % p.C;
-    f[j] = back_of(p, w.n, w.q0 + j);
-    ga[j] = p.gamma ? load_param(p.gamma, p.param_bf16, c) : 1.f;
-    m1[j] = p.coef[((long long)w.n * p.G + c / p.D) * 2];
-    m2[j] = p.coef[((long long)w.n * p.G + c / p.D) * 2 + 1];
+    const long long g = (long long)w.n * p.G + (w.q0 + j) % p.C / p.D;
+    f[j] = affine_at(p, w.n, w.q0 + j);
+    k[j] = dx_coef(p.stats[g * 2], p.stats[g * 2 + 1], p.coef[g * 2], p.coef[g * 2 + 1]);
   }
-  #pragma unroll 2
-  for (int r = w.row0 + w.pl; r < w.row1; r += p.TP) {
-    const long long at = (long long)r * p.L + w.q0;
-    float v[NV], g[NV];
-    const int have = load_x<SRC, NV>(p, w.n, at, one_block, v);
-    load_piece<TY, NV>(dy, at, p.E, g);
+  const float tol = kink_tolerance<NV>(f, p.slope);
+  auto one = [&](const typename X::Raw& rx, const RawVec<TY, NV>& rg, float (&v)[NV]) {
+    float g[NV];
+    X::values(rx, v);
+    widen(rg, g);
+    back_values<NV>(p, w.n, w.q0, v, g, f, tol);
     #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const float d = v[j] - f[j].m, z = fmaf(d, f[j].a, f[j].b), xh = fmaf(d, f[j].rs, f[j].k);
-      const float dz = above_zero(p, f[j], w.n, w.q0 + j, v[j], z) ? g[j] : g[j] * p.slope;
-      v[j] = f[j].rs * (fmaf(dz, ga[j], -m1[j]) - xh * m2[j]);
-    }
-    store_piece<TX, NV>(dx, at, have, v);
-  }
+    for (int j = 0; j < NV; ++j) v[j] = fmaf(g[j], f[j].a, -fmaf(v[j], k[j].c1, k[j].c0));
+  };
+  each_row<U>(p, w, NV,
+    [&](int r) {
+      typename X::Raw rx[U];
+      RawVec<TY, NV> rg[U];
+      #pragma unroll
+      for (int u = 0; u < U; ++u) { rx[u] = src.load(p, r + u * p.TP); rg[u] = load_raw<TY, NV>(dy + (long long)(r + u * p.TP) * p.L); }
+      #pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float v[NV];
+        one(rx[u], rg[u], v);
+        store_vec<TX, NV>(dx + (long long)(r + u * p.TP) * p.L, v);
+      }
+    },
+    [&](int r, int have) {
+      float v[NV];
+      one(src.load_tail(p, r, have), load_some<TY, NV>(dy + (long long)r * p.L, have), v);
+      store_some<TX, NV>(dx + (long long)r * p.L, have, v);
+    });
 }
 
 // ---- the 8-bit form on its own ------------------------------------------------------------------------------------
 
-// 8 lanes per block of 32 channels, 4 elements each
+// A lane takes one 16-byte piece of x; 4 (bfloat16) or 8 (float) neighbouring lanes make a block of 32 channels.  Pieces are
+// numbered along the rows, so that a wave walks memory in order; U of them are in flight per lane.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void pack8_kernel(const T* __restrict__ x, long long rows, int C, int nblk, long long ld,
                                                         signed char* __restrict__ codes, unsigned char* __restrict__ exps) {
-  const long long blocks = rows * nblk, per = (long long)gridDim.x * (THREADS / 8);
-  const int sub = threadIdx.x & 7;
-  for (long long b0 = (long long)blockIdx.x * (THREADS / 8); b0 < blocks; b0 += per) {
-    const long long b = b0 + (threadIdx.x >> 3);
-    const bool on = b < blocks;
-    const long long row = on ? b / nblk : 0;
-    const int blk = (int)(b - row * nblk), c = blk * C8_BLOCK + sub * 4;
-    const int have = on ? min(4, max(0, C - c)) : 0;
-    float v[4];
-    const T* src = x + row * ld + c;
-    if (have == 4) load_vec<T, 4>(src, v);
-    else {
-      #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = j < have ? load1(src + j) : 0.f;
-    }
-    float top = fmaxf(fmaxf(c8_magnitude(v[0]), c8_magnitude(v[1])), fmaxf(c8_magnitude(v[2]), c8_magnitude(v[3])));
+  constexpr int NV = VecOf<T>::n, LANES = C8_BLOCK / NV, U = 4;
+  const int per_row = nblk * LANES;
+  const long long pieces = rows * per_row, step = (long long)gridDim.x * THREADS;
+  for (long long i0 = (long long)blockIdx.x * THREADS + threadIdx.x; i0 - threadIdx.x < pieces; i0 += U * step) {
+    RawVec<T, NV> raw[U];
+    long long row[U];
+    int c[U];
     #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const int e = c8_exponent(top);
-    const float inv = c8_inverse(e);
-    signed char q[4];
-    #pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = c8_encode(v[j], inv);
-    signed char* dst = codes + row * C + c;
-    if (have == 4) __builtin_memcpy(dst, q, 4);
-    else {
-      #pragma unroll
-      for (int j = 0; j < 4; ++j) if (j < have) dst[j] = q[j];
+    for (int k = 0; k < U; ++k) {
+      const long long i = i0 + k * step;
+      const bool on = i < pieces;
+      row[k] = !on ? 0 : pieces <= 0x7fffffffLL ? (long long)((unsigned)i / (unsigned)per_row) : i / per_row;
+      c[k] = on ? (int)(i - row[k] * per_row) * NV : C;
+      raw[k] = load_some<T, NV>(x + row[k] * ld + c[k], C - c[k]);
     }
-    if (on && sub == 0) exps[b] = (unsigned char)e;
+    #pragma unroll
+    for (int k = 0; k < U; ++k) {
+      float v[NV], top = 0.f;
+      widen(raw[k], v);
+      #pragma unroll
+      for (int j = 0; j < NV; ++j) top = fmaxf(top, c8_magnitude(v[j]));
+      #pragma unroll
+      for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+      const int e = c8_exponent(top), have = C - c[k];
+      const float inv = c8_inverse(e);
+      signed char q[NV];
+      #pragma unroll
+      for (int j = 0; j < NV; ++j) q[j] = c8_encode(v[j], inv);
+      signed char* dst = codes + row[k] * C + c[k];
+      if (have >= NV) __builtin_memcpy(dst, q, NV);
+      else {
+        #pragma unroll
+        for (int j = 0; j < NV; ++j) if (j < have) dst[j] = q[j];
+      }
+      if (i0 + k * step < pieces && c[k] % C8_BLOCK == 0) exps[row[k] * nblk + c[k] / C8_BLOCK] = (unsigned char)e;
+    }
   }
 }
 
 template <typename T>
 __global__ __launch_bounds__(THREADS) void unpack8_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ exps,
                                                           long long rows, int C, int nblk, T* __restrict__ out, long long ld) {
-  const int pieces = nblk * 8;
-  const long long total = rows * pieces;
-  for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * THREADS) {
-    const long long row = i / pieces;
-    const int piece = (int)(i - row * pieces), c = piece * 4, have = min(4, C - c);
-    if (have <= 0) continue;
-    const float s = c8_scale(exps[row * nblk + (piece >> 3)]);
-    const signed char* src = codes + row * C + c;
-    T* dst = out + row * ld + c;
-    if (have == 4) {
-      signed char q[4];
-      __builtin_memcpy(q, src, 4);
-      float v[4];
+  constexpr int NV = VecOf<T>::n, U = 4;
+  const int per_row = (C + NV - 1) / NV;
+  const long long pieces = rows * per_row, step = (long long)gridDim.x * THREADS;
+  for (long long i0 = (long long)blockIdx.x * THREADS + threadIdx.x; i0 < pieces; i0 += U * step) {
+    signed char q[U][NV];
+    unsigned char e[U];
+    long long row[U];
+    int c[U];
+    #pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const long long i = i0 + k * step < pieces ? i0 + k * step : i0;      // (behind the end: the first piece once more)
+      row[k] = pieces <= 0x7fffffffLL ? (long long)((unsigned)i / (unsigned)per_row) : i / per_row;
+      c[k] = (int)(i - row[k] * per_row) * NV;
+      const signed char* src = codes + row[k] * C + c[k];
+      if (C - c[k] >= NV) __builtin_memcpy(q[k], src, NV);
+      else {
+        #pragma unroll
+        for (int j = 0; j < NV; ++j) q[k][j] = j < C - c[k] ? src[j] : 0;
+      }
+      e[k] = exps[row[k] * nblk + c[k] / C8_BLOCK];
+    }
+    #pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const float s = c8_scale(e[k]);
+      float v[NV];
       #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = c8_decode(q[j], s);
-      store_vec<T, 4>(dst, v);
-    } else {
-      for (int j = 0; j < have; ++j) store1(dst + j, c8_decode(src[j], s));
+      for (int j = 0; j < NV; ++j) v[j] = c8_decode(q[k][j], s);
+      store_some<T, NV>(out + row[k] * ld + c[k], C - c[k], v);
     }
   }
 }
+
+// workgroups of the two kernels above: U pieces per lane, and no more than 16 workgroups per CU
+unsigned piece_blocks(long long pieces) { return (unsigned)std::max(1LL, std::min((pieces + 4 * THREADS - 1) / (4 * THREADS), 4096LL)); }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
-// How an image is cut: slabs of at most 64 pieces across a row, and chunks of rows so that there are about 2 048
-// workgroups (8 per CU) - but never less than four rows per lane, where a workgroup would be all set-up.
+// How an image is cut: slabs of at most 64 pieces across a row, and chunks of rows so that there are about 1 024
+// workgroups (4 per CU; 2 048 and more cost 3 % and up on the largest map, in partial sums) - but never less than four rows per lane, where a workgroup would be all set-up.
 bool cut(Params& p, int N, long long hw, int C, int G, int x_bf16) {
   const int nv = x_bf16 ? 8 : 4;
   if ((long long)C * nv > 0x7fffffffLL || hw > 0x7fffffffLL / 2) return false;
@@ -486,13 +647,14 @@ bool cut(Params& p, int N, long long hw, int C, int G, int x_bf16) {
   p.nblk = (C + C8_BLOCK - 1) / C8_BLOCK;
   const long long rows = (p.E + p.L - 1) / p.L;
   p.rows = (int)rows;
+  p.full_rows = (int)(p.E / p.L);
   const int pieces = p.L / nv;
   p.slabs = (pieces + 63) / 64;
   p.TV = (pieces + p.slabs - 1) / p.slabs;
   if (C % C8_BLOCK == 0) p.TV = (p.TV + 7) / 8 * 8;        // (a block of 32 channels stays inside one wave)
   p.slabs = (pieces + p.TV - 1) / p.TV;
   p.TP = THREADS / p.TV;
-  const long long want = std::max(1LL, 2048 / std::max(1LL, (long long)N * p.slabs));
+  const long long want = std::max(1LL, 1024 / std::max(1LL, (long long)N * p.slabs));
   long long rpc = std::max((rows + want - 1) / want, (long long)p.TP * 4);
   rpc = std::min(rpc, std::max(1LL, rows));
   p.rows_per_chunk = (int)rpc;
@@ -514,8 +676,7 @@ bool type_ok(int t) { return t == 0 || t == 1; }
 
 template <typename TX>
 int pack(const void* x, long long rows, int C, int nblk, long long ld, signed char* codes, unsigned char* exps, hipStream_t stream) {
-  const long long blocks = (rows * nblk + 31) / 32;
-  SG2IM_LAUNCH(pack8_kernel<TX>, dim3((unsigned)std::min(blocks, 1LL << 20)), dim3(THREADS), 0, stream,
+  SG2IM_LAUNCH(pack8_kernel<TX>, dim3(piece_blocks(rows * nblk * (C8_BLOCK / VecOf<TX>::n))), dim3(THREADS), 0, stream,
                reinterpret_cast<const TX*>(x), rows, C, nblk, ld, codes, exps);
   return status();
 }
@@ -527,21 +688,28 @@ void launch_forward(const Params& p, hipStream_t stream) {
   const long long per = (long long)p.chunks * (p.L / p.C) * p.D;
   const int threads = per <= 256 ? 64 : per <= 4096 ? 256 : 1024;
   SG2IM_LAUNCH(fwd_finish_kernel, dim3((unsigned)((long long)p.N * p.G)), dim3(threads), 0, stream, p);
-  SG2IM_LAUNCH((fwd_apply_kernel<TX, TY>), dim3(blocks), dim3(THREADS), 0, stream, p);
+  if (p.codes_out) SG2IM_LAUNCH((fwd_apply_kernel<TX, TY, true>), dim3(blocks), dim3(THREADS), 0, stream, p);
+  else SG2IM_LAUNCH((fwd_apply_kernel<TX, TY, false>), dim3(blocks), dim3(THREADS), 0, stream, p);
 }
 
-template <typename SRC, typename TX, typename TY>
+template <typename SRC, typename TX, typename TY, bool EVEN>
 void launch_backward(const Params& p, bool need_dx, bool need_params, hipStream_t stream) {
   const long long blocks = (long long)p.N * p.chunks * p.slabs;
-  SG2IM_LAUNCH((bwd_partial_kernel<SRC, TX, TY>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
+  SG2IM_LAUNCH((bwd_partial_kernel<SRC, TX, TY, EVEN>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
   const int gpb = p.D >= FIN_CH ? 1 : FIN_CH / p.D;
   SG2IM_LAUNCH(bwd_finish_kernel, dim3((unsigned)((long long)p.N * ((p.G + gpb - 1) / gpb))), dim3(FIN_CH * FIN_LANES), 0,
                stream, p, gpb);
   const int tail = need_params ? (p.C + 31) / 32 : 0;
   if (need_dx)
-    SG2IM_LAUNCH((bwd_apply_kernel<SRC, TX, TY>), dim3((unsigned)(blocks + tail)), dim3(THREADS), 0, stream, p, blocks);
+    SG2IM_LAUNCH((bwd_apply_kernel<SRC, TX, TY, EVEN>), dim3((unsigned)(blocks + tail)), dim3(THREADS), 0, stream, p, blocks);
   else if (tail)
     SG2IM_LAUNCH(param_grads_kernel, dim3(tail), dim3(THREADS), 0, stream, p);
+}
+template <typename TX, typename TY>
+void launch_backward(const Params& p, bool need_dx, bool need_params, hipStream_t stream) {
+  if (!p.codes) launch_backward<TX, TX, TY, true>(p, need_dx, need_params, stream);        // (the flag is the 8-bit form's alone)
+  else if (p.C % VecOf<TX>::n == 0) launch_backward<signed char, TX, TY, true>(p, need_dx, need_params, stream);
+  else launch_backward<signed char, TX, TY, false>(p, need_dx, need_params, stream);
 }
 
 }  // namespace gn
@@ -571,11 +739,13 @@ int sg2im_groupnorm_act_forward(const void* x, int x_dtype, int batch, long long
   if (!x || !out || !stats || !workspace || workspace_bytes < need_bytes(p, false)) return SG2IM_ERR_ARG;
   p.x = x; p.gamma = gamma; p.beta = beta; p.param_bf16 = param_dtype; p.slope = slope; p.eps = eps; p.out = out;
   p.stats = stats; p.part = workspace;
+  const bool fused = codes && channels % C8_BLOCK == 0;     // the 8-bit form on the way, or in a launch of its own
+  if (fused) { p.codes_out = codes; p.exps_out = exps; }
   if (x_dtype == 0 && out_dtype == 0) launch_forward<float, float>(p, stream);
   else if (x_dtype == 0) launch_forward<float, bf16_s>(p, stream);
   else launch_forward<bf16_s, bf16_s>(p, stream);
   if (status() != SG2IM_OK) return SG2IM_ERR_HIP;
-  if (codes) {
+  if (codes && !fused) {
     const long long rows = (long long)batch * hw;
     return x_dtype ? pack<bf16_s>(x, rows, channels, p.nblk, channels, codes, exps, stream)
                    : pack<float>(x, rows, channels, p.nblk, channels, codes, exps, stream);
@@ -604,16 +774,9 @@ int sg2im_groupnorm_act_backward(const void* dy, int dy_dtype, const void* x, in
     if (need_params) SG2IM_LAUNCH(param_grads_kernel, dim3((channels + 31) / 32), dim3(THREADS), 0, stream, p);
     return status();
   }
-  #define SG2IM_GN_BWD(SRC)                                                                                       \
-    if (x_dtype == 0 && dy_dtype == 0) launch_backward<SRC(float), float, float>(p, dx != nullptr, need_params, stream);      \
-    else if (x_dtype == 0) launch_backward<SRC(float), float, bf16_s>(p, dx != nullptr, need_params, stream);                 \
-    else launch_backward<SRC(bf16_s), bf16_s, bf16_s>(p, dx != nullptr, need_params, stream)
-  #define SG2IM_GN_SAME(T) T
-  #define SG2IM_GN_CODES(T) signed char
-  if (codes) { SG2IM_GN_BWD(SG2IM_GN_CODES); } else { SG2IM_GN_BWD(SG2IM_GN_SAME); }
-  #undef SG2IM_GN_BWD
-  #undef SG2IM_GN_SAME
-  #undef SG2IM_GN_CODES
+  if (x_dtype == 0 && dy_dtype == 0) launch_backward<float, float>(p, dx != nullptr, need_params, stream);
+  else if (x_dtype == 0) launch_backward<float, bf16_s>(p, dx != nullptr, need_params, stream);
+  else launch_backward<bf16_s, bf16_s>(p, dx != nullptr, need_params, stream);
   return status();
 }
 
@@ -633,8 +796,8 @@ int sg2im_unpack8(const signed char* codes, const unsigned char* exps, long long
   if (rows == 0) return SG2IM_OK;
   if (!out || !codes || !exps) return SG2IM_ERR_ARG;
   const int nblk = (channels + C8_BLOCK - 1) / C8_BLOCK;
-  const long long blocks = (rows * nblk * 8 + THREADS - 1) / THREADS;
-  const dim3 grid((unsigned)std::min(blocks, 1LL << 20));
+  const int nv = dtype ? 8 : 4;
+  const dim3 grid(piece_blocks(rows * ((channels + nv - 1) / nv)));
   if (dtype) SG2IM_LAUNCH(unpack8_kernel<bf16_s>, grid, dim3(THREADS), 0, stream, codes, exps, rows, channels, nblk, reinterpret_cast<bf16_s*>(out), ld);
   else SG2IM_LAUNCH(unpack8_kernel<float>, grid, dim3(THREADS), 0, stream, codes, exps, rows, channels, nblk, reinterpret_cast<float*>(out), ld);
   return status();

@@ -8,9 +8,8 @@ from ctypes import c_void_p
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
-from . import ops
+from . import _lib, ops
 from .ops import conv_desc, nhwc_src, rows_src
 
 BN_EPS, BN_MOMENTUM = 1e-5, 0.1
@@ -1442,108 +1441,36 @@ class InstNormAct(Function):
     return ops.instnorm_backward(dyn, y, st, dyn), None
 
 
-def _param_targets(params, needs):
-  """where the gradients of ``params`` go: (buffers, accumulate, what autograd gets).  All of them straight into their
-  registered sinks, or all into new tensors of the parameters' type (added to the sinks that there are)."""
-  live = [p if p is not None and need else None for p, need in zip(params, needs)]
-  sinks = [_sink(p) for p in live]
-  if all(p is None or k is not None for p, k in zip(live, sinks)):
-    return sinks, True, [None] * len(params)
-  bufs = [torch.empty_like(p, memory_format=torch.contiguous_format) if p is not None else None for p in live]
-  return bufs, False, bufs
-
-
-def _into_sinks(params, grads):
-  """gradients of _param_targets for autograd; one whose parameter has a sink is added there"""
-  out = []
-  for p, g in zip(params, grads):
-    k = _sink(p) if g is not None else None
-    if k is not None:
-      k.add_(g.view(k.shape))
-      g = None
-    out.append(g)
-  return out
-
-
-class GroupNormAct(Function):
+class GroupNormAct(object):
   """leaky_slope(group_norm(x)) of a channels-last map x (N, ..., C), float32 or bfloat16 (statistics in 64 bits):
   C / groups channels and all pixels of an image share a mean and a (biased) variance.  weight / bias: (C,) vectors of one
   type, or None.  checkpoint8: the backward pass keeps x in 8 bits (ops.pack8) and is computed from that.
-  out_dtype: x's type (None), or torch.bfloat16."""
+  out_dtype: x's type (None), or torch.bfloat16.  The autograd node is native (csrc/native.cpp); parameters with a
+  registered gradient sink get their gradient there, as everywhere in this module."""
 
   @staticmethod
-  def forward(ctx, x, weight, bias, groups, slope=1.0, eps=BN_EPS, checkpoint8=False, out_dtype=None):
-    x = x.contiguous()
-    need = any(ctx.needs_input_grad[:3])
-    y, stats, packed = ops.group_norm_act_forward(x, weight, bias, groups, slope, eps, out_dtype,
-                                                  pack=bool(checkpoint8) and need)
-    ctx.geom = (int(groups), float(slope), packed is not None, x.dtype)
-    if packed is not None:
-      ctx.save_for_backward(packed.codes, packed.exps, weight, bias, stats)
-    else:
-      ctx.save_for_backward(x, None, weight, bias, stats)
-    return y
-
-  @staticmethod
-  @once_differentiable
-  def backward(ctx, g):
-    x, exps, weight, bias, stats = ctx.saved_tensors
-    groups, slope, packed, dtype = ctx.geom
-    ni = ctx.needs_input_grad
-    if packed:
-      x = ops.Packed8(x, exps, dtype)
-    bufs, acc, grads = _param_targets((weight, bias), ni[1:3])
-    dx = ops.group_norm_act_backward(g.contiguous(), x, weight, bias, groups, slope, stats, ni[0], bufs[0], bufs[1], acc)
-    dw, db = _into_sinks((weight, bias), grads)
-    return dx, dw, db, None, None, None, None, None
+  def apply(x, weight, bias, groups, slope=1.0, eps=BN_EPS, checkpoint8=False, out_dtype=None):
+    if GRAD_SINKS:
+      return _lib.eager().group_norm_act(x, weight, bias, groups, slope, eps, checkpoint8, ops._code(out_dtype, 'group norm output'),
+                                         _sink(weight), _sink(bias))
+    return _lib.eager().group_norm_act(x, weight, bias, groups, slope, eps, checkpoint8, ops._code(out_dtype, 'group norm output'),
+                                       None, None)
 
 
-class LinearResidual(Function):
+class LinearResidual(object):
   """y = leaky_slope(x W^T + b) + residual for x (..., K), W (N, K); float32, or bfloat16 operands with float32
   accumulation.  W has x's type, or is float32 next to a bfloat16 x (it is rounded for the product; its gradient is
-  float32).  bias (N,) and residual (..., N) may be None; the residual has the output's type.  checkpoint8: the weight's
-  gradient is computed from x in 8 bits (ops.pack8), which is what the backward pass keeps of x.  out_dtype: x's
+  float32).  bias (N,) and residual (..., N) may be None; the residual has the output's type and shape.  checkpoint8: the
+  weight's gradient is computed from x in 8 bits (ops.pack8), which is what the backward pass keeps of x.  out_dtype: x's
   type (None), or torch.float32."""
 
   @staticmethod
-  def forward(ctx, x, weight, bias, residual, slope=1.0, checkpoint8=False, out_dtype=None):
-    ni = ctx.needs_input_grad
-    w = weight.contiguous()
-    if x.dtype == torch.bfloat16 and w.dtype == torch.float32:
-      w = w.to(torch.bfloat16)
-    slope = float(slope)
-    need = any(ni[:3])
-    y, signs = ops.linear_forward(x, w, bias, residual, slope, out_dtype, signs=need and slope != 1.0)
-    packed = ops.pack8(x) if checkpoint8 and ni[1] else None
-    ctx.geom = (slope, x.dtype, tuple(x.shape))
-    ctx.save_for_backward(*((packed.codes, packed.exps) if packed is not None else (x if ni[1] else None, None)),
-                          weight, w if ni[0] and w is not weight else None, bias, signs)
-    return y
-
-  @staticmethod
-  @once_differentiable
-  def backward(ctx, g):
-    x, exps, weight, w, bias, signs = ctx.saved_tensors
-    slope, dtype, shape = ctx.geom
-    ni = ctx.needs_input_grad
-    dx = dw = db = None
-    products = ni[0] or ni[1]
-    if products or ni[2]:
-      (db_buf,), acc, dbs = _param_targets((bias,), ni[2:3])
-      plain = signs is None and g.dtype == dtype             # dz is dy itself
-      dz = None
-      if not plain or ni[2]:
-        dz = ops.linear_backward_act(g, signs, slope, None if plain or not products else dtype, db_buf, acc)
-      if plain:
-        dz = ops._rows2d(g, 'linear gradient')[0]
-      (db,) = _into_sinks((bias,), dbs)
-      if ni[0]:
-        dx = ops.linear_backward_data(dz, weight if w is None else w).view(shape)
-      if ni[1]:
-        (dw_buf,), acc, dws = _param_targets((weight,), (True,))
-        ops.linear_backward_weight(dz, x if exps is None else ops.Packed8(x, exps, dtype), dw_buf.view(weight.shape), acc)
-        (dw,) = _into_sinks((weight,), dws)
-    return dx, dw, db, (g if ni[3] else None), None, None, None
+  def apply(x, weight, bias, residual, slope=1.0, checkpoint8=False, out_dtype=None):
+    if GRAD_SINKS:
+      return _lib.eager().linear_residual(x, weight, bias, residual, slope, checkpoint8, ops._code(out_dtype, 'linear output'),
+                                          _sink(weight), _sink(bias))
+    return _lib.eager().linear_residual(x, weight, bias, residual, slope, checkpoint8, ops._code(out_dtype, 'linear output'),
+                                        None, None)
 
 
 class LeakyFn(Function):

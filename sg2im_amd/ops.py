@@ -1295,36 +1295,17 @@ def adam_step_guarded(param, grad, exp_avg, exp_avg_sq, lr, beta1, beta2, eps, s
 # ----------------------------------------------------------------------------
 # group norm + activation, linear + activation + residual, 8-bit activation checkpoints
 # ----------------------------------------------------------------------------
-# These take float32 and bfloat16 tensors.  Their work buffers come from torch's allocator per call (inside a capture:
-# from the graph's own pool), so neither two streams nor two captured graphs share one.
+# These take float32 and bfloat16 tensors; checks, outputs and work buffers are csrc/native.cpp's.  TypeError for a type,
+# ValueError for a shape, a device or a value.
 
-def _on_device(t, what):
-  """device pointer of a float32 / bfloat16 tensor of the CURRENT device (the launch goes to its current stream)"""
-  if not (torch.is_tensor(t) and t.is_cuda and t.dtype in (torch.float32, torch.bfloat16)):
-    raise TypeError('%s: expected a float32 / bfloat16 tensor on the GPU, got %s'
-                    % (what, '%s on %s' % (t.dtype, t.device) if torch.is_tensor(t) else type(t).__name__))
-  if t.device.index != torch.cuda.current_device():
-    raise ValueError('%s lies on cuda:%d but the current device is cuda:%d' % (what, t.device.index, torch.cuda.current_device()))
-  return c_void_p(t.data_ptr())
+_CODES = {None: -1, torch.float32: 0, torch.bfloat16: 1}
 
 
-def _work(device, nbytes):
-  return torch.empty(int(nbytes), dtype=torch.uint8, device=device)
-
-
-def _params(weight, bias, n, what):
-  """dtype code of the two parameter vectors (either may be None)"""
-  code = 0
-  for name, t in (('weight', weight), ('bias', bias)):
-    if t is None:
-      continue
-    _on_device(t, '%s %s' % (what, name))
-    if t.shape != (n,) or not t.is_contiguous():
-      raise ValueError('%s: %s must be a dense vector of %d values, got %s' % (what, name, n, tuple(t.shape)))
-    code = _dt(t)
-  if weight is not None and bias is not None and weight.dtype != bias.dtype:
-    raise TypeError('%s: weight is %s, bias is %s' % (what, weight.dtype, bias.dtype))
-  return code
+def _code(dtype, what):
+  try:
+    return _CODES[dtype]
+  except KeyError:
+    raise TypeError('%s: float32 or bfloat16, not %s' % (what, dtype)) from None
 
 
 class Packed8(object):
@@ -1340,212 +1321,58 @@ class Packed8(object):
     return self.codes.shape
 
 
-def _packed_like(x):
-  C = x.size(-1)
-  return Packed8(torch.empty(x.shape, dtype=torch.int8, device=x.device),
-                 torch.empty(x.shape[:-1] + ((C + 31) // 32,), dtype=torch.uint8, device=x.device), x.dtype)
-
-
-def _rows2d(t, what):
-  """(matrix view, leading dimension) of the rows of t (..., C); a copy where the rows are not dense in memory"""
-  if t.dim() < 1 or t.size(-1) < 1:
-    raise ValueError('%s: expected (..., channels), got %s' % (what, tuple(t.shape)))
-  m = t.reshape(-1, t.size(-1))
-  if (m.size(1) > 1 and m.stride(1) != 1) or (m.size(0) > 1 and m.stride(0) < m.size(1)):
-    m = m.contiguous()
-  return m, (m.stride(0) if m.size(0) > 1 else m.size(1))
-
-
 def pack8(x):
   """the 8-bit form of an activation x (..., channels), float32 or bfloat16"""
-  _on_device(x, 'pack8')
-  m, ld = _rows2d(x, 'pack8')
-  p = _packed_like(x)
-  call('sg2im_pack8', c_void_p(m.data_ptr()), _dt(x), m.size(0), m.size(1), ld, c_void_p(p.codes.data_ptr()),
-       c_void_p(p.exps.data_ptr()), _stream())
-  return p
-
-
-def _check_packed(p, what):
-  C = p.codes.size(-1) if p.codes.dim() else 0
-  if not (p.codes.is_cuda and p.exps.is_cuda and p.codes.dtype == torch.int8 and p.exps.dtype == torch.uint8 and
-          p.codes.is_contiguous() and p.exps.is_contiguous() and C >= 1 and
-          tuple(p.exps.shape) == tuple(p.codes.shape[:-1]) + ((C + 31) // 32,)):
-    raise ValueError('%s: not an 8-bit form made by pack8' % what)
-  if p.codes.device.index != torch.cuda.current_device() or p.exps.device != p.codes.device:
-    raise ValueError('%s: the 8-bit form does not lie on the current device' % what)
+  codes, exps = _lib.eager().pack8(x)
+  return Packed8(codes, exps, x.dtype)
 
 
 def unpack8(p, dtype=None):
   """the values of an 8-bit form, in the type it was made from (or ``dtype``: exact in both)"""
   if not isinstance(p, Packed8):
     raise TypeError('unpack8: expected a Packed8, got %s' % type(p).__name__)
-  _check_packed(p, 'unpack8')
-  out = torch.empty(p.shape, dtype=p.dtype if dtype is None else dtype, device=p.codes.device)
-  _on_device(out, 'unpack8')
-  C = p.shape[-1]
-  call('sg2im_unpack8', c_void_p(p.codes.data_ptr()), c_void_p(p.exps.data_ptr()), p.codes.numel() // C, C,
-       c_void_p(out.data_ptr()), _dt(out), C, _stream())
-  return out
+  return _lib.eager().unpack8(p.codes, p.exps, _code(dtype or p.dtype, 'unpack8'))
 
 
-def _gn_geometry(x, groups):
-  if x.dim() < 2 or x.size(-1) < 1:
-    raise ValueError('group norm: expected (batch, ..., channels), got %s' % (tuple(x.shape),))
-  C, G = x.size(-1), int(groups)
-  if G < 1 or C % G:
-    raise ValueError('group norm: %d channels do not divide into %d groups' % (C, G))
-  hw = 1
-  for d in x.shape[1:-1]:
-    hw *= int(d)
-  if hw < 1:
-    raise ValueError('group norm: an image without pixels %s' % (tuple(x.shape),))
-  return int(x.size(0)), hw, C, G
+def _either(x):
+  """(x, codes, exps, type code) of a tensor or a Packed8"""
+  if isinstance(x, Packed8):
+    return None, x.codes, x.exps, _code(x.dtype, '8-bit form')
+  return x, None, None, _code(x.dtype, 'input')
 
 
 def group_norm_act_forward(x, weight, bias, groups, slope, eps, out_dtype=None, pack=False):
   """leaky_slope(group_norm(x)) of a dense x (batch, ..., channels): (y, stats, Packed8 of x or None)"""
-  px = _on_device(x, 'group norm input')
-  N, hw, C, G = _gn_geometry(x, groups)
-  if not x.is_contiguous():
-    raise ValueError('group norm: the input must be dense')
-  if out_dtype not in (None, torch.bfloat16, x.dtype):
-    raise TypeError('group norm: a %s output of a %s input' % (out_dtype, x.dtype))
-  if not eps >= 0:
-    raise ValueError('group norm: eps = %r' % (eps,))
-  code = _params(weight, bias, C, 'group norm')
-  y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
-  stats = torch.empty(N, G, 2, dtype=torch.float64, device=x.device)
-  p = _packed_like(x) if pack else None
-  nbytes = _lib.load().sg2im_groupnorm_workspace(N, hw, C, G, _dt(x), 0)
-  if nbytes == 0:
-    raise ValueError('group norm: %s is too large' % (tuple(x.shape),))
-  work = _work(x.device, nbytes)
-  call('sg2im_groupnorm_act_forward', px, _dt(x), N, hw, C, G, _ptr(weight), _ptr(bias), code, float(slope), float(eps),
-       _ptr(y), _dt(y), _ptr(stats), _ptr(p.codes) if pack else None, _ptr(p.exps) if pack else None, _ptr(work), nbytes,
-       _stream())
-  return y, stats, p
+  y, stats, codes, exps = _lib.eager().group_norm_act_forward(x, weight, bias, groups, slope, eps,
+                                                              _code(out_dtype, 'group norm output'), pack)
+  return y, stats, Packed8(codes, exps, x.dtype) if pack else None
 
 
 def group_norm_act_backward(dy, x, weight, bias, groups, slope, stats, need_dx=True, dweight=None, dbias=None,
                             accumulate=False):
   """dx (or None) of group_norm_act_forward; x: the input or its Packed8; dweight / dbias: where those gradients go"""
-  packed = isinstance(x, Packed8)
-  if packed:
-    _check_packed(x, 'group norm backward')
-  else:
-    _on_device(x, 'group norm input')
-  pdy = _on_device(dy, 'group norm gradient')
-  if tuple(dy.shape) != tuple(x.shape) or not dy.is_contiguous() or not (packed or x.is_contiguous()):
-    raise ValueError('group norm backward: dense tensors of one shape, got %s and %s' % (tuple(dy.shape), tuple(x.shape)))
-  dt = 1 if x.dtype == torch.bfloat16 else 0
-  if dt == 1 and dy.dtype != torch.bfloat16:
-    raise TypeError('group norm backward: a %s gradient of a bfloat16 input' % dy.dtype)
-  N, hw, C, G = _gn_geometry(dy, groups)
-  code = _params(weight, bias, C, 'group norm')
-  gcode = _params(dweight, dbias, C, 'group norm gradient')
-  if not (stats.is_cuda and stats.dtype == torch.float64 and tuple(stats.shape) == (N, G, 2) and stats.is_contiguous()):
-    raise ValueError('group norm backward: not the statistics of this input')
-  dx = torch.empty(x.shape, dtype=x.dtype, device=dy.device) if need_dx else None
-  nbytes = _lib.load().sg2im_groupnorm_workspace(N, hw, C, G, dt, 1)
-  work = _work(dy.device, nbytes)
-  call('sg2im_groupnorm_act_backward', pdy, _dt(dy), None if packed else _ptr(x), dt, _ptr(x.codes) if packed else None,
-       _ptr(x.exps) if packed else None, N, hw, C, G, _ptr(weight), _ptr(bias), code, float(slope), _ptr(stats), _ptr(dx),
-       _ptr(dweight), _ptr(dbias), gcode, int(accumulate), _ptr(work), nbytes, _stream())
-  return dx
-
-
-def _linear_work(device, M, K, N, dt, which):
-  nbytes = _lib.load().sg2im_linear_workspace(M, K, N, dt, which)
-  return _work(device, nbytes), nbytes
+  xt, codes, exps, dt = _either(x)
+  return _lib.eager().group_norm_act_backward(dy, xt, codes, exps, dt, weight, bias, groups, slope, stats, need_dx, dweight,
+                                              dbias, accumulate)
 
 
 def linear_forward(x, weight, bias, residual, slope, out_dtype=None, signs=False):
   """leaky_slope(x W^T + b) + residual for x (..., K) and a dense W (N, K) of one type: (y, signs or None)"""
-  px = _on_device(x, 'linear input')
-  _on_device(weight, 'linear weight')
-  if weight.dim() != 2 or not weight.is_contiguous() or weight.dtype != x.dtype:
-    raise ValueError('linear: the weight must be a dense matrix of the input\'s type, got %s %s'
-                     % (weight.dtype, tuple(weight.shape)))
-  N, K = weight.shape
-  if x.dim() < 1 or x.size(-1) != K or K < 1 or N < 1:
-    raise ValueError('linear: input %s and weight %s' % (tuple(x.shape), tuple(weight.shape)))
-  out_dtype = out_dtype or x.dtype
-  if out_dtype not in (torch.float32, x.dtype):
-    raise TypeError('linear: a %s output of %s operands' % (out_dtype, x.dtype))
-  code = _params(None, bias, N, 'linear')
-  m, ld = _rows2d(x, 'linear')
-  M = m.size(0)
-  shape = tuple(x.shape[:-1]) + (N,)
-  r, ld_r = None, N
-  if residual is not None:
-    _on_device(residual, 'linear residual')
-    if tuple(residual.shape) != shape or residual.dtype != out_dtype:
-      raise ValueError('linear: the residual must be %s %s, got %s %s'
-                       % (out_dtype, shape, residual.dtype, tuple(residual.shape)))
-    r, ld_r = _rows2d(residual, 'linear residual')
-  y = torch.empty(shape, dtype=out_dtype, device=x.device)
-  bits = torch.empty(M, (N + 31) // 32, dtype=torch.int32, device=x.device) if signs else None
-  work, nbytes = _linear_work(x.device, M, K, N, _dt(x), 0)
-  call('sg2im_linear_forward', _ptr(m), _dt(x), ld, _ptr(weight), _ptr(bias), code, _ptr(r), ld_r, float(slope), _ptr(y),
-       _dt(y), N, _ptr(bits), M, K, N, _ptr(work), nbytes, _stream())
-  return y, bits
+  return _lib.eager().linear_forward(x, weight, bias, residual, slope, _code(out_dtype, 'linear output'), signs)
 
 
 def linear_backward_act(dy, signs, slope, dz_dtype=None, dbias=None, accumulate=False):
   """dz = dy * leaky'(z) as ``dz_dtype`` (None: not written) and the bias gradient into ``dbias``"""
-  _on_device(dy, 'linear gradient')
-  m, ld = _rows2d(dy, 'linear gradient')
-  M, N = m.shape
-  dz = torch.empty(M, N, dtype=dz_dtype, device=dy.device) if dz_dtype is not None else None
-  if signs is not None and not (signs.is_cuda and signs.dtype == torch.int32 and tuple(signs.shape) == (M, (N + 31) // 32) and
-                                signs.is_contiguous()):
-    raise ValueError('linear backward: not the signs of this output')
-  code = _params(None, dbias, N, 'linear gradient')
-  work, nbytes = _linear_work(dy.device, M, 1, N, 0, 3)
-  call('sg2im_linear_backward_act', _ptr(m), _dt(dy), ld, _ptr(signs), float(slope), _ptr(dz),
-       (1 if dz_dtype == torch.bfloat16 else _dt(dy) if dz is None else 0), _ptr(dbias), code, int(accumulate), M, N,
-       _ptr(work), nbytes, _stream())
-  return dz
+  return _lib.eager().linear_backward_act(dy, signs, slope, _code(dz_dtype, 'linear gradient'), dbias, accumulate)
 
 
 def linear_backward_data(dz, weight):
   """dx = dz W for dz (M, N) and a dense W (N, K) of one type"""
-  _on_device(dz, 'linear gradient')
-  _on_device(weight, 'linear weight')
-  if dz.dim() != 2 or weight.dim() != 2 or dz.size(1) != weight.size(0) or dz.dtype != weight.dtype or \
-      not weight.is_contiguous():
-    raise ValueError('linear backward: gradient %s %s and weight %s %s'
-                     % (dz.dtype, tuple(dz.shape), weight.dtype, tuple(weight.shape)))
-  m, ld = _rows2d(dz, 'linear gradient')
-  (M, N), K = m.shape, weight.size(1)
-  dx = torch.empty(M, K, dtype=dz.dtype, device=dz.device)
-  work, nbytes = _linear_work(dz.device, M, K, N, _dt(dz), 1)
-  call('sg2im_linear_backward_data', _ptr(m), _dt(dz), ld, _ptr(weight), _ptr(dx), K, M, K, N, _ptr(work), nbytes, _stream())
-  return dx
+  return _lib.eager().linear_backward_data(dz, weight)
 
 
 def linear_backward_weight(dz, x, dweight, accumulate=False):
   """dweight (N, K) (+)= dz^T x; x: the layer's input (..., K) or its Packed8"""
-  _on_device(dz, 'linear gradient')
-  _on_device(dweight, 'linear weight gradient')
-  packed = isinstance(x, Packed8)
-  if packed:
-    _check_packed(x, 'linear backward')
-    m, ld, K = x, x.shape[-1], x.shape[-1]
-    M = x.codes.numel() // K
-  else:
-    _on_device(x, 'linear input')
-    m, ld = _rows2d(x, 'linear')
-    M, K = m.shape
-  z, ld_z = _rows2d(dz, 'linear gradient')
-  N = z.size(1)
-  if z.size(0) != M or dz.dtype != x.dtype or tuple(dweight.shape) != (N, K) or not dweight.is_contiguous() or \
-      dweight.dtype not in (torch.float32, dz.dtype):
-    raise ValueError('linear backward: gradient %s %s, input %s %s, weight gradient %s %s'
-                     % (dz.dtype, tuple(dz.shape), x.dtype, tuple(x.shape), dweight.dtype, tuple(dweight.shape)))
-  work, nbytes = _linear_work(dz.device, M, K, N, _dt(dz), 2)
-  call('sg2im_linear_backward_weight', _ptr(z), _dt(dz), ld_z, None if packed else _ptr(m), ld,
-       _ptr(x.codes) if packed else None, _ptr(x.exps) if packed else None, _ptr(dweight), _dt(dweight), int(accumulate),
-       M, K, N, _ptr(work), nbytes, _stream())
+  xt, codes, exps, _ = _either(x)
+  _lib.eager().linear_backward_weight(dz, xt, codes, exps, dweight, accumulate)
   return dweight

@@ -558,7 +558,7 @@ def test_wrappers_refuse():
     with pytest.raises((TypeError, ValueError)):
       f()
       pytest.fail('case %d was taken' % k)
-  y = HF.GroupNormAct.apply(x.requires_grad_(True), None, None, 2)
-  (g,) = torch.autograd.grad(y.sum(), (x,), create_graph=True)
-  with pytest.raises(RuntimeError):                                   # no second derivative
-    torch.autograd.grad(g.sum(), (x,))
+  # no second derivative
+  for y in (HF.GroupNormAct.apply(x.requires_grad_(True), None, None, 2), HF.LinearResidual.apply(x, w, None, None)):
+    with pytest.raises(RuntimeError):
+      torch.autograd.grad(y.sum(), (x,), create_graph=True)
