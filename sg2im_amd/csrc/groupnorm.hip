@@ -224,12 +224,14 @@ __device__ __forceinline__ void block_sum2(double& a, double& b, double (*red)[2
   for (int i = 0; i < waves; ++i) { a += red[i][0]; b += red[i][1]; }
 }
 
-__device__ __forceinline__ void write_stats(const Params& p, long long group, double s, double q) {
-  const double cnt = (double)(p.E / p.C) * p.D, mean = s / cnt;
+__device__ __forceinline__ void write_stats(const Params& p, long long group, double s, double q, double& mean, double& rstd) {
+  const double cnt = (double)(p.E / p.C) * p.D;
+  mean = s / cnt;
   double var = q / cnt - mean * mean;
   if (var < 0.0) var = 0.0;                                        // (a NaN stays one)
+  rstd = 1.0 / sqrt(var + (double)p.eps);
   p.stats[group * 2] = mean;
-  p.stats[group * 2 + 1] = 1.0 / sqrt(var + (double)p.eps);
+  p.stats[group * 2 + 1] = rstd;
 }
 
 // one workgroup per (image, group): the chunks' sums joined in a fixed order
@@ -248,7 +250,7 @@ __global__ __launch_bounds__(1024) void fwd_finish_kernel(const Params p) {
     q += part[at + p.L];
   }
   block_sum2(s, q, red);
-  if (threadIdx.x == 0) write_stats(p, b, s, q);
+  if (threadIdx.x == 0) { double mean, rstd; write_stats(p, b, s, q, mean, rstd); }
 }
 
 // a position's affine: z = fma(x - m, a, b) with m = float(mean), the difference of the two means in b
@@ -548,6 +550,243 @@ __global__ __launch_bounds__(THREADS) void bwd_apply_kernel(const Params p, long
     });
 }
 
+// ---- small maps: one workgroup keeps a slab of an image ------------------------------------------------------------------
+// A slab is S positions of a row that hold whole groups, over all rows of one image.  Its pieces stay in registers (up to
+// ITER per thread) between the statistics and their use: x is read once and one launch does the forward pass, one (and one
+// for the parameters' sums over the images) the backward pass.
+
+struct Slab { int q0, pl, n, base, TV, TP; bool on; };
+__device__ __forceinline__ Slab slab_of(const Params& p, int NV) {
+  Slab w;
+  w.n = (int)(blockIdx.x / p.slabs);
+  w.base = (int)(blockIdx.x % p.slabs) * p.S;
+  w.TV = p.S / NV;
+  w.TP = blockDim.x / w.TV;
+  w.q0 = w.base + (int)(threadIdx.x % w.TV) * NV;
+  w.pl = threadIdx.x / w.TV;
+  w.on = w.pl < w.TP && w.q0 < p.L;
+  return w;
+}
+__device__ __forceinline__ int piece_length(const Params& p, const Slab& w, int NV, int row) {
+  const long long left = w.on && row < p.rows ? p.E - (long long)row * p.L - w.q0 : 0;
+  return left >= NV ? NV : left > 0 ? (int)left : 0;
+}
+
+// sums of NV values per thread over the pixel lanes, into sums[0 .. S) (double); buf: blockDim * NV values of V
+template <typename V, int NV>
+__device__ __forceinline__ void slab_sums(const V (&s)[NV], V* buf, double* sums, const Slab& w, int S) {
+  if (w.pl < w.TP) {
+    #pragma unroll
+    for (int j = 0; j < NV; ++j) buf[threadIdx.x * NV + j] = s[j];
+  }
+  __syncthreads();
+  const int B = blockDim.x;
+  if (S >= B) {
+    for (int i = threadIdx.x; i < S; i += B) {
+      double a = 0.0;
+      for (int t = 0; t < w.TP; ++t) a += buf[t * S + i];
+      sums[i] = a;
+    }
+    __syncthreads();
+    return;
+  }
+  // more threads than positions: `parts` threads per position, then one
+  const int parts = B / S, i = threadIdx.x % S, part = threadIdx.x / S;
+  double a = 0.0;
+  if (part < parts) for (int t = part; t < w.TP; t += parts) a += buf[t * S + i];
+  __syncthreads();
+  double* mid = reinterpret_cast<double*>(buf);              // (B doubles; buf holds at least that: NV * sizeof(V) >= 8)
+  if (part < parts) mid[part * S + i] = a;
+  __syncthreads();
+  if ((int)threadIdx.x < S) {
+    a = 0.0;
+    for (int t = 0; t < parts; ++t) a += mid[t * S + threadIdx.x];
+    sums[threadIdx.x] = a;
+  }
+  __syncthreads();
+}
+
+// positions of the slab -> groups: f(group, its sums of two arrays); a wave per group
+template <typename F>
+__device__ __forceinline__ void slab_groups(const Params& p, const Slab& w, const double* s0, const double* s1, F f) {
+  const int reps = p.L / p.C, span = min(p.S, p.L - w.base);          // (reps > 1: the slab is the whole row)
+  const int g0 = reps > 1 ? 0 : w.base / p.D, ng = reps > 1 ? p.G : span / p.D;
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  for (int g = threadIdx.x >> 6; g < ng; g += waves) {
+    double a = 0.0, b = 0.0;
+    for (int i = lane; i < p.D * reps; i += 64) {
+      const int at = reps > 1 ? (i / p.D) * p.C + g * p.D + i % p.D : g * p.D + i;
+      a += s0[at];
+      b += s1[at];
+    }
+    #pragma unroll
+    for (int o = 32; o; o >>= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
+    if (lane == 0) f(g0 + g, a, b);
+  }
+}
+
+constexpr int SLAB_MAX = 2048;              // positions of a slab (two double arrays in LDS)
+
+// (a piece's second use widens it again: without this its floats would be held from the first one on, at twice the registers)
+template <typename R> __device__ __forceinline__ void forget(R& raw) {
+  unsigned w[(sizeof(R) + 3) / 4] = {};
+  __builtin_memcpy(w, &raw, sizeof(R));
+  #pragma unroll
+  for (unsigned i = 0; i < sizeof(w) / 4; ++i) asm volatile("" : "+v"(w[i]));
+  __builtin_memcpy(&raw, w, sizeof(R));
+}
+
+template <typename TX, typename TY, bool PACK, int B, int ITER>
+__global__ __launch_bounds__(B) void fwd_slab_kernel(const Params p) {
+  constexpr int NV = VecOf<TX>::n;
+  __shared__ __attribute__((aligned(16))) double buf[B * NV];
+  __shared__ double s0[SLAB_MAX], s1[SLAB_MAX];
+  const Slab w = slab_of(p, NV);
+  const TX* x = reinterpret_cast<const TX*>(p.x) + (long long)w.n * p.E + w.q0;
+  RawVec<TX, NV> raw[ITER];
+  #pragma unroll
+  for (int k = 0; k < ITER; ++k) {
+    const int row = w.pl + k * w.TP;
+    raw[k] = load_some<TX, NV>(x + (long long)row * p.L, piece_length(p, w, NV, row));
+  }
+  double s[NV], q[NV];
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) s[j] = q[j] = 0.0;
+  #pragma unroll
+  for (int k = 0; k < ITER; ++k) {
+    float v[NV];
+    widen(raw[k], v);
+    #pragma unroll
+    for (int j = 0; j < NV; ++j) { const double d = v[j]; s[j] += d; q[j] = fma(d, d, q[j]); }
+    forget(raw[k]);
+  }
+  slab_sums<double, NV>(s, buf, s0, w, p.S);
+  slab_sums<double, NV>(q, buf, s1, w, p.S);
+  // (a group's results take the place of its first position, which only its own wave has read)
+  const int first = p.L > p.C ? 0 : w.base / p.D;
+  slab_groups(p, w, s0, s1, [&](int g, double a, double b) {
+    double mean, rstd;
+    write_stats(p, (long long)w.n * p.G + g, a, b, mean, rstd);
+    s0[(g - first) * p.D] = mean;
+    s1[(g - first) * p.D] = rstd;
+  });
+  __syncthreads();
+  if (!w.on) return;
+  Affine f[NV];
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (w.q0 + j) % p.C, l = (c / p.D - first) * p.D;
+    f[j] = affine_of(p, c, s0[l], s1[l]);
+  }
+  TY* y = reinterpret_cast<TY*>(p.out) + (long long)w.n * p.E + w.q0;
+  #pragma unroll
+  for (int k = 0; k < ITER; ++k) {
+    const int row = w.pl + k * w.TP, have = piece_length(p, w, NV, row);
+    if (have > 0) {
+      float v[NV];
+      widen(raw[k], v);
+      if constexpr (PACK) write_codes<NV>(p, w.n, row, w.q0, v);
+      forward_values<NV>(v, f, p.slope);
+      store_some<TY, NV>(y + (long long)row * p.L, have, v);
+    }
+  }
+}
+
+template <typename SRC, typename TX, typename TY, bool EVEN, int B, int ITER>
+__global__ __launch_bounds__(B) void bwd_slab_kernel(const Params p) {
+  constexpr int NV = VecOf<TX>::n;
+  __shared__ __attribute__((aligned(16))) float buf[B * NV];
+  __shared__ double s0[SLAB_MAX], s1[SLAB_MAX];
+  typedef Source<SRC, NV, EVEN> X;
+  const Slab w = slab_of(p, NV);
+  const int q0 = w.on ? w.q0 : 0;
+  const X src(p, w.n, q0);
+  const TY* dy = reinterpret_cast<const TY*>(p.dy) + (long long)w.n * p.E + q0;
+  typename X::Raw rx[ITER];
+  RawVec<TY, NV> rg[ITER];
+  #pragma unroll
+  for (int k = 0; k < ITER; ++k) {
+    const int row = w.pl + k * w.TP, have = piece_length(p, w, NV, row);
+    rg[k] = load_some<TY, NV>(dy + (long long)row * p.L, have);
+    if (have > 0) rx[k] = src.load_tail(p, row, have);
+  }
+  Affine f[NV];
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) f[j] = affine_at(p, w.n, q0 + j);
+  const float tol = kink_tolerance<NV>(f, p.slope);
+  float s[NV], q[NV];
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) s[j] = q[j] = 0.f;
+  #pragma unroll
+  for (int k = 0; k < ITER; ++k) {
+    if (piece_length(p, w, NV, w.pl + k * w.TP) > 0) {
+      float v[NV], g[NV];
+      X::values(rx[k], v);
+      widen(rg[k], g);
+      back_values<NV>(p, w.n, q0, v, g, f, tol);
+      #pragma unroll
+      for (int j = 0; j < NV; ++j) { s[j] += g[j]; q[j] = fmaf(g[j], v[j], q[j]); }
+    }
+    forget(rx[k]);
+    forget(rg[k]);
+  }
+  slab_sums<float, NV>(s, buf, s0, w, p.S);
+  slab_sums<float, NV>(q, buf, s1, w, p.S);
+  // positions -> channels (dz, dz xh) for the parameters; then weighted, for the groups
+  const int reps = p.L / p.C, span = min(p.S, p.L - w.base);
+  for (int i = threadIdx.x; i < (reps > 1 ? p.C : span); i += B) {
+    const int c = reps > 1 ? i : w.base + i;
+    const double* st = p.stats + ((long long)w.n * p.G + c / p.D) * 2;
+    double a = 0.0, b = 0.0;
+    for (int r = 0; r < reps; ++r) { a += s0[r * p.C + i]; b += s1[r * p.C + i]; }
+    b = sum_xh(st, a, b);
+    const double ga = p.gamma ? load_param(p.gamma, p.param_bf16, c) : 1.0;
+    s0[i] = ga * a;
+    s1[i] = ga * b;
+    for (int r = 1; r < reps; ++r) s0[r * p.C + i] = s1[r * p.C + i] = 0.0;
+    if (p.N > 1) {
+      p.chan[((long long)w.n * p.C + c) * 2] = a;
+      p.chan[((long long)w.n * p.C + c) * 2 + 1] = b;
+    } else {
+      if (p.dbeta) store_param(p.dbeta, p.grad_bf16, c, (float)a, p.accumulate);
+      if (p.dgamma) store_param(p.dgamma, p.grad_bf16, c, (float)b, p.accumulate);
+    }
+  }
+  if (!p.out) return;
+  __syncthreads();
+  const int first = reps > 1 ? 0 : w.base / p.D;
+  const double inv = 1.0 / ((double)(p.E / p.C) * p.D);
+  slab_groups(p, w, s0, s1, [&](int g, double a, double b) {
+    const double* st = p.stats + ((long long)w.n * p.G + g) * 2;
+    const DxCoef d = dx_coef(st[0], st[1], a * inv, b * inv);
+    s0[(g - first) * p.D] = d.c0;
+    s1[(g - first) * p.D] = d.c1;
+  });
+  __syncthreads();
+  if (!w.on) return;
+  DxCoef kc[NV];
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int l = ((w.q0 + j) % p.C / p.D - first) * p.D;
+    kc[j].c0 = (float)s0[l];
+    kc[j].c1 = (float)s1[l];
+  }
+  TX* dx = reinterpret_cast<TX*>(p.out) + (long long)w.n * p.E + w.q0;
+  #pragma unroll
+  for (int k = 0; k < ITER; ++k) {
+    const int row = w.pl + k * w.TP, have = piece_length(p, w, NV, row);
+    if (have > 0) {
+      float v[NV], g[NV];
+      X::values(rx[k], v);
+      widen(rg[k], g);
+      back_values<NV>(p, w.n, w.q0, v, g, f, tol);
+      #pragma unroll
+      for (int j = 0; j < NV; ++j) v[j] = fmaf(g[j], f[j].a, -fmaf(v[j], kc[j].c1, kc[j].c0));
+      store_some<TX, NV>(dx + (long long)row * p.L, have, v);
+    }
+  }
+}
+
 // ---- the 8-bit form on its own ------------------------------------------------------------------------------------
 
 // A lane takes one 16-byte piece of x; 4 (bfloat16) or 8 (float) neighbouring lanes make a block of 32 channels.  Pieces are
@@ -662,6 +901,27 @@ bool cut(Params& p, int N, long long hw, int C, int G, int x_bf16) {
   return (long long)N * p.chunks * p.slabs + (C + 31) / 32 <= 0x7fffffffLL && (long long)N * G <= 0x7fffffffLL;
 }
 
+// The slab kernels' cut: the fewest positions that hold whole groups, whole pieces (`unit`) and 32 channels, more of them where
+// a thread would not have its first piece yet and there are workgroups to spare.  False: an image does not fit
+// the registers of a workgroup, and the chunked kernels take it.
+struct SlabPlan { int S, slabs, threads, iter; };
+bool slab_plan(const Params& p, int nv, int most, SlabPlan& q) {
+  int unit = p.L > p.C ? p.L : p.D / gcd(p.D, nv) * nv;
+  if (p.codes_out) unit = unit / gcd(unit, C8_BLOCK) * C8_BLOCK;
+  if (unit > SLAB_MAX) return false;
+  int S = std::min(p.L, (C8_BLOCK + unit - 1) / unit * unit);
+  while (2 * S <= p.L && 2 * S <= SLAB_MAX && (long long)(2 * S / nv) * p.rows <= 256 && (long long)p.N * ((p.L + 2 * S - 1) / (2 * S)) >= 256) S *= 2;
+  if (S > SLAB_MAX) return false;
+  q.S = S;
+  q.slabs = (p.L + S - 1) / S;
+  static const int forms[4][2] = {{256, 1}, {256, 4}, {512, 8}, {1024, 4}};      // (as many pieces in registers as spill nothing)
+  for (int k = 0; k < 4; ++k) {
+    const int tp = forms[k][0] / (S / nv);
+    if (k < 2 || k == most) if (tp > 0 && (long long)tp * forms[k][1] >= p.rows) { q.threads = forms[k][0]; q.iter = forms[k][1]; return true; }
+  }
+  return false;
+}
+
 size_t part_bytes(const Params& p, bool backward) {
   return (size_t)p.N * p.chunks * 2 * p.L * (backward ? 4 : 8);
 }
@@ -681,8 +941,28 @@ int pack(const void* x, long long rows, int C, int nblk, long long ld, signed ch
   return status();
 }
 
+template <typename TX, typename TY, int B, int ITER>
+void forward_slabs(const Params& p, hipStream_t stream) {
+  const dim3 grid((unsigned)((long long)p.N * p.slabs));
+  if (p.codes_out) SG2IM_LAUNCH((fwd_slab_kernel<TX, TY, true, B, ITER>), grid, dim3(B), 0, stream, p);
+  else SG2IM_LAUNCH((fwd_slab_kernel<TX, TY, false, B, ITER>), grid, dim3(B), 0, stream, p);
+}
+template <typename SRC, typename TX, typename TY, bool EVEN, int B, int ITER>
+void backward_slabs(const Params& p, hipStream_t stream) {
+  SG2IM_LAUNCH((bwd_slab_kernel<SRC, TX, TY, EVEN, B, ITER>), dim3((unsigned)((long long)p.N * p.slabs)), dim3(B), 0, stream, p);
+}
+
 template <typename TX, typename TY>
-void launch_forward(const Params& p, hipStream_t stream) {
+void launch_forward(const Params& p0, hipStream_t stream) {
+  Params p = p0;
+  SlabPlan q;
+  if (slab_plan(p, VecOf<TX>::n, 3, q)) {
+    p.S = q.S; p.slabs = q.slabs;
+    if (q.iter == 1) forward_slabs<TX, TY, 256, 1>(p, stream);
+    else if (q.threads == 256) forward_slabs<TX, TY, 256, 4>(p, stream);
+    else forward_slabs<TX, TY, 1024, 4>(p, stream);
+    return;
+  }
   const unsigned blocks = (unsigned)((long long)p.N * p.chunks * p.slabs);
   SG2IM_LAUNCH(fwd_partial_kernel<TX>, dim3(blocks), dim3(THREADS), 0, stream, p);
   const long long per = (long long)p.chunks * (p.L / p.C) * p.D;
@@ -693,7 +973,19 @@ void launch_forward(const Params& p, hipStream_t stream) {
 }
 
 template <typename SRC, typename TX, typename TY, bool EVEN>
-void launch_backward(const Params& p, bool need_dx, bool need_params, hipStream_t stream) {
+void launch_backward(const Params& p0, bool need_dx, bool need_params, hipStream_t stream) {
+  Params p = p0;
+  SlabPlan q;
+  constexpr int LARGE = sizeof(TX) == 4 ? 3 : EVEN ? 2 : 0;
+  if (slab_plan(p, VecOf<TX>::n, LARGE, q)) {
+    p.S = q.S; p.slabs = q.slabs;
+    if (q.iter == 1) backward_slabs<SRC, TX, TY, EVEN, 256, 1>(p, stream);
+    else if (q.threads == 256) backward_slabs<SRC, TX, TY, EVEN, 256, 4>(p, stream);
+    else if constexpr (LARGE == 2) backward_slabs<SRC, TX, TY, EVEN, 512, 8>(p, stream);
+    else if constexpr (LARGE == 3) backward_slabs<SRC, TX, TY, EVEN, 1024, 4>(p, stream);
+    if (p.N > 1 && need_params) SG2IM_LAUNCH(param_grads_kernel, dim3((p.C + 31) / 32), dim3(THREADS), 0, stream, p);
+    return;
+  }
   const long long blocks = (long long)p.N * p.chunks * p.slabs;
   SG2IM_LAUNCH((bwd_partial_kernel<SRC, TX, TY, EVEN>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
   const int gpb = p.D >= FIN_CH ? 1 : FIN_CH / p.D;
