@@ -704,7 +704,7 @@ int sg2im_unpack8(const signed char* codes, const unsigned char* exps, long long
  *   backward_data:    dx = dz W
  *   backward_weight:  dweight (+)= dz^T x, from x or from its 8-bit form (codes / exps, dense, of x's rows)
  * workspace: sg2im_linear_workspace bytes for `which` = 0 forward, 1 backward_data, 2 backward_weight, 3 backward_act.
- * Rows below 2^31 - 256; leading dimensions in elements; no alignment beyond an element's is assumed. */
+ * Rows below 2^31 - 256; k, n and the operands' leading dimensions (in elements) at most 2^22; no alignment beyond an element's is assumed. */
 size_t sg2im_linear_workspace(long long rows, int k, int n, int dtype, int which);
 int sg2im_linear_forward(const void* x, int dtype, long long ld_x, const void* weight, const void* bias, int bias_dtype,
                          const void* residual, long long ld_res, float slope, void* out, int out_dtype, long long ld_out,

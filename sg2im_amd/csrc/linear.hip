@@ -8,10 +8,14 @@
 //
 // All three products are C[i][j] = sum_r A(i, r) B(j, r); an operand lies in memory either with r contiguous (x and W of
 // the forward product, dz of dx) or with i / j contiguous (W of dx, both of dW).  A tile goes from memory through registers
-// into LDS in the order it lies in; the operands of v_mfma_f32_32x32x16_bf16 (8 consecutive r of one row per lane) are read
-// with ds_read_b128 from the first kind and with the transposing ds_read_b64_tr_b16 from the second.  float32 uses
-// v_mfma_f32_32x32x2_f32 on the same tiles.  The operands are swapped (B's tile in the instruction's rows), so that a lane
-// ends with four consecutive columns of one output row.
+// into LDS in the order it lies in (so any alignment, any width and the 8-bit form are only a matter of the load); the
+// operands of v_mfma_f32_32x32x16_bf16 (8 consecutive r of one row per lane) are read with ds_read_b128 from the first kind
+// and with the transposing ds_read_b64_tr_b16 from the second.  float32 uses v_mfma_f32_32x32x2_f32 on the same tiles.
+//
+// Four waves share a tile of BM x BN and each computes a quarter.  The reduction advances in chunks of 128 bytes of r, with
+// two LDS images of each operand: while the matrix cores work on chunk c, chunk c + 1 is written to the other image and
+// chunk c + 2 is on its way from memory; operands of the next step are read during the current one, also across the one
+// barrier per chunk.
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include "sg2im_hip.h"
@@ -29,13 +33,14 @@ enum { RC = 0, RM = 1, RM8 = 2 };        // r contiguous; i / j contiguous; the 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+#define SG2IM_FENCE() __builtin_amdgcn_sched_barrier(0)
 
 struct Product {
   const void* a; const void* b;
   const unsigned char* b_exps; int b_nblk;       // RM8
   long long lda, ldb;
   int I, J, R;                                   // rows, columns, reduction
-  int tiles_j, splits, r_per_split;
+  int tiles_i, tiles_j, splits, r_per_split;
   float* part;                                   // [splits][I][J], splits > 1
   // epilogue
   const void* bias; int bias_bf16;
@@ -49,7 +54,11 @@ struct Product {
 template <typename T> struct Geo;
 template <> struct Geo<bf16_s> { static constexpr int BK = 64, NV = 8; };
 template <> struct Geo<float> { static constexpr int BK = 32, NV = 4; };
+constexpr int STEPS = 4;                         // per chunk: 16 r of bfloat16, 8 of float
 
+// the LDS image of ROWS rows of an operand by one chunk.  Strides: 144 bytes (36 banks: the 16 rows of a b128 phase start on
+// 16 different bank quads); columns + 64 bytes (the 4 rows of a transposing read lie on different quarters of the banks) or,
+// for float32, + 32 bytes (rows 4 apart lie on different halves)
 template <typename T, int ROWS, int MODE> struct Tile {
   static constexpr int BK = Geo<T>::BK, NV = Geo<T>::NV;
   static constexpr int LD = MODE == RC ? BK + NV : ROWS + (sizeof(T) == 2 ? 32 : 8);
@@ -58,70 +67,132 @@ template <typename T, int ROWS, int MODE> struct Tile {
 };
 
 struct Piece { unsigned w[4]; };
+template <int MODE, int N> struct Staged { Piece v[N]; };
+template <int N> struct Staged<RM8, N> { unsigned q[N][2]; unsigned char e[N]; };      // codes (float: the first word) and exponent
 
-// one 16-byte piece of `have` valid elements
-template <typename T> __device__ __forceinline__ Piece load_piece(const T* p, int have) {
-  Piece r;
-  if (have >= Geo<T>::NV) { __builtin_memcpy(&r, p, 16); return r; }
-  r.w[0] = r.w[1] = r.w[2] = r.w[3] = 0;
-  if constexpr (sizeof(T) == 4) {
-    for (int j = 0; j < 4; ++j) if (j < have) r.w[j] = reinterpret_cast<const unsigned*>(p)[j];
-  } else {
-    for (int j = 0; j < 8; ++j) if (j < have) r.w[j >> 1] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[j] << (16 * (j & 1));
-  }
-  return r;
-}
-template <typename T> __device__ __forceinline__ Piece load_piece8(const signed char* c, const unsigned char* e, int col, int have) {
-  constexpr int NV = Geo<T>::NV;
-  Piece r;
-  r.w[0] = r.w[1] = r.w[2] = r.w[3] = 0;
-  if (have <= 0) return r;
-  const float s = c8_scale(e[col / C8_BLOCK]);   // (a piece starts at a multiple of its length: inside one block)
-  signed char q[NV];
-  if (have >= NV) __builtin_memcpy(q, c + col, NV);
-  else for (int j = 0; j < NV; ++j) q[j] = j < have ? c[col + j] : 0;
-  float v[NV];
-  #pragma unroll
-  for (int j = 0; j < NV; ++j) v[j] = c8_decode(q[j], s);
-  if constexpr (sizeof(T) == 4) { for (int j = 0; j < 4; ++j) r.w[j] = __float_as_uint(v[j]); }
-  else { for (int j = 0; j < 4; ++j) r.w[j] = f32_to_bf16_bits(v[2 * j]) | (unsigned)f32_to_bf16_bits(v[2 * j + 1]) << 16; }
-  return r;
-}
-
-// memory -> registers: rows [row0, row0 + ROWS) of an operand with `rows` rows, r in [r0, r0 + BK) below r_end
-template <typename T, int ROWS, int MODE>
-__device__ __forceinline__ void fetch(Piece (&out)[ROWS / 32], const void* src, long long ld, const unsigned char* exps, int nblk,
-                                      int row0, int rows, int r0, int r_end) {
-  typedef Tile<T, ROWS, MODE> G;
-  constexpr int NV = G::NV;
-  const int tid = threadIdx.x;
-  #pragma unroll
-  for (int i = 0; i < G::PIECES; ++i) {
-    if constexpr (MODE == RC) {
-      const int row = row0 + (tid >> 3) + 32 * i, r = r0 + (tid & 7) * NV;
-      out[i] = load_piece<T>(reinterpret_cast<const T*>(src) + (long long)row * ld + r, row < rows ? r_end - r : 0);
-    } else {
-      constexpr int PR = ROWS / NV;              // pieces per r
-      const int r = r0 + tid / PR + (THREADS / PR) * i, col = row0 + tid % PR * NV;
-      const int have = r < r_end ? rows - col : 0;
-      if constexpr (MODE == RM) out[i] = load_piece<T>(reinterpret_cast<const T*>(src) + (long long)r * ld + col, have);
-      else out[i] = load_piece8<T>(reinterpret_cast<const signed char*>(src) + (long long)r * ld, exps + (long long)r * nblk, col, have);
+// the first `have` elements of a piece, zeros behind them
+template <typename T> __device__ __forceinline__ Piece load_part(const T* p, int have) {
+  Piece r = {{0, 0, 0, 0}};
+  if (have >= Geo<T>::NV) {
+    __builtin_memcpy(&r.w[0], p, 16);
+  } else if (have > 0) {
+    // (an element behind the end reads the last one instead and is dropped: no branch per element)
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        const unsigned w = reinterpret_cast<const unsigned*>(p)[min(j, have - 1)];
+        r.w[j] = j < have ? w : 0;
+      } else {
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+        const unsigned lo = h[min(2 * j, have - 1)], hi = h[min(2 * j + 1, have - 1)];
+        r.w[j] = (2 * j < have ? lo : 0) | (2 * j + 1 < have ? hi << 16 : 0);
+      }
     }
   }
+  return r;
 }
 
-template <typename T, int ROWS, int MODE>
-__device__ __forceinline__ void stage(T* lds, const Piece (&in)[ROWS / 32]) {
+// One operand's way from memory to LDS: ROWS rows from row0, chunk by chunk.
+//   whole: every piece of every full chunk lies inside the operand (the rows of an r-contiguous one are clamped: what a row
+//   behind the last one computes is not stored), so that loads need no check
+template <typename T, int ROWS, int MODE> struct Feeder {
   typedef Tile<T, ROWS, MODE> G;
-  const int tid = threadIdx.x;
-  #pragma unroll
-  for (int i = 0; i < G::PIECES; ++i) {
-    T* p;
-    if constexpr (MODE == RC) p = lds + ((tid >> 3) + 32 * i) * G::LD + (tid & 7) * G::NV;
-    else { constexpr int PR = ROWS / G::NV; p = lds + (tid / PR + (THREADS / PR) * i) * G::LD + tid % PR * G::NV; }
-    *reinterpret_cast<uint4*>(p) = make_uint4(in[i].w[0], in[i].w[1], in[i].w[2], in[i].w[3]);
+  static constexpr int NV = G::NV, P = G::PIECES;
+  static constexpr int PR = ROWS / NV;                     // pieces per r (i / j contiguous)
+  const char* base;                                        // this chunk
+  const unsigned char* exps;                               // RM8: this chunk's row of exponents
+  unsigned off[MODE == RC ? P : 1];                        // bytes from base
+  long long ld;
+  int rows, row0, nblk;
+  __device__ __forceinline__ Feeder(const void* src, long long ld_, const unsigned char* e, int nblk_, int row0_, int rows_, int r0)
+    : ld(ld_), rows(rows_), row0(row0_), nblk(nblk_) {
+    const int tid = threadIdx.x;
+    if constexpr (MODE == RC) {
+      base = reinterpret_cast<const char*>(src) + ((long long)row0 * ld + r0) * (int)sizeof(T);
+      #pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int row = min((tid >> 3) + 32 * i, rows - 1 - row0);
+        off[i] = (unsigned)(row * (unsigned)ld + (tid & 7) * NV) * (unsigned)sizeof(T);
+      }
+    } else {
+      const int size = MODE == RM8 ? 1 : (int)sizeof(T);
+      base = reinterpret_cast<const char*>(src) + ((long long)r0 * ld + row0) * size;
+      off[0] = (unsigned)((tid / PR) * (unsigned)ld + tid % PR * NV) * (unsigned)size;
+      exps = e + (long long)r0 * nblk;
+    }
   }
-}
+  __device__ __forceinline__ bool whole() const { return MODE == RC || row0 + ROWS <= rows; }
+  __device__ __forceinline__ void next() {
+    if constexpr (MODE == RC) base += 128;
+    else {
+      base += G::BK * ld * (MODE == RM8 ? 1 : (int)sizeof(T));
+      if constexpr (MODE == RM8) exps += (long long)G::BK * nblk;
+    }
+  }
+  // pieces [I0, I1) of a full chunk of a whole tile
+  template <int I0, int I1> __device__ __forceinline__ void load(Staged<MODE, P>& s) const {
+    #pragma unroll
+    for (int i = I0; i < I1; ++i) {
+      if constexpr (MODE == RC) __builtin_memcpy(&s.v[i], base + off[i], 16);
+      else {
+        const char* at = base + (long long)(THREADS / PR * i) * ld * (MODE == RM8 ? 1 : (int)sizeof(T)) + off[0];
+        if constexpr (MODE == RM) __builtin_memcpy(&s.v[i], at, 16);
+        else {
+          __builtin_memcpy(s.q[i], at, NV);
+          s.e[i] = exps[(long long)(threadIdx.x / PR + THREADS / PR * i) * nblk + (row0 + (int)(threadIdx.x % PR) * NV) / C8_BLOCK];
+        }
+      }
+    }
+  }
+  // any chunk: `left` = how many r there are
+  __device__ __forceinline__ void load_checked(Staged<MODE, P>& s, int left) const {
+    const int tid = threadIdx.x;
+    #pragma unroll
+    for (int i = 0; i < P; ++i) {
+      if constexpr (MODE == RC) {
+        s.v[i] = load_part<T>(reinterpret_cast<const T*>(base + off[i]), row0 + (tid >> 3) + 32 * i < rows ? left - (tid & 7) * NV : 0);
+      } else {
+        const int r = tid / PR + THREADS / PR * i, col = row0 + tid % PR * NV, have = r < left ? rows - col : 0;
+        const char* at = base + (long long)(THREADS / PR * i) * ld * (MODE == RM8 ? 1 : (int)sizeof(T)) + off[0];
+        if constexpr (MODE == RM) s.v[i] = load_part<T>(reinterpret_cast<const T*>(at), have);
+        else {
+          s.q[i][0] = s.q[i][1] = 0;
+          s.e[i] = 127;
+          if (have > 0) {
+            #pragma unroll
+            for (int j = 0; j < NV; ++j) {
+              const unsigned q = (unsigned char)at[min(j, have - 1)];
+              s.q[i][j >> 2] |= (j < have ? q : 0) << (8 * (j & 3));
+            }
+            s.e[i] = exps[(long long)r * nblk + col / C8_BLOCK];
+          }
+        }
+      }
+    }
+  }
+  template <int I0, int I1> __device__ __forceinline__ void store(T* lds, const Staged<MODE, P>& s) const {
+    const int tid = threadIdx.x;
+    #pragma unroll
+    for (int i = I0; i < I1; ++i) {
+      T* p;
+      if constexpr (MODE == RC) p = lds + ((tid >> 3) + 32 * i) * G::LD + (tid & 7) * NV;
+      else p = lds + (tid / PR + THREADS / PR * i) * G::LD + tid % PR * NV;
+      uint4 w;
+      if constexpr (MODE == RM8) {
+        const float scale = c8_scale(s.e[i]);              // (a piece starts at a multiple of its length: one block)
+        float v[NV];
+        #pragma unroll
+        for (int j = 0; j < NV; ++j) v[j] = c8_decode((signed char)(s.q[i][j >> 2] >> (8 * (j & 3))), scale);
+        if constexpr (sizeof(T) == 4) w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        else {
+          auto two = [&](int j) { return f32_to_bf16_bits(v[j]) | (unsigned)f32_to_bf16_bits(v[j + 1]) << 16; };
+          w = make_uint4(two(0), two(2), two(4), two(6));
+        }
+      } else w = make_uint4(s.v[i].w[0], s.v[i].w[1], s.v[i].w[2], s.v[i].w[3]);
+      *reinterpret_cast<uint4*>(p) = w;
+    }
+  }
+};
 
 // 8 consecutive r (16 step + 8 (lane / 32) ..) of row row0 + lane % 32
 template <int ROWS, int MODE>
@@ -160,45 +231,70 @@ __device__ __forceinline__ f32x16 multiply(const float4& a, const float4& b, f32
   return __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, b.w, c, 0, 0, 0);
 }
 
-// four consecutive columns of output row i; returns their z > 0 bits
-template <typename TO>
-__device__ __forceinline__ unsigned finish4(const Product& p, int i, int j, float (&v)[4]) {
+// NC consecutive columns of output row i from j on, all of them inside; returns their z > 0 bits
+template <typename TO, int NC>
+__device__ __forceinline__ unsigned finish(const Product& p, int i, int j, float (&v)[NC]) {
   unsigned bits = 0;
-  const int have = min(4, p.J - j);
-  if (i >= p.I || have <= 0) return 0;
+  if (p.bias) {
+    float b[NC];
+    if (p.bias_bf16) load_vec<bf16_s, NC>(reinterpret_cast<const bf16_s*>(p.bias) + j, b);
+    else load_vec<float, NC>(reinterpret_cast<const float*>(p.bias) + j, b);
+    #pragma unroll
+    for (int t = 0; t < NC; ++t) v[t] += b[t];
+  }
   #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    if (p.bias && t < have) v[t] += load_param(p.bias, p.bias_bf16, j + t);
-    if (v[t] > 0.f && t < have) bits |= 1u << t;
+  for (int t = 0; t < NC; ++t) {
+    if (v[t] > 0.f) bits |= 1u << t;
     v[t] = v[t] > 0.f ? v[t] : v[t] * p.slope;
   }
   TO* out = reinterpret_cast<TO*>(p.out) + (long long)i * p.ld_out + j;
   const TO* res = p.residual ? reinterpret_cast<const TO*>(p.residual) + (long long)i * p.ld_res + j : p.accumulate ? out : nullptr;
-  if (have == 4) {
-    if (res) {
-      float r[4];
-      load_vec<TO, 4>(res, r);
-      #pragma unroll
-      for (int t = 0; t < 4; ++t) v[t] += r[t];
-    }
-    store_vec<TO, 4>(out, v);
-  } else {
-    for (int t = 0; t < have; ++t) store1(out + t, res ? v[t] + load1(res + t) : v[t]);
+  if (res) {
+    float r[NC];
+    load_vec<TO, NC>(res, r);
+    #pragma unroll
+    for (int t = 0; t < NC; ++t) v[t] += r[t];
   }
+  store_vec<TO, NC>(out, v);
   return bits;
+}
+template <typename TO>
+__device__ __forceinline__ unsigned finish_one(const Product& p, int i, int j, float v) {
+  if (p.bias) v += load_param(p.bias, p.bias_bf16, j);
+  const unsigned bit = v > 0.f;
+  if (!bit) v *= p.slope;
+  TO* out = reinterpret_cast<TO*>(p.out) + (long long)i * p.ld_out + j;
+  if (p.residual) v += load1(reinterpret_cast<const TO*>(p.residual) + (long long)i * p.ld_res + j);
+  else if (p.accumulate) v += load1(out);
+  store1(out, v);
+  return bit;
 }
 
 template <typename T, typename TO, int BM, int BN, int AMODE, int BMODE>
-__global__ __launch_bounds__(THREADS) void product_kernel(const Product p) {
+__global__ __launch_bounds__(THREADS, BM * BN >= 256 * 256 ? 1 : 2) void product_kernel(const Product p) {
+  typedef Feeder<T, BM, AMODE> FA;
+  typedef Feeder<T, BN, BMODE> FB;
   typedef Tile<T, BM, AMODE> GA;
   typedef Tile<T, BN, BMODE> GB;
-  constexpr int BK = GA::BK, TI = BM / 64, TJ = BN / 64, STEPS = sizeof(T) == 2 ? BK / 16 : BK / 8;
-  __shared__ __attribute__((aligned(16))) T lds_a[GA::ELEMS], lds_b[GB::ELEMS];
-  const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits;
-  const int i0 = tile / p.tiles_j * BM, j0 = tile % p.tiles_j * BN;
+  constexpr int BK = GA::BK, TI = BM / 64, TJ = BN / 64;
+  constexpr int EP = BN / 2 + 4;                                   // floats of an epilogue row (4 banks apart, 32 rows per wave)
+  constexpr int BYTES = 2 * (GA::ELEMS + GB::ELEMS) * (int)sizeof(T), EP_BYTES = 4 * 32 * EP * 4;
+  __shared__ __attribute__((aligned(16))) char lds[BYTES > EP_BYTES ? BYTES : EP_BYTES];
+  T* lds_a = reinterpret_cast<T*>(lds);
+  T* lds_b = lds_a + 2 * GA::ELEMS;
+  // Workgroups go round robin over the 8 XCDs: a contiguous run of tiles each, four rows of tiles at a time, so that the
+  // workgroups that share an L2 share operands
+  const int tiles = p.tiles_i * p.tiles_j, blocks = tiles * p.splits;
+  int id = blockIdx.x;
+  if (blocks % 8 == 0) id = id % 8 * (blocks / 8) + id / 8;
+  const int split = id / tiles, tile = id - split * tiles;
+  const int group = tile / (4 * p.tiles_j), in = tile - group * 4 * p.tiles_j, gi = min(4, p.tiles_i - 4 * group);
+  const int i0 = (4 * group + in % gi) * BM, j0 = in / gi * BN;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int wi = (wave >> 1) * (BM / 2), wj = (wave & 1) * (BN / 2);
-  const int r_begin = split * p.r_per_split, r_end = min(p.R, r_begin + p.r_per_split);
+  const int r_begin = split * p.r_per_split, length = min(p.R - r_begin, p.r_per_split);
+  const int chunks = (length + BK - 1) / BK, full = length / BK;
+
   f32x16 acc[TI][TJ];
   #pragma unroll
   for (int a = 0; a < TI; ++a)
@@ -206,57 +302,154 @@ __global__ __launch_bounds__(THREADS) void product_kernel(const Product p) {
     for (int b = 0; b < TJ; ++b)
       #pragma unroll
       for (int v = 0; v < 16; ++v) acc[a][b][v] = 0.f;
-  Piece pa[GA::PIECES], pb[GB::PIECES];
-  fetch<T, BM, AMODE>(pa, p.a, p.lda, nullptr, 0, i0, p.I, r_begin, r_end);
-  fetch<T, BN, BMODE>(pb, p.b, p.ldb, p.b_exps, p.b_nblk, j0, p.J, r_begin, r_end);
-  for (int r = r_begin; r < r_end; r += BK) {
-    __syncthreads();
-    stage<T, BM, AMODE>(lds_a, pa);
-    stage<T, BN, BMODE>(lds_b, pb);
-    __syncthreads();
-    if (r + BK < r_end) {
-      fetch<T, BM, AMODE>(pa, p.a, p.lda, nullptr, 0, i0, p.I, r + BK, r_end);
-      fetch<T, BN, BMODE>(pb, p.b, p.ldb, p.b_exps, p.b_nblk, j0, p.J, r + BK, r_end);
-    }
+
+  FA fa(p.a, p.lda, nullptr, 0, i0, p.I, r_begin);
+  FB fb(p.b, p.ldb, p.b_exps, p.b_nblk, j0, p.J, r_begin);
+  Staged<AMODE, FA::P> sa;
+  Staged<BMODE, FB::P> sb;
+  const bool quick = fa.whole() && fb.whole();
+  int fetched = 0;                                                 // chunks on their way so far
+  auto fetch_quick = [&]() {
+    fa.template load<0, FA::P>(sa);
+    fb.template load<0, FB::P>(sb);
+    fa.next(); fb.next();
+    ++fetched;
+  };
+  auto fetch = [&]() {
+    if (quick && fetched < full) { fetch_quick(); return; }
+    fa.load_checked(sa, length - fetched * BK);
+    fb.load_checked(sb, length - fetched * BK);
+    fa.next(); fb.next();
+    ++fetched;
+  };
+  auto put = [&](int image) {
+    fa.template store<0, FA::P>(lds_a + image * GA::ELEMS, sa);
+    fb.template store<0, FB::P>(lds_b + image * GB::ELEMS, sb);
+  };
+  auto put_half = [&](int image, int half) {
+    if (half == 0) { fa.template store<0, FA::P / 2>(lds_a + image * GA::ELEMS, sa); fb.template store<0, FB::P / 2>(lds_b + image * GB::ELEMS, sb); }
+    else { fa.template store<FA::P / 2, FA::P>(lds_a + image * GA::ELEMS, sa); fb.template store<FB::P / 2, FB::P>(lds_b + image * GB::ELEMS, sb); }
+  };
+  typedef decltype(operand<BM, AMODE>(lds_a, 0, 0, 0)) Op;
+  Op oa[2][TI], ob[2][TJ];
+  auto read = [&](int into, int image, int step) {
     #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      decltype(operand<BM, AMODE>(lds_a, 0, 0, 0)) fa[TI], fb[TJ];
+    for (int a = 0; a < TI; ++a) oa[into][a] = operand<BM, AMODE>(lds_a + image * GA::ELEMS, wi + 32 * a, step, lane);
+    #pragma unroll
+    for (int b = 0; b < TJ; ++b) ob[into][b] = operand<BN, BMODE>(lds_b + image * GB::ELEMS, wj + 32 * b, step, lane);
+  };
+  auto compute = [&](int from) {
+    #pragma unroll
+    for (int a = 0; a < TI; ++a)
       #pragma unroll
-      for (int a = 0; a < TI; ++a) fa[a] = operand<BM, AMODE>(lds_a, wi + 32 * a, s, lane);
-      #pragma unroll
-      for (int b = 0; b < TJ; ++b) fb[b] = operand<BN, BMODE>(lds_b, wj + 32 * b, s, lane);
-      #pragma unroll
-      for (int a = 0; a < TI; ++a)
-        #pragma unroll
-        for (int b = 0; b < TJ; ++b) acc[a][b] = multiply(fb[b], fa[a], acc[a][b]);
+      for (int b = 0; b < TJ; ++b) acc[a][b] = multiply(ob[from][b], oa[from][a], acc[a][b]);
+  };
+
+  if (chunks > 0) {
+    fetch();
+    put(0);
+    if (chunks > 1) fetch();
+    __syncthreads();
+    read(0, 0, 0);
+    int c = 0;
+    if (quick)
+      for (; c + 2 < full; ++c) {                                  // (the same as below without its questions)
+        const int image = c & 1;
+        // (the fences keep the reads of the next step and the traffic with memory in front of a step's products, where the
+        // compiler would move each of them next to its use)
+        read(1, image, 1);
+        put_half(image ^ 1, 0);
+        SG2IM_FENCE();
+        compute(0);
+        SG2IM_FENCE();
+        read(0, image, 2);
+        put_half(image ^ 1, 1);
+        SG2IM_FENCE();
+        compute(1);
+        SG2IM_FENCE();
+        read(1, image, 3);
+        fetch_quick();
+        SG2IM_FENCE();
+        compute(0);
+        __syncthreads();
+        read(0, image ^ 1, 0);
+        SG2IM_FENCE();
+        compute(1);
+        SG2IM_FENCE();
+      }
+    for (; c < chunks; ++c) {
+      const int image = c & 1;
+      read(1, image, 1);
+      if (c + 1 < chunks) put(image ^ 1);
+      compute(0);
+      read(0, image, 2);
+      if (c + 2 < chunks) fetch();
+      compute(1);
+      read(1, image, 3);
+      compute(0);
+      __syncthreads();
+      if (c + 1 < chunks) read(0, image ^ 1, 0);
+      compute(1);
     }
   }
-  #pragma unroll
-  for (int a = 0; a < TI; ++a) {
-    const int i = i0 + wi + 32 * a + (lane & 31);
+
+  if (p.splits > 1) {
     #pragma unroll
-    for (int b = 0; b < TJ; ++b) {
-      const int jb = j0 + wj + 32 * b;
-      unsigned bits = 0;
+    for (int a = 0; a < TI; ++a) {
+      const int i = i0 + wi + 32 * a + (lane & 31);
       #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int j = jb + 8 * q + 4 * (lane >> 5);
-        float v[4] = {acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]};
-        if (p.splits > 1) {
+      for (int b = 0; b < TJ; ++b)
+        #pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int j = j0 + wj + 32 * b + 8 * q + 4 * (lane >> 5);
+          float v[4] = {acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]};
           if (i < p.I) {
             float* out = p.part + ((long long)split * p.I + i) * p.J + j;
             if (j + 4 <= p.J) store_vec<float, 4>(out, v);
-            else for (int t = 0; t < 4; ++t) if (j + t < p.J) out[t] = v[t];
+            else {
+              #pragma unroll
+              for (int t = 0; t < 4; ++t) if (j + t < p.J) out[t] = v[t];
+            }
           }
-        } else {
-          bits |= finish4<TO>(p, i, j, v) << (8 * q + 4 * (lane >> 5));
         }
+    }
+    return;
+  }
+  // A lane holds scattered fours of one row; 32 rows at a time go through the wave's own part of LDS, so that 8 (4) lanes
+  // then hold whole runs of a row and bias, residual and output are read and written in 16-byte pieces
+  constexpr int NC = 8, LANES = BN / 2 / NC;                       // lanes per row
+  __syncthreads();
+  float* mine = reinterpret_cast<float*>(lds) + wave * 32 * EP;
+  #pragma unroll
+  for (int a = 0; a < TI; ++a) {
+    #pragma unroll
+    for (int b = 0; b < TJ; ++b)
+      #pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<float4*>(mine + (lane & 31) * EP + 32 * b + 8 * q + 4 * (lane >> 5)) =
+            make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
+    __builtin_amdgcn_wave_barrier();
+    #pragma unroll
+    for (int k = 0; k < 32 * LANES / 64; ++k) {
+      const int row = k * (64 / LANES) + lane / LANES, col = lane % LANES * NC;
+      const float* from = mine + row * EP + col;
+      const int i = i0 + wi + 32 * a + row, j = j0 + wj + col;
+      unsigned bits = 0;
+      if (i < p.I && j + NC <= p.J) {
+        const float4 lo = *reinterpret_cast<const float4*>(from), hi = *reinterpret_cast<const float4*>(from + 4);
+        float v[NC] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        bits = finish<TO, NC>(p, i, j, v);
+      } else if (i < p.I) {
+        for (int t = 0; j + t < p.J; ++t) bits |= finish_one<TO>(p, i, j + t, from[t]) << t;
       }
-      if (p.splits == 1 && p.signs) {
-        bits |= __shfl_xor(bits, 32);
-        if (lane < 32 && i < p.I && jb < p.J) p.signs[(long long)i * p.sign_words + jb / 32] = bits;
+      bits <<= 8 * (lane & 3);
+      if (p.signs) {
+        bits |= __shfl_xor(bits, 1);
+        bits |= __shfl_xor(bits, 2);
+        if ((lane & 3) == 0 && i < p.I && j < p.J) p.signs[(long long)i * p.sign_words + j / 32] = bits;
       }
     }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -270,18 +463,25 @@ __global__ __launch_bounds__(THREADS) void join_kernel(const Product p) {
     const long long word = at >> 3;
     const int i = (int)(word / words), w = (int)(word - (long long)i * words), j = w * 32 + (int)(at & 7) * 4;
     unsigned bits = 0;
-    if (at < pieces && j < p.J) {
+    if (at < pieces && j + 4 <= p.J) {
       float v[4] = {0.f, 0.f, 0.f, 0.f};
       const float* src = p.part + (long long)i * p.J + j;
-      for (int s = 0; s < p.splits; ++s, src += plane) {
-        float u[4] = {0.f, 0.f, 0.f, 0.f};
-        if (j + 4 <= p.J) load_vec<float, 4>(src, u);
-        else for (int t = 0; t < 4; ++t) if (j + t < p.J) u[t] = src[t];
+      #pragma unroll 8
+      for (int s = 0; s < p.splits; ++s) {
+        float u[4];
+        load_vec<float, 4>(src + s * plane, u);
         #pragma unroll
         for (int t = 0; t < 4; ++t) v[t] += u[t];
       }
-      bits = finish4<TO>(p, i, j, v) << (4 * (int)(at & 7));
+      bits = finish<TO, 4>(p, i, j, v);
+    } else if (at < pieces) {
+      for (int t = 0; j + t < p.J; ++t) {
+        float v = 0.f;
+        for (int s = 0; s < p.splits; ++s) v += p.part[s * plane + (long long)i * p.J + j + t];
+        bits |= finish_one<TO>(p, i, j + t, v) << t;
+      }
     }
+    bits <<= 4 * (int)(at & 7);
     if (p.signs) {
       #pragma unroll
       for (int o = 1; o < 8; o <<= 1) bits |= __shfl_xor(bits, o);
@@ -336,7 +536,10 @@ __global__ __launch_bounds__(THREADS) void act_backward_kernel(const ActParams p
       if (p.dz) {
         TZ* dst = reinterpret_cast<TZ*>(p.dz) + m * p.N + c0;
         if (have == NV) store_vec<TZ, NV>(dst, g);
-        else for (int j = 0; j < have; ++j) store1(dst + j, g[j]);
+        else {
+          #pragma unroll
+          for (int j = 0; j < NV; ++j) if (j < have) store1(dst + j, g[j]);
+        }
       }
     }
   }
@@ -377,12 +580,12 @@ bool type_ok(int t) { return t == 0 || t == 1; }
 
 struct Plan { int tile, splits, r_per_split; };
 
-// 128 x 128 tiles where they fill the card, 64 x 64 below; the reduction is split where even those leave CUs idle.
+// 256 x 256 tiles where they fill the card, then 128 x 128, 64 x 64; the reduction is split where even those leave CUs idle.
 Plan plan(long long I, long long J, long long R, int bf16) {
   const int bk = bf16 ? 64 : 32;
   auto tiles = [&](int t) { return ((I + t - 1) / t) * ((J + t - 1) / t); };
   Plan q;
-  q.tile = tiles(128) >= 256 ? 128 : 64;
+  q.tile = tiles(256) >= 192 ? 256 : tiles(128) >= 256 ? 128 : 64;
   const long long steps = (R + bk - 1) / bk, n = std::max(1LL, tiles(q.tile));
   long long splits = std::max(1LL, std::min(std::min(512 / n, steps / 4), 64LL));
   const long long per = (steps + splits - 1) / splits;
@@ -396,10 +599,12 @@ int run(Product& p, const Plan& q, void* workspace, size_t workspace_bytes, hipS
   p.splits = q.splits; p.r_per_split = q.r_per_split;
   p.part = reinterpret_cast<float*>(workspace);
   if (q.splits > 1 && (!workspace || workspace_bytes < (size_t)q.splits * p.I * p.J * 4)) return SG2IM_ERR_ARG;
+  p.tiles_i = (p.I + q.tile - 1) / q.tile;
   p.tiles_j = (p.J + q.tile - 1) / q.tile;
-  const long long blocks = (long long)p.tiles_j * ((p.I + q.tile - 1) / q.tile) * q.splits;
+  const long long blocks = (long long)p.tiles_j * p.tiles_i * q.splits;
   if (blocks > 0x7fffffffLL) return SG2IM_ERR_ARG;
-  if (q.tile == 128) SG2IM_LAUNCH((product_kernel<T, TO, 128, 128, AMODE, BMODE>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
+  if (q.tile == 256) SG2IM_LAUNCH((product_kernel<T, TO, 256, 256, AMODE, BMODE>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
+  else if (q.tile == 128) SG2IM_LAUNCH((product_kernel<T, TO, 128, 128, AMODE, BMODE>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
   else SG2IM_LAUNCH((product_kernel<T, TO, 64, 64, AMODE, BMODE>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
   if (q.splits > 1) {
     const long long pieces = (long long)p.I * ((p.J + 31) / 32) * 8;
@@ -408,7 +613,9 @@ int run(Product& p, const Plan& q, void* workspace, size_t workspace_bytes, hipS
   return status();
 }
 
-bool sizes_ok(long long rows, int k, int n) { return rows >= 0 && rows <= 0x7fffffffLL - 256 && k >= 1 && n >= 1 && k <= (1 << 24) && n <= (1 << 24); }
+constexpr int LD_MAX = 1 << 22;      // (a tile's 256 rows stay within 32-bit byte offsets)
+bool ld_ok(long long ld, int cols) { return ld >= cols && ld <= LD_MAX; }
+bool sizes_ok(long long rows, int k, int n) { return rows >= 0 && rows <= 0x7fffffffLL - 256 && k >= 1 && n >= 1 && k <= LD_MAX && n <= LD_MAX; }
 
 ActParams act_plan(long long rows, int n) {
   ActParams p = {};
@@ -444,7 +651,7 @@ int sg2im_linear_forward(const void* x, int dtype, long long ld_x, const void* w
                          unsigned* signs, long long rows, int k, int n, void* workspace, size_t workspace_bytes,
                          hipStream_t stream) {
   if (!sizes_ok(rows, k, n) || !type_ok(dtype) || !type_ok(out_dtype) || !type_ok(bias_dtype) || (dtype == 0 && out_dtype == 1) ||
-      ld_x < k || ld_out < n || (residual && ld_res < n)) return SG2IM_ERR_ARG;
+      !ld_ok(ld_x, k) || ld_out < n || (residual && ld_res < n)) return SG2IM_ERR_ARG;
   if (rows == 0) return SG2IM_OK;
   if (!x || !weight || !out) return SG2IM_ERR_ARG;
   Product p = {};
@@ -481,7 +688,7 @@ int sg2im_linear_backward_act(const void* dy, int dy_dtype, long long ld_dy, con
 
 int sg2im_linear_backward_data(const void* dz, int dtype, long long ld_dz, const void* weight, void* dx, long long ld_dx,
                                long long rows, int k, int n, void* workspace, size_t workspace_bytes, hipStream_t stream) {
-  if (!sizes_ok(rows, k, n) || !type_ok(dtype) || ld_dz < n || ld_dx < k) return SG2IM_ERR_ARG;
+  if (!sizes_ok(rows, k, n) || !type_ok(dtype) || !ld_ok(ld_dz, n) || ld_dx < k) return SG2IM_ERR_ARG;
   if (rows == 0) return SG2IM_OK;
   if (!dz || !weight || !dx) return SG2IM_ERR_ARG;
   Product p = {};
@@ -496,8 +703,8 @@ int sg2im_linear_backward_weight(const void* dz, int dtype, long long ld_dz, con
                                  const signed char* codes, const unsigned char* exps, void* dweight, int dweight_dtype,
                                  int accumulate, long long rows, int k, int n, void* workspace, size_t workspace_bytes,
                                  hipStream_t stream) {
-  if (!sizes_ok(rows, k, n) || !type_ok(dtype) || !type_ok(dweight_dtype) || (dtype == 0 && dweight_dtype == 1) || ld_dz < n ||
-      !codes != !exps || (!codes && ld_x < k) || !dweight) return SG2IM_ERR_ARG;
+  if (!sizes_ok(rows, k, n) || !type_ok(dtype) || !type_ok(dweight_dtype) || (dtype == 0 && dweight_dtype == 1) ||
+      !ld_ok(ld_dz, n) || !codes != !exps || (!codes && !ld_ok(ld_x, k)) || !dweight) return SG2IM_ERR_ARG;
   if (rows > 0 && (!dz || (!x && !codes))) return SG2IM_ERR_ARG;
   Product p = {};
   p.a = dz; p.lda = ld_dz; p.I = n; p.J = k; p.R = (int)rows;

@@ -94,6 +94,7 @@ Tensor work(const Tensor& like, size_t bytes) {
 }
 
 // rows of t (..., C) as a matrix; a copy where they are not dense in memory
+constexpr int64_t LD_MAX = 1 << 22;      // (the products' limit)
 struct Rows { Tensor m; int64_t rows, cols, ld; };
 Rows rows_of(const Tensor& t, const char* what) {
   TORCH_CHECK_VALUE(t.dim() >= 1 && t.size(-1) >= 1, what, ": expected (..., channels), got ", t.sizes());
@@ -101,7 +102,7 @@ Rows rows_of(const Tensor& t, const char* what) {
   r.cols = t.size(-1);
   r.rows = t.numel() / r.cols;
   r.m = t.dim() == 2 ? t : t.is_contiguous() ? t.view({r.rows, r.cols}) : t.reshape({r.rows, r.cols});
-  if ((r.cols > 1 && r.m.stride(1) != 1) || (r.rows > 1 && r.m.stride(0) < r.cols)) r.m = r.m.contiguous();
+  if ((r.cols > 1 && r.m.stride(1) != 1) || (r.rows > 1 && (r.m.stride(0) < r.cols || r.m.stride(0) > LD_MAX))) r.m = r.m.contiguous();
   r.ld = r.rows > 1 ? r.m.stride(0) : r.cols;
   return r;
 }
