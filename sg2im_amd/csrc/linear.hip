@@ -270,6 +270,22 @@ __device__ __forceinline__ unsigned finish_one(const Product& p, int i, int j, f
   return bit;
 }
 
+// the schedule of a step: P products with the LDS reads, LDS writes and memory loads spread evenly between them
+template <int P, int READS, int WRITES, int LOADS, int K = 0>
+__device__ __forceinline__ void interleave() {
+  if constexpr (K < P) {
+    constexpr int r = (K + 1) * READS / P - K * READS / P, w = (K + 1) * WRITES / P - K * WRITES / P, l = (K + 1) * LOADS / P - K * LOADS / P;
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
+    if constexpr (w > 0) __builtin_amdgcn_sched_group_barrier(0x200, w, 0);
+    if constexpr (l > 0) __builtin_amdgcn_sched_group_barrier(0x020, l, 0);
+    interleave<P, READS, WRITES, LOADS, K + 1>();
+  }
+}
+// LDS reads of an operand, matrix instructions of a product
+template <typename T, int MODE> constexpr int READS_OF = MODE == RC ? 1 : sizeof(T) == 2 ? 2 : 4;
+template <typename T> constexpr int MFMAS_OF = sizeof(T) == 2 ? 1 : 4;
+
 template <typename T, typename TO, int BM, int BN, int AMODE, int BMODE>
 __global__ __launch_bounds__(THREADS, BM * BN >= 256 * 256 ? 1 : 2) void product_kernel(const Product p) {
   typedef Feeder<T, BM, AMODE> FA;
@@ -277,6 +293,7 @@ __global__ __launch_bounds__(THREADS, BM * BN >= 256 * 256 ? 1 : 2) void product
   typedef Tile<T, BM, AMODE> GA;
   typedef Tile<T, BN, BMODE> GB;
   constexpr int BK = GA::BK, TI = BM / 64, TJ = BN / 64;
+  constexpr int NP = TI * TJ * MFMAS_OF<T>, NR = TI * READS_OF<T, AMODE> + TJ * READS_OF<T, BMODE>, NL = FA::P + FB::P;
   constexpr int EP = BN / 2 + 4;                                   // floats of an epilogue row (4 banks apart, 32 rows per wave)
   constexpr int BYTES = 2 * (GA::ELEMS + GB::ELEMS) * (int)sizeof(T), EP_BYTES = 4 * 32 * EP * 4;
   __shared__ __attribute__((aligned(16))) char lds[BYTES > EP_BYTES ? BYTES : EP_BYTES];
@@ -355,26 +372,26 @@ __global__ __launch_bounds__(THREADS, BM * BN >= 256 * 256 ? 1 : 2) void product
     if (quick)
       for (; c + 2 < full; ++c) {                                  // (the same as below without its questions)
         const int image = c & 1;
-        // (the fences keep the reads of the next step and the traffic with memory in front of a step's products, where the
-        // compiler would move each of them next to its use)
+        // The order inside a step: the LDS and memory traffic spread between the products (left to itself the compiler moves
+        // each access next to its use, and the matrix cores wait for it)
         read(1, image, 1);
-        put_half(image ^ 1, 0);
-        SG2IM_FENCE();
+        put(image ^ 1);
         compute(0);
+        interleave<NP, NR, NL, 0>();
         SG2IM_FENCE();
         read(0, image, 2);
-        put_half(image ^ 1, 1);
-        SG2IM_FENCE();
+        fetch_quick();
         compute(1);
+        interleave<NP, NR, 0, NL>();
         SG2IM_FENCE();
         read(1, image, 3);
-        fetch_quick();
-        SG2IM_FENCE();
         compute(0);
+        interleave<NP, NR, 0, 0>();
         __syncthreads();
-        read(0, image ^ 1, 0);
         SG2IM_FENCE();
+        read(0, image ^ 1, 0);
         compute(1);
+        interleave<NP, NR, 0, 0>();
         SG2IM_FENCE();
       }
     for (; c < chunks; ++c) {
