@@ -12,7 +12,7 @@
 // operands of v_mfma_f32_32x32x16_bf16 (8 consecutive r of one row per lane) are read with ds_read_b128 from the first kind
 // and with the transposing ds_read_b64_tr_b16 from the second.  float32 uses v_mfma_f32_32x32x2_f32 on the same tiles.
 //
-// Four waves share a tile of BM x BN and each computes a quarter.  The reduction advances in chunks of 128 bytes of r, with
+// Four waves share a tile of BM x BN (eight the largest).  The reduction advances in chunks of 128 bytes of r, with
 // two LDS images of each operand: while the matrix cores work on chunk c, chunk c + 1 is written to the other image and
 // chunk c + 2 is on its way from memory; operands of the next step are read during the current one, also across the one
 // barrier per chunk.
@@ -63,7 +63,6 @@ template <typename T, int ROWS, int MODE> struct Tile {
   static constexpr int BK = Geo<T>::BK, NV = Geo<T>::NV;
   static constexpr int LD = MODE == RC ? BK + NV : ROWS + (sizeof(T) == 2 ? 32 : 8);
   static constexpr int ELEMS = MODE == RC ? ROWS * LD : BK * LD;
-  static constexpr int PIECES = ROWS / 32;       // 16-byte pieces per thread
 };
 
 struct Piece { unsigned w[4]; };
@@ -95,9 +94,9 @@ template <typename T> __device__ __forceinline__ Piece load_part(const T* p, int
 // One operand's way from memory to LDS: ROWS rows from row0, chunk by chunk.
 //   whole: every piece of every full chunk lies inside the operand (the rows of an r-contiguous one are clamped: what a row
 //   behind the last one computes is not stored), so that loads need no check
-template <typename T, int ROWS, int MODE> struct Feeder {
+template <typename T, int ROWS, int MODE, int NT> struct Feeder {
   typedef Tile<T, ROWS, MODE> G;
-  static constexpr int NV = G::NV, P = G::PIECES;
+  static constexpr int NV = G::NV, P = ROWS * 8 / NT;     // 16-byte pieces per thread
   static constexpr int PR = ROWS / NV;                     // pieces per r (i / j contiguous)
   const char* base;                                        // this chunk
   const unsigned char* exps;                               // RM8: this chunk's row of exponents
@@ -111,7 +110,7 @@ template <typename T, int ROWS, int MODE> struct Feeder {
       base = reinterpret_cast<const char*>(src) + ((long long)row0 * ld + r0) * (int)sizeof(T);
       #pragma unroll
       for (int i = 0; i < P; ++i) {
-        const int row = min((tid >> 3) + 32 * i, rows - 1 - row0);
+        const int row = min((tid >> 3) + NT / 8 * i, rows - 1 - row0);
         off[i] = (unsigned)(row * (unsigned)ld + (tid & 7) * NV) * (unsigned)sizeof(T);
       }
     } else {
@@ -135,11 +134,11 @@ template <typename T, int ROWS, int MODE> struct Feeder {
     for (int i = I0; i < I1; ++i) {
       if constexpr (MODE == RC) __builtin_memcpy(&s.v[i], base + off[i], 16);
       else {
-        const char* at = base + (long long)(THREADS / PR * i) * ld * (MODE == RM8 ? 1 : (int)sizeof(T)) + off[0];
+        const char* at = base + (long long)(NT / PR * i) * ld * (MODE == RM8 ? 1 : (int)sizeof(T)) + off[0];
         if constexpr (MODE == RM) __builtin_memcpy(&s.v[i], at, 16);
         else {
           __builtin_memcpy(s.q[i], at, NV);
-          s.e[i] = exps[(long long)(threadIdx.x / PR + THREADS / PR * i) * nblk + (row0 + (int)(threadIdx.x % PR) * NV) / C8_BLOCK];
+          s.e[i] = exps[(long long)(threadIdx.x / PR + NT / PR * i) * nblk + (row0 + (int)(threadIdx.x % PR) * NV) / C8_BLOCK];
         }
       }
     }
@@ -150,10 +149,10 @@ template <typename T, int ROWS, int MODE> struct Feeder {
     #pragma unroll
     for (int i = 0; i < P; ++i) {
       if constexpr (MODE == RC) {
-        s.v[i] = load_part<T>(reinterpret_cast<const T*>(base + off[i]), row0 + (tid >> 3) + 32 * i < rows ? left - (tid & 7) * NV : 0);
+        s.v[i] = load_part<T>(reinterpret_cast<const T*>(base + off[i]), row0 + (tid >> 3) + NT / 8 * i < rows ? left - (tid & 7) * NV : 0);
       } else {
-        const int r = tid / PR + THREADS / PR * i, col = row0 + tid % PR * NV, have = r < left ? rows - col : 0;
-        const char* at = base + (long long)(THREADS / PR * i) * ld * (MODE == RM8 ? 1 : (int)sizeof(T)) + off[0];
+        const int r = tid / PR + NT / PR * i, col = row0 + tid % PR * NV, have = r < left ? rows - col : 0;
+        const char* at = base + (long long)(NT / PR * i) * ld * (MODE == RM8 ? 1 : (int)sizeof(T)) + off[0];
         if constexpr (MODE == RM) s.v[i] = load_part<T>(reinterpret_cast<const T*>(at), have);
         else {
           s.q[i][0] = s.q[i][1] = 0;
@@ -175,8 +174,8 @@ template <typename T, int ROWS, int MODE> struct Feeder {
     #pragma unroll
     for (int i = I0; i < I1; ++i) {
       T* p;
-      if constexpr (MODE == RC) p = lds + ((tid >> 3) + 32 * i) * G::LD + (tid & 7) * NV;
-      else p = lds + (tid / PR + THREADS / PR * i) * G::LD + tid % PR * NV;
+      if constexpr (MODE == RC) p = lds + ((tid >> 3) + NT / 8 * i) * G::LD + (tid & 7) * NV;
+      else p = lds + (tid / PR + NT / PR * i) * G::LD + tid % PR * NV;
       uint4 w;
       if constexpr (MODE == RM8) {
         const float scale = c8_scale(s.e[i]);              // (a piece starts at a multiple of its length: one block)
@@ -286,16 +285,17 @@ __device__ __forceinline__ void interleave() {
 template <typename T, int MODE> constexpr int READS_OF = MODE == RC ? 1 : sizeof(T) == 2 ? 2 : 4;
 template <typename T> constexpr int MFMAS_OF = sizeof(T) == 2 ? 1 : 4;
 
-template <typename T, typename TO, int BM, int BN, int AMODE, int BMODE>
-__global__ __launch_bounds__(THREADS, BM * BN >= 256 * 256 ? 1 : 2) void product_kernel(const Product p) {
-  typedef Feeder<T, BM, AMODE> FA;
-  typedef Feeder<T, BN, BMODE> FB;
+template <typename T, typename TO, int BM, int BN, int NT, int AMODE, int BMODE>
+__global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
+  typedef Feeder<T, BM, AMODE, NT> FA;
+  typedef Feeder<T, BN, BMODE, NT> FB;
   typedef Tile<T, BM, AMODE> GA;
   typedef Tile<T, BN, BMODE> GB;
-  constexpr int BK = GA::BK, TI = BM / 64, TJ = BN / 64;
+  constexpr int WJ = NT / 128, WM = BM / 2, WN = BN / WJ;          // 2 x WJ waves of WM x WN
+  constexpr int BK = GA::BK, TI = WM / 32, TJ = WN / 32;
   constexpr int NP = TI * TJ * MFMAS_OF<T>, NR = TI * READS_OF<T, AMODE> + TJ * READS_OF<T, BMODE>, NL = FA::P + FB::P;
-  constexpr int EP = BN / 2 + 4;                                   // floats of an epilogue row (4 banks apart, 32 rows per wave)
-  constexpr int BYTES = 2 * (GA::ELEMS + GB::ELEMS) * (int)sizeof(T), EP_BYTES = 4 * 32 * EP * 4;
+  constexpr int EP = WN + 4;                                   // floats of an epilogue row (4 banks apart, 32 rows per wave)
+  constexpr int BYTES = 2 * (GA::ELEMS + GB::ELEMS) * (int)sizeof(T), EP_BYTES = NT / 64 * 32 * EP * 4;
   __shared__ __attribute__((aligned(16))) char lds[BYTES > EP_BYTES ? BYTES : EP_BYTES];
   T* lds_a = reinterpret_cast<T*>(lds);
   T* lds_b = lds_a + 2 * GA::ELEMS;
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(THREADS, BM * BN >= 256 * 256 ? 1 : 2) void product
   const int group = tile / (4 * p.tiles_j), in = tile - group * 4 * p.tiles_j, gi = min(4, p.tiles_i - 4 * group);
   const int i0 = (4 * group + in % gi) * BM, j0 = in / gi * BN;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int wi = (wave >> 1) * (BM / 2), wj = (wave & 1) * (BN / 2);
+  const int wi = wave / WJ * WM, wj = wave % WJ * WN;
   const int r_begin = split * p.r_per_split, length = min(p.R - r_begin, p.r_per_split);
   const int chunks = (length + BK - 1) / BK, full = length / BK;
 
@@ -434,7 +434,7 @@ __global__ __launch_bounds__(THREADS, BM * BN >= 256 * 256 ? 1 : 2) void product
   }
   // A lane holds scattered fours of one row; 32 rows at a time go through the wave's own part of LDS, so that 8 (4) lanes
   // then hold whole runs of a row and bias, residual and output are read and written in 16-byte pieces
-  constexpr int NC = 8, LANES = BN / 2 / NC;                       // lanes per row
+  constexpr int NC = 8, LANES = WN / NC;                       // lanes per row
   __syncthreads();
   float* mine = reinterpret_cast<float*>(lds) + wave * 32 * EP;
   #pragma unroll
@@ -620,9 +620,9 @@ int run(Product& p, const Plan& q, void* workspace, size_t workspace_bytes, hipS
   p.tiles_j = (p.J + q.tile - 1) / q.tile;
   const long long blocks = (long long)p.tiles_j * p.tiles_i * q.splits;
   if (blocks > 0x7fffffffLL) return SG2IM_ERR_ARG;
-  if (q.tile == 256) SG2IM_LAUNCH((product_kernel<T, TO, 256, 256, AMODE, BMODE>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
-  else if (q.tile == 128) SG2IM_LAUNCH((product_kernel<T, TO, 128, 128, AMODE, BMODE>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
-  else SG2IM_LAUNCH((product_kernel<T, TO, 64, 64, AMODE, BMODE>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
+  if (q.tile == 256) SG2IM_LAUNCH((product_kernel<T, TO, 256, 256, 512, AMODE, BMODE>), dim3((unsigned)blocks), dim3(512), 0, stream, p);
+  else if (q.tile == 128) SG2IM_LAUNCH((product_kernel<T, TO, 128, 128, 256, AMODE, BMODE>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
+  else SG2IM_LAUNCH((product_kernel<T, TO, 64, 64, 256, AMODE, BMODE>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
   if (q.splits > 1) {
     const long long pieces = (long long)p.I * ((p.J + 31) / 32) * 8;
     SG2IM_LAUNCH(join_kernel<TO>, dim3((unsigned)std::min((pieces + THREADS - 1) / THREADS, 1LL << 20)), dim3(THREADS), 0, stream, p);
