@@ -470,39 +470,61 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
   }
 }
 
-// the splits' sums joined in a fixed order: 8 lanes of 4 columns make a word of signs
-template <typename TO>
+// The splits' sums joined in a fixed order: SL threads share a piece of 4 columns (a small output has few pieces, and one
+// thread's walk over 64 splits took 18 us), and 8 pieces make a word of signs.
+template <typename TO, int SL>
 __global__ __launch_bounds__(THREADS) void join_kernel(const Product p) {
-  const int words = (p.J + 31) / 32;
+  constexpr int NPIECE = THREADS / SL;
+  __shared__ float4 red[SL > 1 ? THREADS : 1];
+  const int words = (p.J + 31) / 32, sl = threadIdx.x / NPIECE, pc = threadIdx.x % NPIECE;
   const long long pieces = (long long)p.I * words * 8, plane = (long long)p.I * p.J;
-  for (long long b0 = (long long)blockIdx.x * THREADS; b0 < pieces; b0 += (long long)gridDim.x * THREADS) {
-    const long long at = b0 + threadIdx.x;
-    const long long word = at >> 3;
+  for (long long b0 = (long long)blockIdx.x * NPIECE; b0 < pieces; b0 += (long long)gridDim.x * NPIECE) {
+    const long long at = b0 + pc, word = at >> 3;
     const int i = (int)(word / words), w = (int)(word - (long long)i * words), j = w * 32 + (int)(at & 7) * 4;
-    unsigned bits = 0;
-    if (at < pieces && j + 4 <= p.J) {
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      const float* src = p.part + (long long)i * p.J + j;
+    const int have = at < pieces ? min(4, p.J - j) : 0;
+    const float* src = p.part + (long long)i * p.J + j;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (have == 4) {
       #pragma unroll 8
-      for (int s = 0; s < p.splits; ++s) {
+      for (int s = sl; s < p.splits; s += SL) {
         float u[4];
         load_vec<float, 4>(src + s * plane, u);
         #pragma unroll
         for (int t = 0; t < 4; ++t) v[t] += u[t];
       }
-      bits = finish<TO, 4>(p, i, j, v);
-    } else if (at < pieces) {
-      for (int t = 0; j + t < p.J; ++t) {
-        float v = 0.f;
-        for (int s = 0; s < p.splits; ++s) v += p.part[s * plane + (long long)i * p.J + j + t];
-        bits |= finish_one<TO>(p, i, j + t, v) << t;
+    } else if (have > 0) {
+      for (int s = sl; s < p.splits; s += SL) {
+        v[0] += src[s * plane];
+        if (have > 1) v[1] += src[s * plane + 1];
+        if (have > 2) v[2] += src[s * plane + 2];
       }
     }
-    bits <<= 4 * (int)(at & 7);
+    if constexpr (SL > 1) {
+      red[threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
+      __syncthreads();
+      if (sl == 0) {
+        #pragma unroll
+        for (int k = 1; k < SL; ++k) {
+          const float4 u = red[k * NPIECE + pc];
+          v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w;
+        }
+      }
+      __syncthreads();
+    }
+    unsigned bits = 0;
+    if (sl == 0) {
+      if (have == 4) bits = finish<TO, 4>(p, i, j, v);
+      else if (have > 0) {
+        bits = finish_one<TO>(p, i, j, v[0]);
+        if (have > 1) bits |= finish_one<TO>(p, i, j + 1, v[1]) << 1;
+        if (have > 2) bits |= finish_one<TO>(p, i, j + 2, v[2]) << 2;
+      }
+    }
     if (p.signs) {
+      bits <<= 4 * (int)(at & 7);
       #pragma unroll
       for (int o = 1; o < 8; o <<= 1) bits |= __shfl_xor(bits, o);
-      if (at < pieces && (at & 7) == 0) p.signs[(long long)i * p.sign_words + w] = bits;
+      if (sl == 0 && at < pieces && (at & 7) == 0) p.signs[(long long)i * p.sign_words + w] = bits;
     }
   }
 }
@@ -576,16 +598,21 @@ __global__ __launch_bounds__(THREADS) void act_backward_kernel(const ActParams p
   }
 }
 
-__global__ __launch_bounds__(THREADS) void bias_finish_kernel(const ActParams p) {
-  __shared__ double red[8][32];
+// the chunks' sums joined: 32 columns x 32 chunk lanes
+__global__ __launch_bounds__(1024) void bias_finish_kernel(const ActParams p) {
+  __shared__ double red[32][33];
   const int cl = threadIdx.x & 31, lane = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
   double s = 0.0;
-  if (c < p.N) for (int k = lane; k < p.chunks; k += 8) s += p.part[(long long)k * p.N + c];
+  if (c < p.N) {
+    #pragma unroll 8
+    for (int k = lane; k < p.chunks; k += 32) s += p.part[(long long)k * p.N + c];
+  }
   red[lane][cl] = s;
   __syncthreads();
   if (lane == 0 && c < p.N) {
     s = 0.0;
-    for (int i = 0; i < 8; ++i) s += red[i][cl];
+    #pragma unroll
+    for (int i = 0; i < 32; ++i) s += red[i][cl];
     store_param(p.db, p.db_bf16, c, (float)s, p.accumulate);
   }
 }
@@ -597,18 +624,35 @@ bool type_ok(int t) { return t == 0 || t == 1; }
 
 struct Plan { int tile, splits, r_per_split; };
 
-// 256 x 256 tiles where they fill the card, then 128 x 128, 64 x 64; the reduction is split where even those leave CUs idle.
+// The tile and the number of splits with the least estimated time.  A CU holds 3 / 2 / 1 workgroups of the 64 / 128 / 256
+// tile; a round of o of them takes the tile's fixed part and, per chunk, the larger of its latency and o times its share of
+// the matrix cores; splitting costs a second launch and the partial sums' way to memory and back at 3.5 TB/s.  The figures
+// (microseconds) are fitted to 13 shapes x 3 products x all tiles and splits, 0.2 to 340 us; the estimate is within 20 %, and
+// the tile it picks within 10 % of the best.  E.g. (bfloat16, I x J x R): 32768 x 4096 x 1024 256-tile 272, 128 327, 64 473;
+// 32768 x 256 x 1024 33, 27, 33; 131072 x 64 x 256 38, 28, 19; 256 x 1024 x 32768 with 16 splits of the 128-tile 40, none
+// split faster than 44; 2048 x 2048 x 512 12.4 with one, 30 with two.
+struct TileCost { int tile, per_cu; double fixed, latency, share; };
+constexpr TileCost COSTS[2][3] = {{{64, 3, 2.0, 0.55, 0.50}, {128, 2, 3.0, 1.9, 1.85}, {256, 1, 6.0, 7.5, 7.5}},        // float
+                                  {{64, 3, 2.0, 0.33, 0.23}, {128, 2, 3.0, 0.65, 0.62}, {256, 1, 6.0, 1.75, 1.75}}};    // bfloat16
 Plan plan(long long I, long long J, long long R, int bf16) {
+  static const int ways[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128};
   const int bk = bf16 ? 64 : 32;
-  auto tiles = [&](int t) { return ((I + t - 1) / t) * ((J + t - 1) / t); };
-  Plan q;
-  q.tile = tiles(256) >= 192 ? 256 : tiles(128) >= 256 ? 128 : 64;
-  const long long steps = (R + bk - 1) / bk, n = std::max(1LL, tiles(q.tile));
-  long long splits = std::max(1LL, std::min(std::min(512 / n, steps / 4), 64LL));
-  const long long per = (steps + splits - 1) / splits;
-  q.splits = (int)((steps + per - 1) / per);
-  q.r_per_split = (int)(per * bk);
-  return q;
+  const long long steps = std::max(1LL, (R + bk - 1) / bk);
+  Plan best = {64, 1, (int)(steps * bk)};
+  double least = 1e30;
+  for (const TileCost& t : COSTS[bf16]) {
+    const long long tiles = ((I + t.tile - 1) / t.tile) * ((J + t.tile - 1) / t.tile);
+    for (int w : ways) {
+      if (w > steps || (w > 1 && tiles * w > 1024)) break;
+      const long long per = (steps + w - 1) / w, splits = (steps + per - 1) / per, q = (tiles * splits + 255) / 256;
+      const long long rounds = (q + t.per_cu - 1) / t.per_cu, last = q - (rounds - 1) * t.per_cu;
+      auto round = [&](long long o) { return t.fixed + per * std::max(t.latency, o * t.share); };
+      double us = (rounds - 1) * round(t.per_cu) + round(last);
+      if (splits > 1) us += 3.5 + 8.0 * splits * I * J / 3.5e6;
+      if (us < least) { least = us; best = {t.tile, (int)splits, (int)(per * bk)}; }
+    }
+  }
+  return best;
 }
 
 template <typename T, typename TO, int AMODE, int BMODE>
@@ -625,7 +669,8 @@ int run(Product& p, const Plan& q, void* workspace, size_t workspace_bytes, hipS
   else SG2IM_LAUNCH((product_kernel<T, TO, 64, 64, 256, AMODE, BMODE>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
   if (q.splits > 1) {
     const long long pieces = (long long)p.I * ((p.J + 31) / 32) * 8;
-    SG2IM_LAUNCH(join_kernel<TO>, dim3((unsigned)std::min((pieces + THREADS - 1) / THREADS, 1LL << 20)), dim3(THREADS), 0, stream, p);
+    if (q.splits >= 8 && pieces < 1 << 16) SG2IM_LAUNCH((join_kernel<TO, 8>), dim3((unsigned)((pieces + 31) / 32)), dim3(THREADS), 0, stream, p);
+    else SG2IM_LAUNCH((join_kernel<TO, 1>), dim3((unsigned)std::min((pieces + THREADS - 1) / THREADS, 1LL << 20)), dim3(THREADS), 0, stream, p);
   }
   return status();
 }
@@ -641,7 +686,7 @@ ActParams act_plan(long long rows, int n) {
   p.slabs = (pieces + 63) / 64;
   p.TV = (pieces + p.slabs - 1) / p.slabs;
   p.TP = THREADS / p.TV;
-  const long long want = std::max(1LL, 2048LL / p.slabs);
+  const long long want = std::max(1LL, 1024LL / p.slabs);
   p.rows_per_chunk = std::max((rows + want - 1) / want, (long long)p.TP * 4);
   p.chunks = (int)((rows + p.rows_per_chunk - 1) / p.rows_per_chunk);
   return p;
@@ -699,7 +744,7 @@ int sg2im_linear_backward_act(const void* dy, int dy_dtype, long long ld_dy, con
     else if (dy_dtype == 0) SG2IM_LAUNCH((act_backward_kernel<float, bf16_s>), grid, dim3(THREADS), 0, stream, p);
     else SG2IM_LAUNCH((act_backward_kernel<bf16_s, bf16_s>), grid, dim3(THREADS), 0, stream, p);
   }
-  if (dbias) SG2IM_LAUNCH(bias_finish_kernel, dim3((n + 31) / 32), dim3(THREADS), 0, stream, p);
+  if (dbias) SG2IM_LAUNCH(bias_finish_kernel, dim3((n + 31) / 32), dim3(1024), 0, stream, p);
   return status();
 }
 
