@@ -702,9 +702,13 @@ int sg2im_unpack8(const signed char* codes, const unsigned char* exps, long long
  *   backward_act:     dz = dy * (sign ? 1 : slope) in dz_dtype, dense, and dbias (+)= column sums of the unrounded dz.
  *                     signs NULL: dz = dy.  dz NULL: only dbias; dbias NULL: only dz.
  *   backward_data:    dx = dz W
- *   backward_weight:  dweight (+)= dz^T x, from x or from its 8-bit form (codes / exps, dense, of x's rows)
+ *   backward_weight:  dweight (+)= dz^T x, from x or from its 8-bit form (codes / exps, dense, of x's rows); dbias (may be NULL)
+ *                     (+)= column sums of dz.  signs given to either: `dz` is dy, and dz = dy * (sign ? 1 : slope), rounded to
+ *                     `dtype`, is formed on its way into the product (the same numbers as backward_act's).
  * workspace: sg2im_linear_workspace bytes for `which` = 0 forward, 1 backward_data, 2 backward_weight, 3 backward_act.
  * Rows below 2^31 - 256; k, n and the operands' leading dimensions (in elements) at most 2^22; no alignment beyond an element's is assumed. */
+/* 1: backward_act first and plain products are the faster way for these sizes, 0: the products' own signs / dbias */
+int sg2im_linear_backward_act_first(long long rows, int k, int n, int dtype, int gated, int bias, int need_dx, int need_dw);
 size_t sg2im_linear_workspace(long long rows, int k, int n, int dtype, int which);
 int sg2im_linear_forward(const void* x, int dtype, long long ld_x, const void* weight, const void* bias, int bias_dtype,
                          const void* residual, long long ld_res, float slope, void* out, int out_dtype, long long ld_out,
@@ -713,12 +717,13 @@ int sg2im_linear_forward(const void* x, int dtype, long long ld_x, const void* w
 int sg2im_linear_backward_act(const void* dy, int dy_dtype, long long ld_dy, const unsigned* signs, float slope, void* dz,
                               int dz_dtype, void* dbias, int bias_dtype, int accumulate, long long rows, int n,
                               void* workspace, size_t workspace_bytes, hipStream_t stream);
-int sg2im_linear_backward_data(const void* dz, int dtype, long long ld_dz, const void* weight, void* dx, long long ld_dx,
-                               long long rows, int k, int n, void* workspace, size_t workspace_bytes, hipStream_t stream);
-int sg2im_linear_backward_weight(const void* dz, int dtype, long long ld_dz, const void* x, long long ld_x,
-                                 const signed char* codes, const unsigned char* exps, void* dweight, int dweight_dtype,
-                                 int accumulate, long long rows, int k, int n, void* workspace, size_t workspace_bytes,
-                                 hipStream_t stream);
+int sg2im_linear_backward_data(const void* dz, int dtype, long long ld_dz, const unsigned* signs, float slope, const void* weight,
+                               void* dx, long long ld_dx, long long rows, int k, int n, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream);
+int sg2im_linear_backward_weight(const void* dz, int dtype, long long ld_dz, const unsigned* signs, float slope, const void* x,
+                                 long long ld_x, const signed char* codes, const unsigned char* exps, void* dweight,
+                                 int dweight_dtype, int accumulate, void* dbias, int bias_dtype, int bias_accumulate, long long rows,
+                                 int k, int n, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -11,7 +11,7 @@ CSRC = os.path.join(HERE, 'csrc')
 LIBDIR = os.path.join(HERE, 'lib')
 LIB = os.path.join(LIBDIR, 'libsg2im_hip.so')
 SOURCES = ['conv.hip', 'graph.hip', 'gconv.hip', 'gcn_persist.hip', 'heads.hip', 'norm.hip', 'layout.hip', 'loss.hip',
-           'groupnorm.hip', 'linear.hip']
+           'groupnorm.hip', 'linear.hip', 'linear_dw.hip']
 NATIVE = os.path.join(LIBDIR, 'sg2im_native.so')
 INCLUDES = {}      # (.hip files another translation unit includes: none)
 # (packed fp32 arithmetic off: hipcc -O3 forms v_pk_{add,mul,fma}_f32 from ordinary float code, and some of their forms have

@@ -6,528 +6,12 @@
 //
 // The forward pass keeps one bit per element, z > 0, for the backward pass.
 //
-// All three products are C[i][j] = sum_r A(i, r) B(j, r); an operand lies in memory either with r contiguous (x and W of
-// the forward product, dz of dx) or with i / j contiguous (W of dx, both of dW).  A tile goes from memory through registers
-// into LDS in the order it lies in (so any alignment, any width and the 8-bit form are only a matter of the load); the
-// operands of v_mfma_f32_32x32x16_bf16 (8 consecutive r of one row per lane) are read with ds_read_b128 from the first kind
-// and with the transposing ds_read_b64_tr_b16 from the second.  float32 uses v_mfma_f32_32x32x2_f32 on the same tiles.
-//
-// Four waves share a tile of BM x BN (eight the largest).  The reduction advances in chunks of 128 bytes of r, with
-// two LDS images of each operand: while the matrix cores work on chunk c, chunk c + 1 is written to the other image and
-// chunk c + 2 is on its way from memory; operands of the next step are read during the current one, also across the one
-// barrier per chunk.
-#include <hip/hip_runtime.h>
-#include <algorithm>
-#include "sg2im_hip.h"
+// The products are linear.h's.
 #define SG2IM_GEMM_TU 1
-#include "launch_count.h"
-#include "vecio.h"
-#include "ckpt8.h"
+#include "linear.h"
 
 namespace sg2im {
 namespace lin {
-
-constexpr int THREADS = 256;
-enum { RC = 0, RM = 1, RM8 = 2 };        // r contiguous; i / j contiguous; the same in 8 bits
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-#define SG2IM_FENCE() __builtin_amdgcn_sched_barrier(0)
-
-struct Product {
-  const void* a; const void* b;
-  const unsigned char* b_exps; int b_nblk;       // RM8
-  long long lda, ldb;
-  int I, J, R;                                   // rows, columns, reduction
-  int tiles_i, tiles_j, splits, r_per_split;
-  float* part;                                   // [splits][I][J], splits > 1
-  // epilogue
-  const void* bias; int bias_bf16;
-  const void* residual; long long ld_res;
-  float slope;
-  unsigned* signs; int sign_words;               // [I][sign_words]
-  void* out; long long ld_out;
-  int accumulate;
-};
-
-template <typename T> struct Geo;
-template <> struct Geo<bf16_s> { static constexpr int BK = 64, NV = 8; };
-template <> struct Geo<float> { static constexpr int BK = 32, NV = 4; };
-constexpr int STEPS = 4;                         // per chunk: 16 r of bfloat16, 8 of float
-
-// the LDS image of ROWS rows of an operand by one chunk.  Strides: 144 bytes (36 banks: the 16 rows of a b128 phase start on
-// 16 different bank quads); columns + 64 bytes (the 4 rows of a transposing read lie on different quarters of the banks) or,
-// for float32, + 32 bytes (rows 4 apart lie on different halves)
-template <typename T, int ROWS, int MODE> struct Tile {
-  static constexpr int BK = Geo<T>::BK, NV = Geo<T>::NV;
-  static constexpr int LD = MODE == RC ? BK + NV : ROWS + (sizeof(T) == 2 ? 32 : 8);
-  static constexpr int ELEMS = MODE == RC ? ROWS * LD : BK * LD;
-};
-
-struct Piece { unsigned w[4]; };
-template <int MODE, int N> struct Staged { Piece v[N]; };
-template <int N> struct Staged<RM8, N> { unsigned q[N][2]; unsigned char e[N]; };      // codes (float: the first word) and exponent
-
-// the first `have` elements of a piece, zeros behind them
-template <typename T> __device__ __forceinline__ Piece load_part(const T* p, int have) {
-  Piece r = {{0, 0, 0, 0}};
-  if (have >= Geo<T>::NV) {
-    __builtin_memcpy(&r.w[0], p, 16);
-  } else if (have > 0) {
-    // (an element behind the end reads the last one instead and is dropped: no branch per element)
-    #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (sizeof(T) == 4) {
-        const unsigned w = reinterpret_cast<const unsigned*>(p)[min(j, have - 1)];
-        r.w[j] = j < have ? w : 0;
-      } else {
-        const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
-        const unsigned lo = h[min(2 * j, have - 1)], hi = h[min(2 * j + 1, have - 1)];
-        r.w[j] = (2 * j < have ? lo : 0) | (2 * j + 1 < have ? hi << 16 : 0);
-      }
-    }
-  }
-  return r;
-}
-
-// One operand's way from memory to LDS: ROWS rows from row0, chunk by chunk.
-//   whole: every piece of every full chunk lies inside the operand (the rows of an r-contiguous one are clamped: what a row
-//   behind the last one computes is not stored), so that loads need no check
-template <typename T, int ROWS, int MODE, int NT> struct Feeder {
-  typedef Tile<T, ROWS, MODE> G;
-  static constexpr int NV = G::NV, P = ROWS * 8 / NT;     // 16-byte pieces per thread
-  static constexpr int PR = ROWS / NV;                     // pieces per r (i / j contiguous)
-  const char* base;                                        // this chunk
-  const unsigned char* exps;                               // RM8: this chunk's row of exponents
-  unsigned off[MODE == RC ? P : 1];                        // bytes from base
-  long long ld;
-  int rows, row0, nblk;
-  __device__ __forceinline__ Feeder(const void* src, long long ld_, const unsigned char* e, int nblk_, int row0_, int rows_, int r0)
-    : ld(ld_), rows(rows_), row0(row0_), nblk(nblk_) {
-    const int tid = threadIdx.x;
-    if constexpr (MODE == RC) {
-      base = reinterpret_cast<const char*>(src) + ((long long)row0 * ld + r0) * (int)sizeof(T);
-      #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const int row = min((tid >> 3) + NT / 8 * i, rows - 1 - row0);
-        off[i] = (unsigned)(row * (unsigned)ld + (tid & 7) * NV) * (unsigned)sizeof(T);
-      }
-    } else {
-      const int size = MODE == RM8 ? 1 : (int)sizeof(T);
-      base = reinterpret_cast<const char*>(src) + ((long long)r0 * ld + row0) * size;
-      off[0] = (unsigned)((tid / PR) * (unsigned)ld + tid % PR * NV) * (unsigned)size;
-      exps = e + (long long)r0 * nblk;
-    }
-  }
-  __device__ __forceinline__ bool whole() const { return MODE == RC || row0 + ROWS <= rows; }
-  __device__ __forceinline__ void next() {
-    if constexpr (MODE == RC) base += 128;
-    else {
-      base += G::BK * ld * (MODE == RM8 ? 1 : (int)sizeof(T));
-      if constexpr (MODE == RM8) exps += (long long)G::BK * nblk;
-    }
-  }
-  // pieces [I0, I1) of a full chunk of a whole tile
-  template <int I0, int I1> __device__ __forceinline__ void load(Staged<MODE, P>& s) const {
-    #pragma unroll
-    for (int i = I0; i < I1; ++i) {
-      if constexpr (MODE == RC) __builtin_memcpy(&s.v[i], base + off[i], 16);
-      else {
-        const char* at = base + (long long)(NT / PR * i) * ld * (MODE == RM8 ? 1 : (int)sizeof(T)) + off[0];
-        if constexpr (MODE == RM) __builtin_memcpy(&s.v[i], at, 16);
-        else {
-          __builtin_memcpy(s.q[i], at, NV);
-          s.e[i] = exps[(long long)(threadIdx.x / PR + NT / PR * i) * nblk + (row0 + (int)(threadIdx.x % PR) * NV) / C8_BLOCK];
-        }
-      }
-    }
-  }
-  // any chunk: `left` = how many r there are
-  __device__ __forceinline__ void load_checked(Staged<MODE, P>& s, int left) const {
-    const int tid = threadIdx.x;
-    #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      if constexpr (MODE == RC) {
-        s.v[i] = load_part<T>(reinterpret_cast<const T*>(base + off[i]), row0 + (tid >> 3) + NT / 8 * i < rows ? left - (tid & 7) * NV : 0);
-      } else {
-        const int r = tid / PR + NT / PR * i, col = row0 + tid % PR * NV, have = r < left ? rows - col : 0;
-        const char* at = base + (long long)(NT / PR * i) * ld * (MODE == RM8 ? 1 : (int)sizeof(T)) + off[0];
-        if constexpr (MODE == RM) s.v[i] = load_part<T>(reinterpret_cast<const T*>(at), have);
-        else {
-          s.q[i][0] = s.q[i][1] = 0;
-          s.e[i] = 127;
-          if (have > 0) {
-            #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-              const unsigned q = (unsigned char)at[min(j, have - 1)];
-              s.q[i][j >> 2] |= (j < have ? q : 0) << (8 * (j & 3));
-            }
-            s.e[i] = exps[(long long)r * nblk + col / C8_BLOCK];
-          }
-        }
-      }
-    }
-  }
-  template <int I0, int I1> __device__ __forceinline__ void store(T* lds, const Staged<MODE, P>& s) const {
-    const int tid = threadIdx.x;
-    #pragma unroll
-    for (int i = I0; i < I1; ++i) {
-      T* p;
-      if constexpr (MODE == RC) p = lds + ((tid >> 3) + NT / 8 * i) * G::LD + (tid & 7) * NV;
-      else p = lds + (tid / PR + NT / PR * i) * G::LD + tid % PR * NV;
-      uint4 w;
-      if constexpr (MODE == RM8) {
-        const float scale = c8_scale(s.e[i]);              // (a piece starts at a multiple of its length: one block)
-        float v[NV];
-        #pragma unroll
-        for (int j = 0; j < NV; ++j) v[j] = c8_decode((signed char)(s.q[i][j >> 2] >> (8 * (j & 3))), scale);
-        if constexpr (sizeof(T) == 4) w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-        else {
-          auto two = [&](int j) { return f32_to_bf16_bits(v[j]) | (unsigned)f32_to_bf16_bits(v[j + 1]) << 16; };
-          w = make_uint4(two(0), two(2), two(4), two(6));
-        }
-      } else w = make_uint4(s.v[i].w[0], s.v[i].w[1], s.v[i].w[2], s.v[i].w[3]);
-      *reinterpret_cast<uint4*>(p) = w;
-    }
-  }
-};
-
-// 8 consecutive r (16 step + 8 (lane / 32) ..) of row row0 + lane % 32
-template <int ROWS, int MODE>
-__device__ __forceinline__ bf16x8 operand(const bf16_s* lds, int row0, int step, int lane) {
-  typedef Tile<bf16_s, ROWS, MODE> G;
-  if constexpr (MODE == RC) {
-    return *reinterpret_cast<const bf16x8*>(lds + (row0 + (lane & 31)) * G::LD + 16 * step + 8 * (lane >> 5));
-  } else {
-    // the 16 lanes of a group pass 4 rows x 4 pieces of 4 and receive 4 consecutive r of one column each
-    typedef __attribute__((address_space(3))) bf16x4* LdsPtr;
-    const int p = lane & 15, g = lane >> 4;
-    const bf16_s* at = lds + (16 * step + 8 * (g >> 1) + (p >> 2)) * G::LD + row0 + 16 * (g & 1) + 4 * (p & 3);
-    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LdsPtr)at);
-    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LdsPtr)(at + 4 * G::LD));
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-  }
-}
-// float32: r = 8 step + 4 (lane / 32) .. + 3 of row row0 + lane % 32, one per matrix instruction
-template <int ROWS, int MODE>
-__device__ __forceinline__ float4 operand(const float* lds, int row0, int step, int lane) {
-  typedef Tile<float, ROWS, MODE> G;
-  const int r = 8 * step + 4 * (lane >> 5);
-  if constexpr (MODE == RC) return *reinterpret_cast<const float4*>(lds + (row0 + (lane & 31)) * G::LD + r);
-  else {
-    const float* p = lds + r * G::LD + row0 + (lane & 31);
-    return make_float4(p[0], p[G::LD], p[2 * G::LD], p[3 * G::LD]);
-  }
-}
-__device__ __forceinline__ f32x16 multiply(const bf16x8& a, const bf16x8& b, const f32x16& c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 multiply(const float4& a, const float4& b, f32x16 c) {
-  c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, b.x, c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, b.y, c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, b.z, c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, b.w, c, 0, 0, 0);
-}
-
-// NC consecutive columns of output row i from j on, all of them inside; returns their z > 0 bits
-template <typename TO, int NC>
-__device__ __forceinline__ unsigned finish(const Product& p, int i, int j, float (&v)[NC]) {
-  unsigned bits = 0;
-  if (p.bias) {
-    float b[NC];
-    if (p.bias_bf16) load_vec<bf16_s, NC>(reinterpret_cast<const bf16_s*>(p.bias) + j, b);
-    else load_vec<float, NC>(reinterpret_cast<const float*>(p.bias) + j, b);
-    #pragma unroll
-    for (int t = 0; t < NC; ++t) v[t] += b[t];
-  }
-  #pragma unroll
-  for (int t = 0; t < NC; ++t) {
-    if (v[t] > 0.f) bits |= 1u << t;
-    v[t] = v[t] > 0.f ? v[t] : v[t] * p.slope;
-  }
-  TO* out = reinterpret_cast<TO*>(p.out) + (long long)i * p.ld_out + j;
-  const TO* res = p.residual ? reinterpret_cast<const TO*>(p.residual) + (long long)i * p.ld_res + j : p.accumulate ? out : nullptr;
-  if (res) {
-    float r[NC];
-    load_vec<TO, NC>(res, r);
-    #pragma unroll
-    for (int t = 0; t < NC; ++t) v[t] += r[t];
-  }
-  store_vec<TO, NC>(out, v);
-  return bits;
-}
-template <typename TO>
-__device__ __forceinline__ unsigned finish_one(const Product& p, int i, int j, float v) {
-  if (p.bias) v += load_param(p.bias, p.bias_bf16, j);
-  const unsigned bit = v > 0.f;
-  if (!bit) v *= p.slope;
-  TO* out = reinterpret_cast<TO*>(p.out) + (long long)i * p.ld_out + j;
-  if (p.residual) v += load1(reinterpret_cast<const TO*>(p.residual) + (long long)i * p.ld_res + j);
-  else if (p.accumulate) v += load1(out);
-  store1(out, v);
-  return bit;
-}
-
-// the schedule of a step: P products with the LDS reads, LDS writes and memory loads spread evenly between them
-template <int P, int READS, int WRITES, int LOADS, int K = 0>
-__device__ __forceinline__ void interleave() {
-  if constexpr (K < P) {
-    constexpr int r = (K + 1) * READS / P - K * READS / P, w = (K + 1) * WRITES / P - K * WRITES / P, l = (K + 1) * LOADS / P - K * LOADS / P;
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
-    if constexpr (w > 0) __builtin_amdgcn_sched_group_barrier(0x200, w, 0);
-    if constexpr (l > 0) __builtin_amdgcn_sched_group_barrier(0x020, l, 0);
-    interleave<P, READS, WRITES, LOADS, K + 1>();
-  }
-}
-// LDS reads of an operand, matrix instructions of a product
-template <typename T, int MODE> constexpr int READS_OF = MODE == RC ? 1 : sizeof(T) == 2 ? 2 : 4;
-template <typename T> constexpr int MFMAS_OF = sizeof(T) == 2 ? 1 : 4;
-
-template <typename T, typename TO, int BM, int BN, int NT, int AMODE, int BMODE>
-__global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
-  typedef Feeder<T, BM, AMODE, NT> FA;
-  typedef Feeder<T, BN, BMODE, NT> FB;
-  typedef Tile<T, BM, AMODE> GA;
-  typedef Tile<T, BN, BMODE> GB;
-  constexpr int WJ = NT / 128, WM = BM / 2, WN = BN / WJ;          // 2 x WJ waves of WM x WN
-  constexpr int BK = GA::BK, TI = WM / 32, TJ = WN / 32;
-  constexpr int NP = TI * TJ * MFMAS_OF<T>, NR = TI * READS_OF<T, AMODE> + TJ * READS_OF<T, BMODE>, NL = FA::P + FB::P;
-  constexpr int EP = WN + 4;                                   // floats of an epilogue row (4 banks apart, 32 rows per wave)
-  constexpr int BYTES = 2 * (GA::ELEMS + GB::ELEMS) * (int)sizeof(T), EP_BYTES = NT / 64 * 32 * EP * 4;
-  __shared__ __attribute__((aligned(16))) char lds[BYTES > EP_BYTES ? BYTES : EP_BYTES];
-  T* lds_a = reinterpret_cast<T*>(lds);
-  T* lds_b = lds_a + 2 * GA::ELEMS;
-  // Workgroups go round robin over the 8 XCDs: a contiguous run of tiles each, four rows of tiles at a time, so that the
-  // workgroups that share an L2 share operands
-  const int tiles = p.tiles_i * p.tiles_j, blocks = tiles * p.splits;
-  int id = blockIdx.x;
-  if (blocks % 8 == 0) id = id % 8 * (blocks / 8) + id / 8;
-  const int split = id / tiles, tile = id - split * tiles;
-  const int group = tile / (4 * p.tiles_j), in = tile - group * 4 * p.tiles_j, gi = min(4, p.tiles_i - 4 * group);
-  const int i0 = (4 * group + in % gi) * BM, j0 = in / gi * BN;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int wi = wave / WJ * WM, wj = wave % WJ * WN;
-  const int r_begin = split * p.r_per_split, length = min(p.R - r_begin, p.r_per_split);
-  const int chunks = (length + BK - 1) / BK, full = length / BK;
-
-  f32x16 acc[TI][TJ];
-  #pragma unroll
-  for (int a = 0; a < TI; ++a)
-    #pragma unroll
-    for (int b = 0; b < TJ; ++b)
-      #pragma unroll
-      for (int v = 0; v < 16; ++v) acc[a][b][v] = 0.f;
-
-  FA fa(p.a, p.lda, nullptr, 0, i0, p.I, r_begin);
-  FB fb(p.b, p.ldb, p.b_exps, p.b_nblk, j0, p.J, r_begin);
-  Staged<AMODE, FA::P> sa;
-  Staged<BMODE, FB::P> sb;
-  const bool quick = fa.whole() && fb.whole();
-  int fetched = 0;                                                 // chunks on their way so far
-  auto fetch_quick = [&]() {
-    fa.template load<0, FA::P>(sa);
-    fb.template load<0, FB::P>(sb);
-    fa.next(); fb.next();
-    ++fetched;
-  };
-  auto fetch = [&]() {
-    if (quick && fetched < full) { fetch_quick(); return; }
-    fa.load_checked(sa, length - fetched * BK);
-    fb.load_checked(sb, length - fetched * BK);
-    fa.next(); fb.next();
-    ++fetched;
-  };
-  auto put = [&](int image) {
-    fa.template store<0, FA::P>(lds_a + image * GA::ELEMS, sa);
-    fb.template store<0, FB::P>(lds_b + image * GB::ELEMS, sb);
-  };
-  auto put_half = [&](int image, int half) {
-    if (half == 0) { fa.template store<0, FA::P / 2>(lds_a + image * GA::ELEMS, sa); fb.template store<0, FB::P / 2>(lds_b + image * GB::ELEMS, sb); }
-    else { fa.template store<FA::P / 2, FA::P>(lds_a + image * GA::ELEMS, sa); fb.template store<FB::P / 2, FB::P>(lds_b + image * GB::ELEMS, sb); }
-  };
-  typedef decltype(operand<BM, AMODE>(lds_a, 0, 0, 0)) Op;
-  Op oa[2][TI], ob[2][TJ];
-  auto read = [&](int into, int image, int step) {
-    #pragma unroll
-    for (int a = 0; a < TI; ++a) oa[into][a] = operand<BM, AMODE>(lds_a + image * GA::ELEMS, wi + 32 * a, step, lane);
-    #pragma unroll
-    for (int b = 0; b < TJ; ++b) ob[into][b] = operand<BN, BMODE>(lds_b + image * GB::ELEMS, wj + 32 * b, step, lane);
-  };
-  auto compute = [&](int from) {
-    #pragma unroll
-    for (int a = 0; a < TI; ++a)
-      #pragma unroll
-      for (int b = 0; b < TJ; ++b) acc[a][b] = multiply(ob[from][b], oa[from][a], acc[a][b]);
-  };
-
-  if (chunks > 0) {
-    fetch();
-    put(0);
-    if (chunks > 1) fetch();
-    __syncthreads();
-    read(0, 0, 0);
-    int c = 0;
-    if (quick)
-      for (; c + 2 < full; ++c) {                                  // (the same as below without its questions)
-        const int image = c & 1;
-        // The order inside a step: the LDS and memory traffic spread between the products (left to itself the compiler moves
-        // each access next to its use, and the matrix cores wait for it)
-        read(1, image, 1);
-        put(image ^ 1);
-        compute(0);
-        interleave<NP, NR, NL, 0>();
-        SG2IM_FENCE();
-        read(0, image, 2);
-        fetch_quick();
-        compute(1);
-        interleave<NP, NR, 0, NL>();
-        SG2IM_FENCE();
-        read(1, image, 3);
-        compute(0);
-        interleave<NP, NR, 0, 0>();
-        __syncthreads();
-        SG2IM_FENCE();
-        read(0, image ^ 1, 0);
-        compute(1);
-        interleave<NP, NR, 0, 0>();
-        SG2IM_FENCE();
-      }
-    for (; c < chunks; ++c) {
-      const int image = c & 1;
-      read(1, image, 1);
-      if (c + 1 < chunks) put(image ^ 1);
-      compute(0);
-      read(0, image, 2);
-      if (c + 2 < chunks) fetch();
-      compute(1);
-      read(1, image, 3);
-      compute(0);
-      __syncthreads();
-      if (c + 1 < chunks) read(0, image ^ 1, 0);
-      compute(1);
-    }
-  }
-
-  if (p.splits > 1) {
-    #pragma unroll
-    for (int a = 0; a < TI; ++a) {
-      const int i = i0 + wi + 32 * a + (lane & 31);
-      #pragma unroll
-      for (int b = 0; b < TJ; ++b)
-        #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int j = j0 + wj + 32 * b + 8 * q + 4 * (lane >> 5);
-          float v[4] = {acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]};
-          if (i < p.I) {
-            float* out = p.part + ((long long)split * p.I + i) * p.J + j;
-            if (j + 4 <= p.J) store_vec<float, 4>(out, v);
-            else {
-              #pragma unroll
-              for (int t = 0; t < 4; ++t) if (j + t < p.J) out[t] = v[t];
-            }
-          }
-        }
-    }
-    return;
-  }
-  // A lane holds scattered fours of one row; 32 rows at a time go through the wave's own part of LDS, so that 8 (4) lanes
-  // then hold whole runs of a row and bias, residual and output are read and written in 16-byte pieces
-  constexpr int NC = 8, LANES = WN / NC;                       // lanes per row
-  __syncthreads();
-  float* mine = reinterpret_cast<float*>(lds) + wave * 32 * EP;
-  #pragma unroll
-  for (int a = 0; a < TI; ++a) {
-    #pragma unroll
-    for (int b = 0; b < TJ; ++b)
-      #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<float4*>(mine + (lane & 31) * EP + 32 * b + 8 * q + 4 * (lane >> 5)) =
-            make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
-    __builtin_amdgcn_wave_barrier();
-    #pragma unroll
-    for (int k = 0; k < 32 * LANES / 64; ++k) {
-      const int row = k * (64 / LANES) + lane / LANES, col = lane % LANES * NC;
-      const float* from = mine + row * EP + col;
-      const int i = i0 + wi + 32 * a + row, j = j0 + wj + col;
-      unsigned bits = 0;
-      if (i < p.I && j + NC <= p.J) {
-        const float4 lo = *reinterpret_cast<const float4*>(from), hi = *reinterpret_cast<const float4*>(from + 4);
-        float v[NC] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        bits = finish<TO, NC>(p, i, j, v);
-      } else if (i < p.I) {
-        for (int t = 0; j + t < p.J; ++t) bits |= finish_one<TO>(p, i, j + t, from[t]) << t;
-      }
-      bits <<= 8 * (lane & 3);
-      if (p.signs) {
-        bits |= __shfl_xor(bits, 1);
-        bits |= __shfl_xor(bits, 2);
-        if ((lane & 3) == 0 && i < p.I && j < p.J) p.signs[(long long)i * p.sign_words + j / 32] = bits;
-      }
-    }
-    __builtin_amdgcn_wave_barrier();
-  }
-}
-
-// The splits' sums joined in a fixed order: SL threads share a piece of 4 columns (a small output has few pieces, and one
-// thread's walk over 64 splits took 18 us), and 8 pieces make a word of signs.
-template <typename TO, int SL>
-__global__ __launch_bounds__(THREADS) void join_kernel(const Product p) {
-  constexpr int NPIECE = THREADS / SL;
-  __shared__ float4 red[SL > 1 ? THREADS : 1];
-  const int words = (p.J + 31) / 32, sl = threadIdx.x / NPIECE, pc = threadIdx.x % NPIECE;
-  const long long pieces = (long long)p.I * words * 8, plane = (long long)p.I * p.J;
-  for (long long b0 = (long long)blockIdx.x * NPIECE; b0 < pieces; b0 += (long long)gridDim.x * NPIECE) {
-    const long long at = b0 + pc, word = at >> 3;
-    const int i = (int)(word / words), w = (int)(word - (long long)i * words), j = w * 32 + (int)(at & 7) * 4;
-    const int have = at < pieces ? min(4, p.J - j) : 0;
-    const float* src = p.part + (long long)i * p.J + j;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (have == 4) {
-      #pragma unroll 8
-      for (int s = sl; s < p.splits; s += SL) {
-        float u[4];
-        load_vec<float, 4>(src + s * plane, u);
-        #pragma unroll
-        for (int t = 0; t < 4; ++t) v[t] += u[t];
-      }
-    } else if (have > 0) {
-      for (int s = sl; s < p.splits; s += SL) {
-        v[0] += src[s * plane];
-        if (have > 1) v[1] += src[s * plane + 1];
-        if (have > 2) v[2] += src[s * plane + 2];
-      }
-    }
-    if constexpr (SL > 1) {
-      red[threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
-      __syncthreads();
-      if (sl == 0) {
-        #pragma unroll
-        for (int k = 1; k < SL; ++k) {
-          const float4 u = red[k * NPIECE + pc];
-          v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w;
-        }
-      }
-      __syncthreads();
-    }
-    unsigned bits = 0;
-    if (sl == 0) {
-      if (have == 4) bits = finish<TO, 4>(p, i, j, v);
-      else if (have > 0) {
-        bits = finish_one<TO>(p, i, j, v[0]);
-        if (have > 1) bits |= finish_one<TO>(p, i, j + 1, v[1]) << 1;
-        if (have > 2) bits |= finish_one<TO>(p, i, j + 2, v[2]) << 2;
-      }
-    }
-    if (p.signs) {
-      bits <<= 4 * (int)(at & 7);
-      #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) bits |= __shfl_xor(bits, o);
-      if (sl == 0 && at < pieces && (at & 7) == 0) p.signs[(long long)i * p.sign_words + w] = bits;
-    }
-  }
-}
 
 // ---- dz and the bias gradient -------------------------------------------------------------------------------------
 
@@ -619,62 +103,6 @@ __global__ __launch_bounds__(1024) void bias_finish_kernel(const ActParams p) {
 
 // ---- host ---------------------------------------------------------------------------------------------------------
 
-int status() { return hipGetLastError() == hipSuccess ? SG2IM_OK : SG2IM_ERR_HIP; }
-bool type_ok(int t) { return t == 0 || t == 1; }
-
-struct Plan { int tile, splits, r_per_split; };
-
-// The tile and the number of splits with the least estimated time.  A CU holds 3 / 2 / 1 workgroups of the 64 / 128 / 256
-// tile; a round of o of them takes the tile's fixed part and, per chunk, the larger of its latency and o times its share of
-// the matrix cores; splitting costs a second launch and the partial sums' way to memory and back at 3.5 TB/s.  The figures
-// (microseconds) are fitted to 13 shapes x 3 products x all tiles and splits, 0.2 to 340 us; the estimate is within 20 %, and
-// the tile it picks within 10 % of the best.  E.g. (bfloat16, I x J x R): 32768 x 4096 x 1024 256-tile 272, 128 327, 64 473;
-// 32768 x 256 x 1024 33, 27, 33; 131072 x 64 x 256 38, 28, 19; 256 x 1024 x 32768 with 16 splits of the 128-tile 40, none
-// split faster than 44; 2048 x 2048 x 512 12.4 with one, 30 with two.
-struct TileCost { int tile, per_cu; double fixed, latency, share; };
-constexpr TileCost COSTS[2][3] = {{{64, 3, 2.0, 0.55, 0.50}, {128, 2, 3.0, 1.9, 1.85}, {256, 1, 6.0, 7.5, 7.5}},        // float
-                                  {{64, 3, 2.0, 0.33, 0.23}, {128, 2, 3.0, 0.65, 0.62}, {256, 1, 6.0, 1.75, 1.75}}};    // bfloat16
-Plan plan(long long I, long long J, long long R, int bf16) {
-  static const int ways[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128};
-  const int bk = bf16 ? 64 : 32;
-  const long long steps = std::max(1LL, (R + bk - 1) / bk);
-  Plan best = {64, 1, (int)(steps * bk)};
-  double least = 1e30;
-  for (const TileCost& t : COSTS[bf16]) {
-    const long long tiles = ((I + t.tile - 1) / t.tile) * ((J + t.tile - 1) / t.tile);
-    for (int w : ways) {
-      if (w > steps || (w > 1 && tiles * w > 1024)) break;
-      const long long per = (steps + w - 1) / w, splits = (steps + per - 1) / per, q = (tiles * splits + 255) / 256;
-      const long long rounds = (q + t.per_cu - 1) / t.per_cu, last = q - (rounds - 1) * t.per_cu;
-      auto round = [&](long long o) { return t.fixed + per * std::max(t.latency, o * t.share); };
-      double us = (rounds - 1) * round(t.per_cu) + round(last);
-      if (splits > 1) us += 3.5 + 8.0 * splits * I * J / 3.5e6;
-      if (us < least) { least = us; best = {t.tile, (int)splits, (int)(per * bk)}; }
-    }
-  }
-  return best;
-}
-
-template <typename T, typename TO, int AMODE, int BMODE>
-int run(Product& p, const Plan& q, void* workspace, size_t workspace_bytes, hipStream_t stream) {
-  p.splits = q.splits; p.r_per_split = q.r_per_split;
-  p.part = reinterpret_cast<float*>(workspace);
-  if (q.splits > 1 && (!workspace || workspace_bytes < (size_t)q.splits * p.I * p.J * 4)) return SG2IM_ERR_ARG;
-  p.tiles_i = (p.I + q.tile - 1) / q.tile;
-  p.tiles_j = (p.J + q.tile - 1) / q.tile;
-  const long long blocks = (long long)p.tiles_j * p.tiles_i * q.splits;
-  if (blocks > 0x7fffffffLL) return SG2IM_ERR_ARG;
-  if (q.tile == 256) SG2IM_LAUNCH((product_kernel<T, TO, 256, 256, 512, AMODE, BMODE>), dim3((unsigned)blocks), dim3(512), 0, stream, p);
-  else if (q.tile == 128) SG2IM_LAUNCH((product_kernel<T, TO, 128, 128, 256, AMODE, BMODE>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
-  else SG2IM_LAUNCH((product_kernel<T, TO, 64, 64, 256, AMODE, BMODE>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
-  if (q.splits > 1) {
-    const long long pieces = (long long)p.I * ((p.J + 31) / 32) * 8;
-    if (q.splits >= 8 && pieces < 1 << 16) SG2IM_LAUNCH((join_kernel<TO, 8>), dim3((unsigned)((pieces + 31) / 32)), dim3(THREADS), 0, stream, p);
-    else SG2IM_LAUNCH((join_kernel<TO, 1>), dim3((unsigned)std::min((pieces + THREADS - 1) / THREADS, 1LL << 20)), dim3(THREADS), 0, stream, p);
-  }
-  return status();
-}
-
 constexpr int LD_MAX = 1 << 22;      // (a tile's 256 rows stay within 32-bit byte offsets)
 bool ld_ok(long long ld, int cols) { return ld >= cols && ld <= LD_MAX; }
 bool sizes_ok(long long rows, int k, int n) { return rows >= 0 && rows <= 0x7fffffffLL - 256 && k >= 1 && n >= 1 && k <= LD_MAX && n <= LD_MAX; }
@@ -703,9 +131,24 @@ extern "C" {
 size_t sg2im_linear_workspace(long long rows, int k, int n, int dtype, int which) {
   if (!sizes_ok(rows, k, n) || !type_ok(dtype) || rows == 0) return 16;
   if (which == 3) return std::max((size_t)16, (size_t)act_plan(rows, n).chunks * n * 4);
-  const Plan q = which == 0 ? plan(rows, n, k, dtype) : which == 1 ? plan(rows, k, n, dtype) : plan(n, k, rows, dtype);
-  const size_t elems = which == 0 ? (size_t)rows * n : which == 1 ? (size_t)rows * k : (size_t)n * k;
-  return q.splits > 1 ? q.splits * elems * 4 : 16;
+  if (which == 0) return plan_bytes(plan(rows, n, k, dtype), rows, n, false);
+  if (which == 1) return std::max(plan_bytes(plan(rows, k, n, dtype), rows, k, false), plan_bytes(plan(rows, k, n, dtype, GATED[dtype]), rows, k, false));
+  return std::max({plan_bytes(plan(n, k, rows, dtype), n, k, false), plan_bytes(plan(n, k, rows, dtype, GATED[dtype]), n, k, true),
+                   plan_bytes(plan(n, k, rows, dtype, SUMMED[dtype]), n, k, true)});
+}
+
+int sg2im_linear_backward_act_first(long long rows, int k, int n, int dtype, int gated, int bias, int need_dx, int need_dw) {
+  if (!sizes_ok(rows, k, n) || !type_ok(dtype) || (!need_dx && !need_dw) || rows == 0) return 0;
+  if (!gated && !(bias && need_dw)) return 0;
+  // one pass over dy (and dz to memory) at 4.5 TB/s and its last sum, then plain products; or products that do it themselves
+  const double es = dtype ? 2 : 4;
+  double first = 8.0 + es * rows * n * (gated ? 2 : 1) / 4.5e6, itself = 0.0;
+  if (need_dx && gated) { first += plan(rows, k, n, dtype).us; itself += plan(rows, k, n, dtype, GATED[dtype]).us; }
+  if (need_dw) {
+    first += plan(n, k, rows, dtype).us;
+    itself += plan(n, k, rows, dtype, gated ? GATED[dtype] : SUMMED[dtype]).us;
+  }
+  return first < itself;
 }
 
 int sg2im_linear_forward(const void* x, int dtype, long long ld_x, const void* weight, const void* bias, int bias_dtype,
@@ -719,11 +162,10 @@ int sg2im_linear_forward(const void* x, int dtype, long long ld_x, const void* w
   Product p = {};
   p.a = x; p.lda = ld_x; p.b = weight; p.ldb = k; p.I = (int)rows; p.J = n; p.R = k;
   p.bias = bias; p.bias_bf16 = bias_dtype; p.residual = residual; p.ld_res = ld_res; p.slope = slope;
-  p.signs = signs; p.sign_words = (n + 31) / 32; p.out = out; p.ld_out = ld_out;
+  p.signs = signs; p.sign_words = (n + 31) / 32; p.out = out; p.out_bf16 = out_dtype; p.ld_out = ld_out;
   const Plan q = plan(rows, n, k, dtype);
-  if (dtype == 0) return run<float, float, RC, RC>(p, q, workspace, workspace_bytes, stream);
-  if (out_dtype == 0) return run<bf16_s, float, RC, RC>(p, q, workspace, workspace_bytes, stream);
-  return run<bf16_s, bf16_s, RC, RC>(p, q, workspace, workspace_bytes, stream);
+  return dtype == 0 ? run<float, RC, RC, false, false>(p, q, workspace, workspace_bytes, stream)
+                    : run<bf16_s, RC, RC, false, false>(p, q, workspace, workspace_bytes, stream);
 }
 
 int sg2im_linear_backward_act(const void* dy, int dy_dtype, long long ld_dy, const unsigned* signs, float slope, void* dz,
@@ -748,40 +190,39 @@ int sg2im_linear_backward_act(const void* dy, int dy_dtype, long long ld_dy, con
   return status();
 }
 
-int sg2im_linear_backward_data(const void* dz, int dtype, long long ld_dz, const void* weight, void* dx, long long ld_dx,
-                               long long rows, int k, int n, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+int sg2im_linear_backward_data(const void* dz, int dtype, long long ld_dz, const unsigned* signs, float slope, const void* weight,
+                               void* dx, long long ld_dx, long long rows, int k, int n, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream) {
   if (!sizes_ok(rows, k, n) || !type_ok(dtype) || !ld_ok(ld_dz, n) || ld_dx < k) return SG2IM_ERR_ARG;
   if (rows == 0) return SG2IM_OK;
   if (!dz || !weight || !dx) return SG2IM_ERR_ARG;
   Product p = {};
   p.a = dz; p.lda = ld_dz; p.b = weight; p.ldb = k; p.I = (int)rows; p.J = k; p.R = n;
-  p.slope = 1.f; p.out = dx; p.ld_out = ld_dx;
-  const Plan q = plan(rows, k, n, dtype);
-  return dtype == 0 ? run<float, float, RC, RM>(p, q, workspace, workspace_bytes, stream)
-                    : run<bf16_s, bf16_s, RC, RM>(p, q, workspace, workspace_bytes, stream);
+  p.slope = 1.f; p.out = dx; p.out_bf16 = dtype; p.ld_out = ld_dx;
+  p.gate = reinterpret_cast<const unsigned char*>(signs); p.gate_ld = (n + 31) / 32 * 4LL; p.gate_slope = slope;
+  const Plan q = plan(rows, k, n, dtype, signs ? GATED[dtype] : 0.0);
+  if (signs) return dtype == 0 ? run<float, RC, RM, true, false>(p, q, workspace, workspace_bytes, stream)
+                               : run<bf16_s, RC, RM, true, false>(p, q, workspace, workspace_bytes, stream);
+  return dtype == 0 ? run<float, RC, RM, false, false>(p, q, workspace, workspace_bytes, stream)
+                    : run<bf16_s, RC, RM, false, false>(p, q, workspace, workspace_bytes, stream);
 }
 
-int sg2im_linear_backward_weight(const void* dz, int dtype, long long ld_dz, const void* x, long long ld_x,
-                                 const signed char* codes, const unsigned char* exps, void* dweight, int dweight_dtype,
-                                 int accumulate, long long rows, int k, int n, void* workspace, size_t workspace_bytes,
-                                 hipStream_t stream) {
-  if (!sizes_ok(rows, k, n) || !type_ok(dtype) || !type_ok(dweight_dtype) || (dtype == 0 && dweight_dtype == 1) ||
+int sg2im_linear_backward_weight(const void* dz, int dtype, long long ld_dz, const unsigned* signs, float slope, const void* x,
+                                 long long ld_x, const signed char* codes, const unsigned char* exps, void* dweight,
+                                 int dweight_dtype, int accumulate, void* dbias, int bias_dtype, int bias_accumulate, long long rows,
+                                 int k, int n, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (!sizes_ok(rows, k, n) || !type_ok(dtype) || !type_ok(dweight_dtype) || !type_ok(bias_dtype) || (dtype == 0 && dweight_dtype == 1) ||
       !ld_ok(ld_dz, n) || !codes != !exps || (!codes && !ld_ok(ld_x, k)) || !dweight) return SG2IM_ERR_ARG;
   if (rows > 0 && (!dz || (!x && !codes))) return SG2IM_ERR_ARG;
   Product p = {};
   p.a = dz; p.lda = ld_dz; p.I = n; p.J = k; p.R = (int)rows;
-  p.slope = 1.f; p.out = dweight; p.ld_out = k; p.accumulate = accumulate;
-  const Plan q = plan(n, k, std::max(1LL, rows), dtype);   // (no row: one empty sum, zeros or what was there)
-  if (codes) {
-    p.b = codes; p.ldb = k; p.b_exps = exps; p.b_nblk = (k + C8_BLOCK - 1) / C8_BLOCK;
-    if (dtype == 0) return run<float, float, RM, RM8>(p, q, workspace, workspace_bytes, stream);
-    if (dweight_dtype == 0) return run<bf16_s, float, RM, RM8>(p, q, workspace, workspace_bytes, stream);
-    return run<bf16_s, bf16_s, RM, RM8>(p, q, workspace, workspace_bytes, stream);
-  }
-  p.b = x; p.ldb = ld_x;
-  if (dtype == 0) return run<float, float, RM, RM>(p, q, workspace, workspace_bytes, stream);
-  if (dweight_dtype == 0) return run<bf16_s, float, RM, RM>(p, q, workspace, workspace_bytes, stream);
-  return run<bf16_s, bf16_s, RM, RM>(p, q, workspace, workspace_bytes, stream);
+  p.slope = 1.f; p.out = dweight; p.out_bf16 = dweight_dtype; p.ld_out = k; p.accumulate = accumulate;
+  p.gate = reinterpret_cast<const unsigned char*>(signs); p.gate_ld = (n + 31) / 32 * 4LL; p.gate_slope = slope;
+  p.sum = dbias; p.sum_bf16 = bias_dtype; p.sum_accumulate = bias_accumulate;
+  if (codes) { p.b = codes; p.ldb = k; p.b_exps = exps; p.b_nblk = (k + C8_BLOCK - 1) / C8_BLOCK; }
+  else { p.b = x; p.ldb = ld_x; }
+  const Plan q = plan(n, k, std::max(1LL, rows), dtype, signs ? GATED[dtype] : dbias ? SUMMED[dtype] : 0.0);   // (no row: one empty sum, zeros or what was there)
+  return run_weight(p, dtype, codes != nullptr, q, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

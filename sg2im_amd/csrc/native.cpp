@@ -31,6 +31,7 @@ struct Api {
   decltype(&sg2im_pack8) pack8;
   decltype(&sg2im_unpack8) unpack8;
   decltype(&sg2im_linear_workspace) linear_workspace;
+  decltype(&sg2im_linear_backward_act_first) linear_backward_act_first;
   decltype(&sg2im_linear_forward) linear_forward;
   decltype(&sg2im_linear_backward_act) linear_backward_act;
   decltype(&sg2im_linear_backward_data) linear_backward_data;
@@ -40,7 +41,7 @@ struct Api {
 void bind(const std::unordered_map<std::string, uintptr_t>& at) {
   #define SG2IM_BIND(f) api.f = reinterpret_cast<decltype(api.f)>(at.at("sg2im_" #f))
   SG2IM_BIND(init); SG2IM_BIND(groupnorm_workspace); SG2IM_BIND(groupnorm_act_forward); SG2IM_BIND(groupnorm_act_backward);
-  SG2IM_BIND(pack8); SG2IM_BIND(unpack8); SG2IM_BIND(linear_workspace); SG2IM_BIND(linear_forward);
+  SG2IM_BIND(pack8); SG2IM_BIND(unpack8); SG2IM_BIND(linear_workspace); SG2IM_BIND(linear_backward_act_first); SG2IM_BIND(linear_forward);
   SG2IM_BIND(linear_backward_act); SG2IM_BIND(linear_backward_data); SG2IM_BIND(linear_backward_weight);
   #undef SG2IM_BIND
 }
@@ -315,11 +316,16 @@ std::tuple<Tensor, Tensor> lin_forward(const Tensor& x, const Tensor& weight, co
   return {y, signs};
 }
 
+void check_signs(const Tensor& signs, const Rows& dy) {
+  TORCH_CHECK_VALUE(!signs.defined() || (signs.is_cuda() && signs.scalar_type() == at::kInt && signs.is_contiguous() && signs.dim() == 2 &&
+                                         signs.size(0) == dy.rows && signs.size(1) == (dy.cols + 31) / 32), "linear backward: not the signs of this output");
+}
+const unsigned* signs_ptr(const Tensor& t) { return reinterpret_cast<const unsigned*>(ptr(t)); }
+
 // dz in `dz_type` (-1: not written) and the bias gradient into dbias (undefined: none)
 Tensor lin_backward_act(const Rows& dy, const Tensor& signs, double slope, int dz_type, const Tensor& dbias, bool accumulate) {
   const int N = int_of(dy.cols, "linear gradient");
-  TORCH_CHECK_VALUE(!signs.defined() || (signs.is_cuda() && signs.scalar_type() == at::kInt && signs.is_contiguous() && signs.dim() == 2 &&
-                                         signs.size(0) == dy.rows && signs.size(1) == (N + 31) / 32), "linear backward: not the signs of this output");
+  check_signs(signs, dy);
   TORCH_CHECK_TYPE(dz_type != 0 || !is_bf16(dy.m), "linear backward: a float32 dz of a bfloat16 gradient");
   const int bc = params(Tensor(), dbias, N, "linear bias gradient");
   Tensor dz;
@@ -332,19 +338,23 @@ Tensor lin_backward_act(const Rows& dy, const Tensor& signs, double slope, int d
   return dz;
 }
 
-Tensor lin_backward_data(const Rows& dz, const Tensor& weight, at::IntArrayRef shape) {
+Tensor lin_backward_data(const Rows& dz, const Tensor& signs, double slope, const Tensor& weight, at::IntArrayRef shape) {
+  check_signs(signs, dz);
   check_weight(weight, dz.m.scalar_type());
   TORCH_CHECK_VALUE(weight.size(0) == dz.cols, "linear backward: gradient ", dz.m.sizes(), " and weight ", weight.sizes());
   const int N = (int)weight.size(0), K = int_of(weight.size(1), "linear");
   Tensor dx = at::empty(shape, dz.m.options().memory_format(c10::nullopt));
   const size_t bytes = api.linear_workspace(dz.rows, K, N, code(dz.m), 1);
   const Tensor w = work(dz.m, bytes);
-  done(api.linear_backward_data(ptr(dz.m), code(dz.m), dz.ld, ptr(weight), out_ptr(dx), K, dz.rows, K, N, out_ptr(w), bytes, stream_of(dz.m)),
+  done(api.linear_backward_data(ptr(dz.m), code(dz.m), dz.ld, signs_ptr(signs), (float)slope, ptr(weight), out_ptr(dx), K, dz.rows, K, N, out_ptr(w), bytes, stream_of(dz.m)),
        "sg2im_linear_backward_data");
   return dx;
 }
 
-void lin_backward_weight(const Rows& dz, const Tensor& x, const Packed& packed, const Tensor& dweight, bool accumulate) {
+void lin_backward_weight(const Rows& dz, const Tensor& signs, double slope, const Tensor& x, const Packed& packed, const Tensor& dweight,
+                         bool accumulate, const Tensor& dbias, bool bias_accumulate) {
+  check_signs(signs, dz);
+  const int bc = params(Tensor(), dbias, dz.cols, "linear bias gradient");
   on_device(dweight, "linear weight gradient");
   Rows r;
   if (x.defined()) {
@@ -363,8 +373,8 @@ void lin_backward_weight(const Rows& dz, const Tensor& x, const Packed& packed, 
                     r.rows, " x ", r.cols, ", weight gradient ", dweight.scalar_type(), " ", dweight.sizes());
   const size_t bytes = api.linear_workspace(dz.rows, K, N, code(dz.m), 2);
   const Tensor w = work(dz.m, bytes);
-  done(api.linear_backward_weight(ptr(dz.m), code(dz.m), dz.ld, ptr(r.m), r.ld, codes_ptr(packed.codes), exps_ptr(packed.exps), out_ptr(dweight),
-                                  code(dweight), accumulate, dz.rows, K, N, out_ptr(w), bytes, stream_of(dz.m)), "sg2im_linear_backward_weight");
+  done(api.linear_backward_weight(ptr(dz.m), code(dz.m), dz.ld, signs_ptr(signs), (float)slope, ptr(r.m), r.ld, codes_ptr(packed.codes),
+                                  exps_ptr(packed.exps), out_ptr(dweight), code(dweight), accumulate, out_ptr(dbias), bc, bias_accumulate, dz.rows, K, N, out_ptr(w), bytes, stream_of(dz.m)), "sg2im_linear_backward_weight");
 }
 
 struct LinearResidual : torch::autograd::Function<LinearResidual> {
@@ -396,20 +406,28 @@ struct LinearResidual : torch::autograd::Function<LinearResidual> {
     if (nx || nw || nb) {
       on_device(grads[0], "linear gradient");
       const Rows dy = rows_of(grads[0], "linear gradient");
-      const bool plain = !signs.defined() && code(dy.m) == type;             // dz is dy itself
+      const double slope = ctx->saved_data["slope"].toDouble();
       const Target tb(nb, s[5], Sinks::kept(ctx, "sink_b"));
+      // dz = dy * leaky' and the bias gradient: a pass of their own, or done by the products as they read dy
+      const bool same = code(dy.m) == type, products = nx || nw;
+      const bool first = products && same && api.linear_backward_act_first(dy.rows, (int)s[3].size(1), (int)s[3].size(0), type, signs.defined(),
+                                                                           nb, nx, nw);
+      const bool own = products && (!same || (first && signs.defined()));
       Rows dz = dy;
-      if (nb || (!plain && (nx || nw))) {
-        const Tensor z = lin_backward_act(dy, signs, ctx->saved_data["slope"].toDouble(), plain || !(nx || nw) ? -1 : type, tb.buf, !tb.own);
-        if (z.defined()) { dz.m = z; dz.ld = dz.cols; }
+      Tensor gate = signs;
+      bool summed = false;
+      if (own || (nb && (!nw || first))) {
+        const Tensor z = lin_backward_act(dy, signs, slope, own ? type : -1, tb.buf, !tb.own);
+        summed = true;
+        if (own) { dz.m = z; dz.ld = dz.cols; gate = Tensor(); }
       }
-      db = tb.grad();
-      if (nx) dx = lin_backward_data(dz, s[4].defined() ? s[4] : s[3], ctx->saved_data["shape"].toIntVector());
+      if (nx) dx = lin_backward_data(dz, gate, slope, s[4].defined() ? s[4] : s[3], ctx->saved_data["shape"].toIntVector());
       if (nw) {
         const Target tw(true, s[3], Sinks::kept(ctx, "sink_w"));
-        lin_backward_weight(dz, s[0], Packed{s[1], s[2]}, tw.buf, !tw.own);
+        lin_backward_weight(dz, gate, slope, s[0], Packed{s[1], s[2]}, tw.buf, !tw.own, summed ? Tensor() : tb.buf, !tb.own);
         dw = tw.grad();
       }
+      db = tb.grad();
     }
     return {dx, dw, db, nr ? grads[0] : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -454,14 +472,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     on_device(dy, "linear gradient");
     return lin_backward_act(rows_of(dy, "linear gradient"), given(signs), slope, (int)dz_type, given(db), accumulate);
   });
-  m.def("linear_backward_data", [](const Tensor& dz, const Tensor& w) {
+  m.def("linear_backward_data", [](const Tensor& dz, const Tensor& w, const MaybeTensor& signs, double slope) {
     on_device(dz, "linear gradient");
     const Rows r = rows_of(dz, "linear gradient");
-    return lin_backward_data(r, w, {r.rows, w.size(-1)});
+    return lin_backward_data(r, given(signs), slope, w, {r.rows, w.size(-1)});
   });
   m.def("linear_backward_weight", [](const Tensor& dz, const MaybeTensor& x, const MaybeTensor& codes, const MaybeTensor& exps, const Tensor& dw,
-                                     bool accumulate) {
+                                     bool accumulate, const MaybeTensor& db, bool bias_accumulate, const MaybeTensor& signs, double slope) {
     on_device(dz, "linear gradient");
-    lin_backward_weight(rows_of(dz, "linear gradient"), given(x), Packed{given(codes), given(exps)}, dw, accumulate);
+    lin_backward_weight(rows_of(dz, "linear gradient"), given(signs), slope, given(x), Packed{given(codes), given(exps)}, dw, accumulate, given(db),
+                        bias_accumulate);
   });
 }

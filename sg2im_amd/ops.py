@@ -1366,13 +1366,14 @@ def linear_backward_act(dy, signs, slope, dz_dtype=None, dbias=None, accumulate=
   return _lib.eager().linear_backward_act(dy, signs, slope, _code(dz_dtype, 'linear gradient'), dbias, accumulate)
 
 
-def linear_backward_data(dz, weight):
-  """dx = dz W for dz (M, N) and a dense W (N, K) of one type"""
-  return _lib.eager().linear_backward_data(dz, weight)
+def linear_backward_data(dz, weight, signs=None, slope=1.0):
+  """dx = dz W for dz (M, N) and a dense W (N, K) of one type; with ``signs``, ``dz`` is dy and takes leaky'(z) on its way"""
+  return _lib.eager().linear_backward_data(dz, weight, signs, slope)
 
 
-def linear_backward_weight(dz, x, dweight, accumulate=False):
-  """dweight (N, K) (+)= dz^T x; x: the layer's input (..., K) or its Packed8"""
+def linear_backward_weight(dz, x, dweight, accumulate=False, dbias=None, bias_accumulate=False, signs=None, slope=1.0):
+  """dweight (N, K) (+)= dz^T x, dbias (N,) (+)= dz's column sums; x: the layer's input (..., K) or its Packed8; with
+  ``signs``, ``dz`` is dy and takes leaky'(z) on its way"""
   xt, codes, exps, _ = _either(x)
-  _lib.eager().linear_backward_weight(dz, xt, codes, exps, dweight, accumulate)
+  _lib.eager().linear_backward_weight(dz, xt, codes, exps, dweight, accumulate, dbias, bias_accumulate, signs, slope)
   return dweight

@@ -266,7 +266,8 @@ def lin_bounds(x, xs, w, b, res, slope, dy, bits, t_op, dz_type):
   rz = 0.0 if bits is None and dy.dtype == t_op else half_step(t_op)
   r['dx'], r['dx_tol'] = dz @ w, ((N + 2) * u32 + rz) * (dz.abs() @ w.abs())
   r['dw'], r['dw_tol'] = dz.t() @ xs, ((M + 2) * u32 + rz) * (dz.abs().t() @ xs.abs())
-  r['db'], r['db_tol'] = dz.sum(0), (64 + T) * u32 * dz.abs().sum(0)
+  # (a thread adds up four rows of a chunk of 32, then the chunks, then 32 threads, then the splits)
+  r['db'], r['db_tol'] = dz.sum(0), (4 + M / 32 + 32 + 128) * u32 * dz.abs().sum(0)
   return r
 
 
@@ -504,10 +505,9 @@ def test_entry_points_refuse_without_a_gpu():
               dict(m=1 << 31), dict(yd=1), dict(xd=3), dict(bd=2)):
     assert lin(**bad) == E, bad
   assert lin(m=0) == _lib.SG2IM_OK
-  assert lib.sg2im_linear_backward_data(one, 0, 7, one, one, 8, 4, 8, 8, None, 0, None) == E
-  assert lib.sg2im_linear_backward_weight(one, 0, 8, one, 7, None, None, one, 0, 0, 4, 8, 8, None, 0, None) == E
-  assert lib.sg2im_linear_backward_weight(one, 0, 8, None, 8, one, None, one, 0, 0, 4, 8, 8, None, 0, None) == E
-  assert lib.sg2im_linear_backward_weight(one, 0, 8, one, 8, None, None, one, 1, 0, 4, 8, 8, None, 0, None) == E
+  assert lib.sg2im_linear_backward_data(one, 0, 7, None, 1.0, one, one, 8, 4, 8, 8, None, 0, None) == E
+  for x, ldx, co, wt, bt in ((one, 7, None, 0, 0), (None, 8, one, 0, 0), (one, 8, None, 1, 0), (one, 8, None, 0, 2), (None, 8, None, 0, 0)):
+    assert lib.sg2im_linear_backward_weight(one, 0, 8, None, 1.0, x, ldx, co, None, one, wt, 0, one, bt, 0, 4, 8, 8, None, 0, None) == E
   assert lib.sg2im_linear_backward_act(one, 0, 8, None, 0.2, None, 0, one, 0, 0, 4, 8, None, 0, None) == E
   assert lib.sg2im_linear_backward_act(one, 1, 8, None, 0.2, one, 0, None, 0, 0, 4, 8, None, 0, None) == E
   for args in ((None, 0, 4, 8, 8, one, one), (one, 0, 4, 8, 7, one, one), (one, 2, 4, 8, 8, one, one), (one, 0, -1, 8, 8, one, one),
