@@ -90,6 +90,20 @@ template <typename T> __device__ __forceinline__ Piece load_part(const T* p, int
   return r;
 }
 
+// 128 bits moved down by n, zeros from above
+__device__ __forceinline__ uint4 moved(const uint4& w, int n) {
+  typedef unsigned long long u64;
+  const u64 lo = w.x | (u64)w.y << 32, hi = w.z | (u64)w.w << 32;
+  const int k = n & 63;
+  const u64 l = n >= 64 ? hi : lo, h = n >= 64 ? 0 : hi;
+  const u64 a = (l >> k) | ((h << 1) << (63 - k)), b = h >> k;
+  const bool none = n >= 128;
+  return make_uint4(none ? 0 : (unsigned)a, none ? 0 : (unsigned)(a >> 32), none ? 0 : (unsigned)b, none ? 0 : (unsigned)(b >> 32));
+}
+
+enum { WHOLE = 0, EDGE = 1, NARROW = 2 };
+template <int V> struct Int { static constexpr int value = V; };
+
 // One operand's way from memory to LDS: ROWS rows from row0, chunk by chunk.
 //   whole: every piece of every full chunk lies inside the operand (the rows of an r-contiguous one are clamped: what a row
 //   behind the last one computes is not stored), so that loads need no check
@@ -146,10 +160,10 @@ template <typename T, int ROWS, int MODE, int NT, bool GATE, bool SUM> struct Fe
       if constexpr (MODE == RM8) exps += (long long)G::BK * nblk;
     }
   }
-  // pieces [I0, I1) of a full chunk of a whole tile
-  template <int I0, int I1> __device__ __forceinline__ void load(Staged<MODE, P>& s) const {
+  // a full chunk of a whole tile
+  __device__ __forceinline__ void load(Staged<MODE, P>& s) const {
     #pragma unroll
-    for (int i = I0; i < I1; ++i) {
+    for (int i = 0; i < P; ++i) {
       if constexpr (GATE) s.g[i] = gate[gate_off[i]];
       if constexpr (MODE == RC) __builtin_memcpy(&s.v[i], base + off[i], 16);
       else {
@@ -162,8 +176,35 @@ template <typename T, int ROWS, int MODE, int NT, bool GATE, bool SUM> struct Fe
       }
     }
   }
-  // any chunk: `left` = how many r there are
-  __device__ __forceinline__ void load_checked(Staged<MODE, P>& s, int left) const {
+  // A chunk of `left` r, or of a tile that reaches over the operand's columns.  A piece over the end is read from where it
+  // just fits and moved into place when it is stored (take), so that the loads stay free of branches; what lies behind the
+  // end becomes zero.  (An operand narrower than a piece goes element by element.)
+  __device__ __forceinline__ bool narrow(int R) const { return (MODE == RC ? R : rows) < NV; }
+  __device__ __forceinline__ int over(int left) const {                    // elements that a piece starts too late for
+    const int tid = threadIdx.x;
+    return MODE == RC ? max(0, (tid & 7) * NV - (left - NV)) : max(0, row0 + tid % PR * NV - (rows - NV));
+  }
+  __device__ __forceinline__ void load_edge(Staged<MODE, P>& s, int left) const {
+    const int tid = threadIdx.x, d = over(left);
+    #pragma unroll
+    for (int i = 0; i < P; ++i) {
+      if constexpr (MODE == RC) {
+        __builtin_memcpy(&s.v[i], base + off[i] - d * (int)sizeof(T), 16);
+        if constexpr (GATE) s.g[i] = gate[gate_off[i] - (tid & 7) * NV / 8 + min((tid & 7) * NV, left - 1) / 8];
+      } else {
+        constexpr int size = MODE == RM8 ? 1 : (int)sizeof(T);
+        const int r = min(tid / PR + NT / PR * i, left - 1), c = tid % PR * NV;
+        const char* at = base + (r * ld + c - d) * size;
+        if constexpr (GATE) s.g[i] = gate[r * gate_ld + min(c, rows - 1 - row0) / 8];
+        if constexpr (MODE == RM) __builtin_memcpy(&s.v[i], at, 16);
+        else {
+          __builtin_memcpy(s.q[i], at, NV);
+          s.e[i] = exps[(long long)r * nblk + min(row0 + c, rows - 1) / C8_BLOCK];
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void load_narrow(Staged<MODE, P>& s, int left) const {
     const int tid = threadIdx.x;
     #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -191,19 +232,23 @@ template <typename T, int ROWS, int MODE, int NT, bool GATE, bool SUM> struct Fe
       }
     }
   }
-  template <int I0, int I1> __device__ __forceinline__ void store(T* lds, const Staged<MODE, P>& s) {
-    const int tid = threadIdx.x;
+  // how: WHOLE, EDGE (load_edge's pieces are moved into place) or NARROW
+  template <int HOW> __device__ __forceinline__ void store(T* lds, const Staged<MODE, P>& s, int left) {
+    const int tid = threadIdx.x, d = HOW == EDGE ? over(left) : 0;
     #pragma unroll
-    for (int i = I0; i < I1; ++i) {
+    for (int i = 0; i < P; ++i) {
+      const bool gone = HOW == EDGE && MODE != RC && tid / PR + NT / PR * i >= left;       // (this r is behind the end)
       T* p;
       if constexpr (MODE == RC) p = lds + ((tid >> 3) + NT / 8 * i) * G::LD + (tid & 7) * NV;
       else p = lds + (tid / PR + NT / PR * i) * G::LD + tid % PR * NV;
       uint4 w;
       if constexpr (MODE == RM8) {
         const float scale = c8_scale(s.e[i]);              // (a piece starts at a multiple of its length: one block)
+        unsigned long long q = s.q[i][0] | (NV == 8 ? (unsigned long long)s.q[i][1] << 32 : 0);
+        if constexpr (HOW == EDGE) q = gone || d >= NV ? 0 : (NV == 8 ? q : q & 0xffffffffu) >> (8 * d);
         float v[NV];
         #pragma unroll
-        for (int j = 0; j < NV; ++j) v[j] = c8_decode((signed char)(s.q[i][j >> 2] >> (8 * (j & 3))), scale);
+        for (int j = 0; j < NV; ++j) v[j] = c8_decode((signed char)(q >> (8 * j)), scale);
         if constexpr (sizeof(T) == 4) w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
         else {
           auto two = [&](int j) { return f32_to_bf16_bits(v[j]) | (unsigned)f32_to_bf16_bits(v[j + 1]) << 16; };
@@ -211,6 +256,7 @@ template <typename T, int ROWS, int MODE, int NT, bool GATE, bool SUM> struct Fe
         }
       } else {
         w = make_uint4(s.v[i].w[0], s.v[i].w[1], s.v[i].w[2], s.v[i].w[3]);
+        if constexpr (HOW == EDGE) w = moved(w, gone ? 128 : d * (int)sizeof(T) * 8);
         if constexpr (GATE || SUM) {
           RawVec<T, NV> raw;
           __builtin_memcpy(&raw, &w, 16);
@@ -338,7 +384,8 @@ __device__ __forceinline__ void interleave() {
 template <typename T, int MODE> constexpr int READS_OF = MODE == RC ? 1 : sizeof(T) == 2 ? 2 : 4;
 template <typename T> constexpr int MFMAS_OF = sizeof(T) == 2 ? 1 : 4;
 
-template <typename T, int BM, int BN, int NT, int AMODE, int BMODE, bool GATE, bool SUM>
+// EDGES: there are partial chunks or tiles over the end of an i / j contiguous operand
+template <typename T, int BM, int BN, int NT, int AMODE, int BMODE, bool GATE, bool SUM, bool EDGES>
 __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
   typedef Feeder<T, BM, AMODE, NT, GATE, SUM> FA;
   typedef Feeder<T, BN, BMODE, NT, false, false> FB;
@@ -377,24 +424,19 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
   FB fb(p, p.b, p.ldb, p.b_exps, p.b_nblk, j0, p.J, r_begin);
   Staged<AMODE, FA::P> sa;
   Staged<BMODE, FB::P> sb;
-  const bool quick = fa.whole() && fb.whole();
-  int fetched = 0;                                                 // chunks on their way so far
-  auto fetch_quick = [&]() {
-    fa.template load<0, FA::P>(sa);
-    fb.template load<0, FB::P>(sb);
+  const bool whole = fa.whole() && fb.whole(), narrow = fa.narrow(p.R) || fb.narrow(p.R);
+  int fetched = 0, staged = 0;                                     // chunks on their way so far; how many r the last one has
+  auto fetch = [&](auto how) {
+    staged = length - fetched * BK;
+    if constexpr (how.value == WHOLE) { fa.load(sa); fb.load(sb); }
+    else if constexpr (how.value == EDGE) { fa.load_edge(sa, staged); fb.load_edge(sb, staged); }
+    else { fa.load_narrow(sa, staged); fb.load_narrow(sb, staged); }
     fa.next(); fb.next();
     ++fetched;
   };
-  auto fetch = [&]() {
-    if (quick && fetched < full) { fetch_quick(); return; }
-    fa.load_checked(sa, length - fetched * BK);
-    fb.load_checked(sb, length - fetched * BK);
-    fa.next(); fb.next();
-    ++fetched;
-  };
-  auto put = [&](int image) {
-    fa.template store<0, FA::P>(lds_a + image * GA::ELEMS, sa);
-    fb.template store<0, FB::P>(lds_b + image * GB::ELEMS, sb);
+  auto put = [&](auto how, int image) {
+    fa.template store<how.value>(lds_a + image * GA::ELEMS, sa, staged);
+    fb.template store<how.value>(lds_b + image * GB::ELEMS, sb, staged);
   };
   typedef decltype(operand<BM, AMODE>(lds_a, 0, 0, 0)) Op;
   Op oa[2][TI], ob[2][TJ];
@@ -411,45 +453,55 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
       for (int b = 0; b < TJ; ++b) acc[a][b] = multiply(ob[from][b], oa[from][a], acc[a][b]);
   };
 
+  // the products of chunks [c, end), with chunk c + 1 put and c + 2 fetched next to those of chunk c
+  int c = 0;
+  auto run_to = [&](auto how, int end) {
+    for (; c < end; ++c) {
+      const int image = c & 1;
+      // The order inside a step: the LDS and memory traffic spread between the products (left to itself the compiler moves
+      // each access next to its use, and the matrix cores wait for it)
+      read(1, image, 1);
+      put(how, image ^ 1);
+      compute(0);
+      interleave<NP, NR, NL, 0>();
+      SG2IM_FENCE();
+      read(0, image, 2);
+      fetch(how);
+      compute(1);
+      interleave<NP, NR, 0, NL>();
+      SG2IM_FENCE();
+      read(1, image, 3);
+      compute(0);
+      interleave<NP, NR, 0, 0>();
+      __syncthreads();
+      SG2IM_FENCE();
+      read(0, image ^ 1, 0);
+      compute(1);
+      interleave<NP, NR, 0, 0>();
+      SG2IM_FENCE();
+    }
+  };
+  // One that has all its pieces is loaded without checks, and so is each of its full chunks
+  auto with_form = [&](int chunk, auto f) {
+    if constexpr (!EDGES) f(Int<WHOLE>());
+    else if (narrow) f(Int<NARROW>());
+    else if (whole && chunk < full) f(Int<WHOLE>());
+    else f(Int<EDGE>());
+  };
   if (chunks > 0) {
-    fetch();
-    put(0);
-    if (chunks > 1) fetch();
+    with_form(0, [&](auto how) { fetch(how); put(how, 0); });
+    if (chunks > 1) with_form(1, fetch);
     __syncthreads();
     read(0, 0, 0);
-    int c = 0;
-    if (quick)
-      for (; c + 2 < full; ++c) {                                  // (the same as below without its questions)
-        const int image = c & 1;
-        // The order inside a step: the LDS and memory traffic spread between the products (left to itself the compiler moves
-        // each access next to its use, and the matrix cores wait for it)
-        read(1, image, 1);
-        put(image ^ 1);
-        compute(0);
-        interleave<NP, NR, NL, 0>();
-        SG2IM_FENCE();
-        read(0, image, 2);
-        fetch_quick();
-        compute(1);
-        interleave<NP, NR, 0, NL>();
-        SG2IM_FENCE();
-        read(1, image, 3);
-        compute(0);
-        interleave<NP, NR, 0, 0>();
-        __syncthreads();
-        SG2IM_FENCE();
-        read(0, image ^ 1, 0);
-        compute(1);
-        interleave<NP, NR, 0, 0>();
-        SG2IM_FENCE();
-      }
+    if (!EDGES || (whole && !narrow)) run_to(Int<WHOLE>(), full - 2);
+    if constexpr (EDGES) if (!whole && !narrow) run_to(Int<EDGE>(), chunks - 2);
     for (; c < chunks; ++c) {
       const int image = c & 1;
       read(1, image, 1);
-      if (c + 1 < chunks) put(image ^ 1);
+      if (c + 1 < chunks) with_form(c + 1, [&](auto how) { put(how, image ^ 1); });
       compute(0);
       read(0, image, 2);
-      if (c + 2 < chunks) fetch();
+      if (c + 2 < chunks) with_form(c + 2, fetch);
       compute(1);
       read(1, image, 3);
       compute(0);
@@ -622,19 +674,19 @@ struct Plan { int tile, splits, r_per_split; double us; };
 // 32768 x 256 x 1024 33, 27, 33; 131072 x 64 x 256 38, 28, 19; 256 x 1024 x 32768 with 16 splits of the 128-tile 40, none
 // split faster than 44; 2048 x 2048 x 512 12.4 with one, 30 with two.
 // work: what the gate (GATED) or the sums (SUMMED) add to the 128 tile's chunk (bfloat16, 2048 x 512 x 2048: dx 13.6 -> 21.7 us
-// gated, 32768 x 512 x 512 29 -> 42; dW with its sums 14.4 -> 17.2); their kernels have no 256 tile (the registers of two
-// waves per SIMD do not hold it).
+// gated, 32768 x 512 x 512 29 -> 42; dW with its sums 14.4 -> 17.2); their kernels have no 256 tile, nor
+// have products with edges (which: 0 forward, 1 dx, 2 dW): the registers of two waves per SIMD do not hold more.
 constexpr double GATED[2] = {0.20, 0.35}, SUMMED[2] = {0.05, 0.12};
 struct TileCost { int tile, per_cu; double fixed, latency, share; };
 constexpr TileCost COSTS[2][3] = {{{64, 3, 2.0, 0.55, 0.50}, {128, 2, 3.0, 1.9, 1.85}, {256, 1, 6.0, 7.5, 7.5}},        // float
                                   {{64, 3, 2.0, 0.33, 0.23}, {128, 2, 3.0, 0.65, 0.62}, {256, 1, 6.0, 1.75, 1.75}}};    // bfloat16
-inline Plan plan(long long I, long long J, long long R, int bf16, double work = 0.0) {
+inline Plan plan(int which, long long I, long long J, long long R, int bf16, double work = 0.0) {
   static const int ways[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128};
   const int bk = bf16 ? 64 : 32;
   const long long steps = std::max(1LL, (R + bk - 1) / bk);
   Plan best = {64, 1, (int)(steps * bk), 1e30};
   for (const TileCost& t : COSTS[bf16]) {
-    if (work > 0.0 && t.tile == 256) break;
+    if (t.tile == 256 && (work > 0.0 || R % bk || (which >= 1 && J % 256) || (which == 2 && I % 256))) break;
     const long long tiles = ((I + t.tile - 1) / t.tile) * ((J + t.tile - 1) / t.tile);
     for (int w : ways) {
       if (w > steps || (w > 1 && tiles * w > 1024)) break;
@@ -664,9 +716,9 @@ int run(Product& p, const Plan& q, void* workspace, size_t workspace_bytes, hipS
   const long long blocks = (long long)p.tiles_j * p.tiles_i * q.splits;
   if (blocks > 0x7fffffffLL) return SG2IM_ERR_ARG;
   const dim3 grid((unsigned)blocks);
-  if constexpr (!GATE && !SUM) if (q.tile == 256) SG2IM_LAUNCH((product_kernel<T, 256, 256, 512, AMODE, BMODE, GATE, SUM>), grid, dim3(512), 0, stream, p);
-  if (q.tile == 128) SG2IM_LAUNCH((product_kernel<T, 128, 128, 256, AMODE, BMODE, GATE, SUM>), grid, dim3(256), 0, stream, p);
-  if (q.tile == 64) SG2IM_LAUNCH((product_kernel<T, 64, 64, 256, AMODE, BMODE, GATE, SUM>), grid, dim3(256), 0, stream, p);
+  if constexpr (!GATE && !SUM) if (q.tile == 256) SG2IM_LAUNCH((product_kernel<T, 256, 256, 512, AMODE, BMODE, GATE, SUM, false>), grid, dim3(512), 0, stream, p);
+  if (q.tile == 128) SG2IM_LAUNCH((product_kernel<T, 128, 128, 256, AMODE, BMODE, GATE, SUM, true>), grid, dim3(256), 0, stream, p);
+  if (q.tile == 64) SG2IM_LAUNCH((product_kernel<T, 64, 64, 256, AMODE, BMODE, GATE, SUM, true>), grid, dim3(256), 0, stream, p);
   if (q.splits > 1) {
     const long long pieces = (long long)p.I * ((p.J + 31) / 32) * 8;
     if (q.splits >= 8 && pieces < 1 << 16) SG2IM_LAUNCH(join_kernel<8>, dim3((unsigned)((pieces + 31) / 32)), dim3(THREADS), 0, stream, p);

@@ -131,10 +131,10 @@ extern "C" {
 size_t sg2im_linear_workspace(long long rows, int k, int n, int dtype, int which) {
   if (!sizes_ok(rows, k, n) || !type_ok(dtype) || rows == 0) return 16;
   if (which == 3) return std::max((size_t)16, (size_t)act_plan(rows, n).chunks * n * 4);
-  if (which == 0) return plan_bytes(plan(rows, n, k, dtype), rows, n, false);
-  if (which == 1) return std::max(plan_bytes(plan(rows, k, n, dtype), rows, k, false), plan_bytes(plan(rows, k, n, dtype, GATED[dtype]), rows, k, false));
-  return std::max({plan_bytes(plan(n, k, rows, dtype), n, k, false), plan_bytes(plan(n, k, rows, dtype, GATED[dtype]), n, k, true),
-                   plan_bytes(plan(n, k, rows, dtype, SUMMED[dtype]), n, k, true)});
+  if (which == 0) return plan_bytes(plan(0, rows, n, k, dtype), rows, n, false);
+  if (which == 1) return std::max(plan_bytes(plan(1, rows, k, n, dtype), rows, k, false), plan_bytes(plan(1, rows, k, n, dtype, GATED[dtype]), rows, k, false));
+  return std::max({plan_bytes(plan(2, n, k, rows, dtype), n, k, false), plan_bytes(plan(2, n, k, rows, dtype, GATED[dtype]), n, k, true),
+                   plan_bytes(plan(2, n, k, rows, dtype, SUMMED[dtype]), n, k, true)});
 }
 
 int sg2im_linear_backward_act_first(long long rows, int k, int n, int dtype, int gated, int bias, int need_dx, int need_dw) {
@@ -143,10 +143,10 @@ int sg2im_linear_backward_act_first(long long rows, int k, int n, int dtype, int
   // one pass over dy (and dz to memory) at 4.5 TB/s and its last sum, then plain products; or products that do it themselves
   const double es = dtype ? 2 : 4;
   double first = 8.0 + es * rows * n * (gated ? 2 : 1) / 4.5e6, itself = 0.0;
-  if (need_dx && gated) { first += plan(rows, k, n, dtype).us; itself += plan(rows, k, n, dtype, GATED[dtype]).us; }
+  if (need_dx && gated) { first += plan(1, rows, k, n, dtype).us; itself += plan(1, rows, k, n, dtype, GATED[dtype]).us; }
   if (need_dw) {
-    first += plan(n, k, rows, dtype).us;
-    itself += plan(n, k, rows, dtype, gated ? GATED[dtype] : SUMMED[dtype]).us;
+    first += plan(2, n, k, rows, dtype).us;
+    itself += plan(2, n, k, rows, dtype, gated ? GATED[dtype] : SUMMED[dtype]).us;
   }
   return first < itself;
 }
@@ -163,7 +163,7 @@ int sg2im_linear_forward(const void* x, int dtype, long long ld_x, const void* w
   p.a = x; p.lda = ld_x; p.b = weight; p.ldb = k; p.I = (int)rows; p.J = n; p.R = k;
   p.bias = bias; p.bias_bf16 = bias_dtype; p.residual = residual; p.ld_res = ld_res; p.slope = slope;
   p.signs = signs; p.sign_words = (n + 31) / 32; p.out = out; p.out_bf16 = out_dtype; p.ld_out = ld_out;
-  const Plan q = plan(rows, n, k, dtype);
+  const Plan q = plan(0, rows, n, k, dtype);
   return dtype == 0 ? run<float, RC, RC, false, false>(p, q, workspace, workspace_bytes, stream)
                     : run<bf16_s, RC, RC, false, false>(p, q, workspace, workspace_bytes, stream);
 }
@@ -200,7 +200,7 @@ int sg2im_linear_backward_data(const void* dz, int dtype, long long ld_dz, const
   p.a = dz; p.lda = ld_dz; p.b = weight; p.ldb = k; p.I = (int)rows; p.J = k; p.R = n;
   p.slope = 1.f; p.out = dx; p.out_bf16 = dtype; p.ld_out = ld_dx;
   p.gate = reinterpret_cast<const unsigned char*>(signs); p.gate_ld = (n + 31) / 32 * 4LL; p.gate_slope = slope;
-  const Plan q = plan(rows, k, n, dtype, signs ? GATED[dtype] : 0.0);
+  const Plan q = plan(1, rows, k, n, dtype, signs ? GATED[dtype] : 0.0);
   if (signs) return dtype == 0 ? run<float, RC, RM, true, false>(p, q, workspace, workspace_bytes, stream)
                                : run<bf16_s, RC, RM, true, false>(p, q, workspace, workspace_bytes, stream);
   return dtype == 0 ? run<float, RC, RM, false, false>(p, q, workspace, workspace_bytes, stream)
@@ -221,7 +221,7 @@ int sg2im_linear_backward_weight(const void* dz, int dtype, long long ld_dz, con
   p.sum = dbias; p.sum_bf16 = bias_dtype; p.sum_accumulate = bias_accumulate;
   if (codes) { p.b = codes; p.ldb = k; p.b_exps = exps; p.b_nblk = (k + C8_BLOCK - 1) / C8_BLOCK; }
   else { p.b = x; p.ldb = ld_x; }
-  const Plan q = plan(n, k, std::max(1LL, rows), dtype, signs ? GATED[dtype] : dbias ? SUMMED[dtype] : 0.0);   // (no row: one empty sum, zeros or what was there)
+  const Plan q = plan(2, n, k, std::max(1LL, rows), dtype, signs ? GATED[dtype] : dbias ? SUMMED[dtype] : 0.0);   // (no row: one empty sum, zeros or what was there)
   return run_weight(p, dtype, codes != nullptr, q, workspace, workspace_bytes, stream);
 }
 
