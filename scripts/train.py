@@ -110,6 +110,9 @@ parser.add_argument('--seed', default=0, type=int)
 parser.add_argument('--use_graphs', default=True, type=bool_flag)
 parser.add_argument('--bucket_objects', default=32, type=int)
 parser.add_argument('--bucket_triples', default=64, type=int)
+# (with --normalization / --d_normalization group, or M tokens in --d_obj_arch / --d_img_arch: these layers' backward pass
+# keeps its activations in 8 bits)
+parser.add_argument('--checkpoint8', default=False, type=bool_flag)
 parser.add_argument('--align_corners', default=False, type=bool_flag,
                     help='bilinear sampling convention of layout / crops: False = F.grid_sample of torch >= 1.3, '
                          'True = torch 0.4 (what the reference authors trained with)')
@@ -296,6 +299,8 @@ def main(args):
             normalization=args.normalization, activation=args.activation, mask_size=args.mask_size,
             layout_noise_dim=args.layout_noise_dim)
   dk = dict(normalization=args.d_normalization, activation=args.d_activation, padding=args.d_padding)
+  if args.checkpoint8:
+    gk['checkpoint8'] = dk['checkpoint8'] = True
   lw = {k: getattr(args, k) for k in ('l1_pixel_loss_weight', 'bbox_pred_loss_weight', 'predicate_pred_loss_weight',
                                       'mask_loss_weight', 'discriminator_loss_weight', 'd_obj_weight',
                                       'd_img_weight', 'ac_loss_weight')}

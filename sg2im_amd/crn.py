@@ -10,14 +10,15 @@ class RefinementModule(nn.Module):
   Sequential(conv3x3, norm, act, conv3x3, norm, act).  The compute happens in
   RefinementNetwork.forward_nhwc, which runs all modules as one fused HIP sequence."""
 
-  def __init__(self, layout_dim, input_dim, output_dim, normalization='instance', activation='leakyrelu'):
+  def __init__(self, layout_dim, input_dim, output_dim, normalization='instance', activation='leakyrelu',
+               checkpoint8=False):
     super(RefinementModule, self).__init__()
     layers = [
       nn.Conv2d(layout_dim + input_dim, output_dim, kernel_size=3, padding=1),
-      get_normalization_2d(output_dim, normalization),
+      get_normalization_2d(output_dim, normalization, checkpoint8),
       get_activation(activation),
       nn.Conv2d(output_dim, output_dim, kernel_size=3, padding=1),
-      get_normalization_2d(output_dim, normalization),
+      get_normalization_2d(output_dim, normalization, checkpoint8),
       get_activation(activation),
     ]
     layers = [l for l in layers if l is not None]
@@ -29,11 +30,13 @@ class RefinementModule(nn.Module):
 
 class RefinementNetwork(nn.Module):
   """reference sg2im/crn.py:68-111.  ``forward(layout NCHW) -> image NCHW`` keeps the
-  reference signature; ``forward_nhwc`` is the zero-conversion entry the model uses."""
+  reference signature; ``forward_nhwc`` is the zero-conversion entry the model uses.
+  normalization='group' and checkpoint8 (its backward pass keeps the convolutions' outputs in 8 bits) are not the
+  reference's."""
 
-  def __init__(self, dims, normalization='instance', activation='leakyrelu'):
+  def __init__(self, dims, normalization='instance', activation='leakyrelu', checkpoint8=False):
     super(RefinementNetwork, self).__init__()
-    if normalization not in ('batch', 'none', 'instance'):
+    if normalization not in ('batch', 'none', 'instance', 'group'):
       raise ValueError('Unrecognized normalization type "%s"' % normalization)
     self.normalization = normalization
     layout_dim = dims[0]
@@ -42,7 +45,8 @@ class RefinementNetwork(nn.Module):
     for i in range(1, len(dims)):
       input_dim = 1 if i == 1 else dims[i - 1]
       self.refinement_modules.append(
-        RefinementModule(layout_dim, input_dim, dims[i], normalization=normalization, activation=activation))
+        RefinementModule(layout_dim, input_dim, dims[i], normalization=normalization, activation=activation,
+                         checkpoint8=checkpoint8))
     out_layers = [
       nn.Conv2d(dims[-1], dims[-1], kernel_size=3, padding=1),
       get_activation(activation),
@@ -57,14 +61,18 @@ class RefinementNetwork(nn.Module):
     """link: the functional.LayoutLink of the LayoutFn call that produced ``layout_nhwc`` when this network is
     that tensor's ONLY consumer (Sg2ImModel.forward_nhwc): pyramid and per-level gradients travel through it"""
     o0, o2 = self.output_conv[0], self.output_conv[2]
-    if self.normalization in ('none', 'instance'):      # no norm parameters, no running statistics
-      convs = []
+    if self.normalization in ('none', 'instance', 'group'):      # no running statistics
+      convs, norms = [], []
       for mod in self.refinement_modules:
         c0, c1 = [m for m in mod.net if isinstance(m, nn.Conv2d)]
         convs += [c0.weight, c0.bias, c1.weight, c1.bias]
+        norms += [m for m in mod.net if isinstance(m, nn.GroupNorm)]
       params = convs + [o0.weight, o0.bias, o2.weight, o2.bias]
+      for n in norms:
+        params += [n.weight, n.bias]
+      spec = [(n.num_groups, n.eps, n.checkpoint8) for n in norms] if norms else self.normalization == 'instance'
       return HF.RefinementNoNormFn.apply(layout_nhwc, len(self.refinement_modules), self.slope,
-                                         layout_grad_channels, self.normalization == 'instance', link, *params)
+                                         layout_grad_channels, spec, link, *params)
     convs, bnps, bns = [], [], []
     for mod in self.refinement_modules:
       c0, n0, _, c1, n1, _ = mod.net

@@ -15,11 +15,12 @@ TWO_HEADS = os.environ.get('SG2IM_TWO_HEADS', '1') != '0'      # (A/B knob)
 
 class PatchDiscriminator(nn.Module):
   def __init__(self, arch, normalization='batch', activation='leakyrelu-0.2', padding='same', pooling='avg',
-               input_size=(128, 128), layout_dim=0):
+               input_size=(128, 128), layout_dim=0, checkpoint8=False):
+    """checkpoint8 (not a reference argument): see layers.build_cnn"""
     super(PatchDiscriminator, self).__init__()
     input_dim = 3 + layout_dim
     self.cnn, output_dim = build_cnn(arch='I%d,%s' % (input_dim, arch), normalization=normalization,
-                                     activation=activation, pooling=pooling, padding=padding)
+                                     activation=activation, pooling=pooling, padding=padding, checkpoint8=checkpoint8)
     # present in the state_dict but never applied (reference sg2im/discriminators.py:40-45)
     self.classifier = nn.Conv2d(output_dim, 1, kernel_size=1, stride=1)
 
@@ -36,11 +37,12 @@ class PatchDiscriminator(nn.Module):
 
 
 class AcDiscriminator(nn.Module):
-  def __init__(self, vocab, arch, normalization='none', activation='relu', padding='same', pooling='avg'):
+  def __init__(self, vocab, arch, normalization='none', activation='relu', padding='same', pooling='avg',
+               checkpoint8=False):
     super(AcDiscriminator, self).__init__()
     self.vocab = vocab
     cnn, D = build_cnn(arch=arch, normalization=normalization, activation=activation, pooling=pooling,
-                       padding=padding)
+                       padding=padding, checkpoint8=checkpoint8)
     self.cnn = nn.Sequential(cnn, GlobalAvgPool(), nn.Linear(D, 1024))
     num_objects = len(vocab['object_idx_to_name'])
     self.real_classifier = nn.Linear(1024, 1)
@@ -73,12 +75,12 @@ class AcDiscriminator(nn.Module):
 
 class AcCropDiscriminator(nn.Module):
   def __init__(self, vocab, arch, normalization='none', activation='relu', object_size=64, padding='same',
-               pooling='avg', align_corners=ALIGN_CORNERS):
+               pooling='avg', align_corners=ALIGN_CORNERS, checkpoint8=False):
     """align_corners (not a reference argument): sampling convention of the crops
-    (reference sg2im/bilinear.py:132), see Sg2ImModel"""
+    (reference sg2im/bilinear.py:132), see Sg2ImModel; checkpoint8: see layers.build_cnn"""
     super(AcCropDiscriminator, self).__init__()
     self.vocab = vocab
-    self.discriminator = AcDiscriminator(vocab, arch, normalization, activation, padding, pooling)
+    self.discriminator = AcDiscriminator(vocab, arch, normalization, activation, padding, pooling, checkpoint8)
     self.object_size = object_size
     self.align_corners = bool(align_corners)
 

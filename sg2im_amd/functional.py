@@ -1054,11 +1054,12 @@ class RefinementFn(Function):
 
 class RefinementNoNormFn(Function):
   """RefinementNetwork with normalization='none' (reference sg2im/crn.py:41-47 drops the norm
-  layers): conv3x3 + LeakyReLU fused in the conv epilogue, twice per module.
-  params (flat): per module [W0, b0, W1, b1] ..., then [Wo0, bo0, Wo2, bo2]."""
+  layers): conv3x3 + LeakyReLU fused in the conv epilogue, twice per module; or with 'instance' / 'group'
+  normalisation between the two.  norm: False, True ('instance'), or per group norm (groups, eps, checkpoint8).
+  params (flat): per module [W0, b0, W1, b1] ..., then [Wo0, bo0, Wo2, bo2], then per group norm [gamma, beta]."""
 
   @staticmethod
-  def forward(ctx, layout, n_modules, slope, grad_channels, inorm, link, *params):
+  def forward(ctx, layout, n_modules, slope, grad_channels, norm, link, *params):
     ops.TIMER_TAG = 'crn'
     try:
       L = n_modules
@@ -1072,6 +1073,15 @@ class RefinementNoNormFn(Function):
       pyr, from_link = _layout_pyramid(layout, L, link)
       ctx.link = link if from_link else None
       saved = []
+      inorm, gnorm = norm is True, norm if isinstance(norm, list) else None
+      out_slope = slope if norm is False else 1.0
+
+      def group(y, k):
+        """group norm k and its activation: (what the backward pass keeps of y, statistics, activated)"""
+        groups, eps, ck = gnorm[k]
+        a, st, packed = ops.group_norm_act_forward(y, params[4 * L + 4 + 2 * k], params[4 * L + 5 + 2 * k], groups, slope, eps,
+                                                   pack=ck)
+        return (y if packed is None else packed), st, a
       for i in range(L):
         h, w = H >> (L - 1 - i), W >> (L - 1 - i)
         W0p, b0, W1p, b1 = params[4 * i:4 * i + 4]
@@ -1080,15 +1090,19 @@ class RefinementNoNormFn(Function):
         # 'none': the activation rides in the conv epilogue; 'instance': the conv output is kept
         # (y), normalised per image and activated into a separate tensor (a)
         y0 = st0 = y1 = st1 = None
-        a0 = ops.conv2d_forward(d0, _cl_weight(W0p), C, b0, _new(layout, N, h, w, C), C, 1.0 if inorm else slope)
+        a0 = ops.conv2d_forward(d0, _cl_weight(W0p), C, b0, _new(layout, N, h, w, C), C, out_slope)
         if inorm:
           y0, st0 = a0, ops.instnorm_stats(a0, BN_EPS)
           a0 = ops.instnorm_act_forward(y0, st0, slope, _new(layout, N, h, w, C))
+        elif gnorm:
+          y0, st0, a0 = group(a0, 2 * i)
         d1 = conv_desc([nhwc_src(a0)], N, h, w, 3, 3, 1, 1)
-        a1 = ops.conv2d_forward(d1, _cl_weight(W1p), C, b1, _new(layout, N, h, w, C), C, 1.0 if inorm else slope)
+        a1 = ops.conv2d_forward(d1, _cl_weight(W1p), C, b1, _new(layout, N, h, w, C), C, out_slope)
         if inorm:
           y1, st1 = a1, ops.instnorm_stats(a1, BN_EPS)
           a1 = ops.instnorm_act_forward(y1, st1, slope, _new(layout, N, h, w, C))
+        elif gnorm:
+          y1, st1, a1 = group(a1, 2 * i + 1)
         saved.append((pyr[i], feat_src, a0, a1, h, w, C, y0, st0, y1, st1))
         feat_src = nhwc_src(a1, 1)
       Wo0, bo0, Wo2, bo2 = params[4 * L:4 * L + 4]
@@ -1100,7 +1114,7 @@ class RefinementNoNormFn(Function):
       img = ops.conv2d_forward(do2, _cl_weight(Wo2), Wo2.size(0), bo2, _new(layout, N, H, W, Wo2.size(0)),
                                Wo2.size(0))
       ctx.saved = saved
-      ctx.misc = (L, slope, z, do0, do2, Cl, Cf, grad_channels, (N, H, W), inorm)
+      ctx.misc = (L, slope, z, do0, do2, Cl, Cf, grad_channels, (N, H, W), norm)
       ctx.save_for_backward(*params)
       return img
     finally:
@@ -1111,12 +1125,22 @@ class RefinementNoNormFn(Function):
     ops.TIMER_TAG = 'crn'
     try:
       params = ctx.saved_tensors
-      L, slope, z, do0, do2, Cl, Cf, grad_channels, (N, H, W), inorm = ctx.misc
+      L, slope, z, do0, do2, Cl, Cf, grad_channels, (N, H, W), norm = ctx.misc
+      inorm, gnorm = norm is True, norm if isinstance(norm, list) else None
       saved = ctx.saved
       ni = ctx.needs_input_grad[6:]
       grads = [None] * len(params)
       Wo0, bo0, Wo2, bo2 = params[4 * L:4 * L + 4]
       g = g.contiguous()
+
+      def through_group(gz, pool2, y, st, k, N, h, w, C, a):
+        """gradient of the activated map (summed over 2x2 where it came through the upsample) -> of group norm k's input"""
+        at = 4 * L + 4 + 2 * k
+        gamma, beta = params[at], params[at + 1]
+        if pool2:
+          gz = ops.act_backward(_fptr(gz), C, 1, N, h, w, a, C, C, 1.0, _new(gz, N, h, w, C))
+        dg, db, acc, grads[at], grads[at + 1] = _bn_grad_bufs(gz, C, gamma, beta, ni[at], ni[at + 1])
+        return ops.group_norm_act_backward(gz, y, gamma, beta, gnorm[k][0], slope, st, True, dg, db, acc)
       Co = Wo0.size(0)
       grads[4 * L + 2], grads[4 * L + 3] = _conv_param_grads(do2, g, Wo2.size(0), (Wo2.size(0), 1, 1, Co),
                                                              ni[4 * L + 2], ni[4 * L + 3], Wo2, bo2)
@@ -1133,7 +1157,10 @@ class RefinementNoNormFn(Function):
         lay, feat_src, a0, a1, h, w, C, y0, st0, y1, st1 = saved[i]
         W0p, b0, W1p, b1 = params[4 * i:4 * i + 4]
         # through the second activation (with the 2x2 sum of the nearest-upsample backward)
-        dy1 = ops.act_backward(_fptr(gz), gz.size(3), pool2, N, h, w, a1, C, C, slope, _new(g, N, h, w, C))
+        if gnorm:
+          dy1 = through_group(gz, pool2, y1, st1, 2 * i + 1, N, h, w, C, a1)
+        else:
+          dy1 = ops.act_backward(_fptr(gz), gz.size(3), pool2, N, h, w, a1, C, C, slope, _new(g, N, h, w, C))
         if inorm:
           ops.instnorm_backward(dy1, y1, st1, dy1)
         d1 = conv_desc([nhwc_src(a0)], N, h, w, 3, 3, 1, 1)
@@ -1144,7 +1171,10 @@ class RefinementNoNormFn(Function):
           grads[4 * i + 3] = _shadowed_bias_grad(b1, ni[4 * i + 3])
         gz0 = _new(g, N, h, w, C)
         ops.conv2d_backward_data(d1, _cl_weight(W1p), C, dy1, C, 0, C, gz0, C)
-        dy0 = ops.act_backward(_fptr(gz0), C, 0, N, h, w, a0, C, C, slope, gz0)
+        if gnorm:
+          dy0 = through_group(gz0, 0, y0, st0, 2 * i, N, h, w, C, a0)
+        else:
+          dy0 = ops.act_backward(_fptr(gz0), C, 0, N, h, w, a0, C, C, slope, gz0)
         if inorm:
           ops.instnorm_backward(dy0, y0, st0, dy0)
         Cprev = feat_src.channels

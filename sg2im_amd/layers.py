@@ -5,6 +5,8 @@ torch.nn modules are used only as *parameter containers* (so state_dict keys, de
 initialisers and ``load_state_dict`` behave exactly like the reference); their own
 ``forward`` is never called - the containers' parents dispatch to HIP kernels.
 """
+import math
+
 import torch
 import torch.nn as nn
 
@@ -20,14 +22,20 @@ def to_channels_last(module):
   return module
 
 
-def get_normalization_2d(channels, normalization):
-  """reference sg2im/layers.py:22-31"""
+def get_normalization_2d(channels, normalization, checkpoint8=False):
+  """reference sg2im/layers.py:22-31, and 'group' (not a reference value): groups of channels / 32 channels (the most
+  groups up to 32 that divide ``channels``), independent of the batch; computed by functional.GroupNormAct.
+  checkpoint8: its backward pass keeps the input in 8 bits."""
   if normalization == 'batch':
     return nn.BatchNorm2d(channels)
   if normalization == 'none':
     return None
   if normalization == 'instance':
     return nn.InstanceNorm2d(channels)      # parameter-free marker; computed by sg2im_instnorm_*
+  if normalization == 'group':
+    norm = nn.GroupNorm(math.gcd(32, channels), channels)
+    norm.checkpoint8 = bool(checkpoint8)
+    return norm
   raise ValueError('Unrecognized normalization type "%s"' % normalization)
 
 
@@ -167,6 +175,8 @@ def _norm_act(norm, act, x, training):
     return HF.BnActRows.apply(x, norm, training, norm.weight, norm.bias, slope)
   if isinstance(norm, nn.InstanceNorm2d):
     return HF.InstNormAct.apply(x, slope)
+  if isinstance(norm, nn.GroupNorm):
+    return HF.GroupNormAct.apply(x, norm.weight, norm.bias, norm.num_groups, slope, norm.eps, norm.checkpoint8)
   return HF.LeakyFn.apply(x, slope)
 
 
@@ -179,7 +189,7 @@ def _run_layers(mods, x, training, bn_inputs=None):
   while i < len(mods):
     m = mods[i]
     nxt = mods[i + 1] if i + 1 < len(mods) else None
-    if isinstance(m, (nn.BatchNorm2d, nn.InstanceNorm2d)):
+    if isinstance(m, (nn.BatchNorm2d, nn.InstanceNorm2d, nn.GroupNorm)):
       if bn_inputs is not None and isinstance(m, nn.BatchNorm2d):
         bn_inputs.append((m, x))
       x = _norm_act(m, nxt, x, training)            # a norm is always followed by its activation
@@ -190,7 +200,7 @@ def _run_layers(mods, x, training, bn_inputs=None):
     elif isinstance(m, nn.Conv2d):
       shadowed = isinstance(nxt, nn.InstanceNorm2d) or (training and isinstance(nxt, nn.BatchNorm2d))
       x = HF.Conv2dFn.apply(x, m.weight, m.bias, m.stride[0], m.padding[0], shadowed)
-    elif isinstance(m, ResidualBlock):
+    elif isinstance(m, (ResidualBlock, PixelMlp)):
       x = m(x)
     elif isinstance(m, nn.Upsample):
       x = HF.UpsampleFn.apply(x, int(m.scale_factor))
@@ -215,14 +225,14 @@ class ResidualBlock(nn.Module):
   Reproduced by a second statistics-only pass over the same inputs."""
 
   def __init__(self, channels, normalization='batch', activation='relu', padding='same', kernel_size=3,
-               init='default'):
+               init='default', checkpoint8=False):
     super(ResidualBlock, self).__init__()
     K, C = kernel_size, channels
     P = _get_padding(K, padding)
     self.padding = P
-    layers = [get_normalization_2d(C, normalization), get_activation(activation),
+    layers = [get_normalization_2d(C, normalization, checkpoint8), get_activation(activation),
               nn.Conv2d(C, C, kernel_size=K, padding=P),
-              get_normalization_2d(C, normalization), get_activation(activation),
+              get_normalization_2d(C, normalization, checkpoint8), get_activation(activation),
               nn.Conv2d(C, C, kernel_size=K, padding=P)]
     layers = [l for l in layers if l is not None]
     for l in layers:
@@ -243,17 +253,43 @@ class ResidualBlock(nn.Module):
     return HF.AddFn.apply(x_nhwc, y)
 
 
-class SeqCnn(nn.Sequential):
-  """build_cnn result for architecture strings with R / U / P / FC tokens: run layer by layer"""
+class PixelMlp(nn.Module):
+  """x + fc2(act(fc1(act(norm(x))))) at every pixel of an NHWC map: group norm and two linear layers (functional.GroupNormAct,
+  LinearResidual; not a reference block - ResidualBlock's shape without its 3x3 windows).  In the bf16 compute mode the
+  two products take bfloat16 operands, and x stays as it is.  checkpoint8: what the backward pass keeps of x and of
+  the two layers' inputs is their 8-bit form - a quarter of float32, half of bfloat16."""
+
+  def __init__(self, channels, hidden, activation='relu', checkpoint8=False):
+    super(PixelMlp, self).__init__()
+    self.norm = get_normalization_2d(channels, 'group', checkpoint8)
+    self.fc1, self.fc2 = nn.Linear(channels, hidden), nn.Linear(hidden, channels)
+    self.slope, self.checkpoint8 = activation_slope(activation), bool(checkpoint8)
 
   def forward(self, x_nhwc):
+    from . import ops
+    n, ck = self.norm, self.checkpoint8
+    half = torch.bfloat16 if ops.CONV_COMPUTE == 1 and x_nhwc.dtype == torch.float32 else None
+    h = HF.GroupNormAct.apply(x_nhwc, n.weight, n.bias, n.num_groups, self.slope, n.eps, ck, half)
+    h = HF.LinearResidual.apply(h, self.fc1.weight, self.fc1.bias, None, self.slope, ck)
+    return HF.LinearResidual.apply(h, self.fc2.weight, self.fc2.bias, x_nhwc, 1.0, ck, x_nhwc.dtype)
+
+
+class SeqCnn(nn.Sequential):
+  """build_cnn result for architecture strings with R / M / U / P / FC tokens or group norms: run layer by layer"""
+
+  def forward(self, x_nhwc, count=None):
+    """count: see DiscCnn; a layer-by-layer network has no batch statistics that could leave padding out"""
+    if count is not None and any(isinstance(m, (nn.BatchNorm2d, nn.BatchNorm1d)) for m in self.modules()):
+      raise NotImplementedError('batch statistics over a padded batch in a layer-by-layer network')
     return _run_layers(self, x_nhwc, self.training)
 
 
-def build_cnn(arch, normalization='batch', activation='relu', padding='same', pooling='max', init='default'):
+def build_cnn(arch, normalization='batch', activation='relu', padding='same', pooling='max', init='default',
+              checkpoint8=False):
   """Architecture-string CNN builder (reference sg2im/layers.py:129-213): I<C>, C<K>-<X>[-<S>], R,
-  U<f>, P<f>, FC-<in>-<out>.  Strings made of 'C' tokens only (every default of scripts/train.py)
-  become a DiscCnn, whose norm + activation ride in the next conv's loader; anything else becomes
+  U<f>, P<f>, FC-<in>-<out>, and (not a reference token) M<hidden>: a PixelMlp.  checkpoint8: group norms and PixelMlps
+  keep what their backward pass needs in 8 bits.  Strings made of 'C' tokens only (every default of scripts/train.py)
+  become - but for normalization='group' - a DiscCnn, whose norm + activation ride in the next conv's loader; anything else becomes
   a SeqCnn that runs one HIP op per module.  Module order, and so the state_dict, is the reference's."""
   if isinstance(arch, str):
     arch = arch.split(',')
@@ -269,7 +305,7 @@ def build_cnn(arch, normalization='batch', activation='relu', padding='same', po
       K, next_C = vals[0], vals[1]
       stride = vals[2] if len(vals) == 3 else 1
       if not first_conv:
-        layers.append(get_normalization_2d(cur_C, normalization))
+        layers.append(get_normalization_2d(cur_C, normalization, checkpoint8))
         layers.append(get_activation(activation))
       first_conv = False
       P = _get_padding(K, padding)
@@ -279,7 +315,10 @@ def build_cnn(arch, normalization='batch', activation='relu', padding='same', po
       cur_C = next_C
     elif tok[0] == 'R':
       layers.append(ResidualBlock(cur_C, normalization='none' if first_conv else normalization,
-                                  activation=activation, padding=padding, init=init))
+                                  activation=activation, padding=padding, init=init, checkpoint8=checkpoint8))
+      first_conv = False
+    elif tok[0] == 'M':
+      layers.append(PixelMlp(cur_C, int(tok[1:]), activation, checkpoint8))
       first_conv = False
     elif tok[0] == 'U':
       layers.append(nn.Upsample(scale_factor=int(tok[1:]), mode='nearest'))
@@ -299,7 +338,7 @@ def build_cnn(arch, normalization='batch', activation='relu', padding='same', po
     else:
       raise ValueError('Invalid layer "%s"' % tok)
   layers = [l for l in layers if l is not None]
-  if all(tok[0] == 'C' for tok in arch):
+  if all(tok[0] == 'C' for tok in arch) and normalization != 'group':
     cnn = DiscCnn(*layers).configure(specs, activation_slope(activation))
   else:
     cnn = SeqCnn(*layers)

@@ -19,11 +19,13 @@ class Sg2ImModel(nn.Module):
   def __init__(self, vocab, image_size=(64, 64), embedding_dim=64, gconv_dim=128, gconv_hidden_dim=512,
                gconv_pooling='avg', gconv_num_layers=5, refinement_dims=(1024, 512, 256, 128, 64),
                normalization='batch', activation='leakyrelu-0.2', mask_size=None,
-               mlp_normalization='none', layout_noise_dim=0, align_corners=ALIGN_CORNERS, **kwargs):
+               mlp_normalization='none', layout_noise_dim=0, align_corners=ALIGN_CORNERS,
+               checkpoint8=False, **kwargs):
     """align_corners (not a reference argument): the bilinear sampling convention of the layout
     (reference sg2im/layout.py:53,88 call F.grid_sample without it): False = torch >= 1.3, what the
     reference computes under a current torch; True = torch 0.4, what the authors trained their
-    released checkpoints with (SURVEY.md section 8c caveat i)."""
+    released checkpoints with (SURVEY.md section 8c caveat i).  checkpoint8 (not a reference argument): with
+    normalization='group' (neither) the refinement network's backward pass keeps the convolutions' outputs in 8 bits."""
     super(Sg2ImModel, self).__init__()
     if len(kwargs) > 0:      # reference sg2im/model.py:41-42
       print('WARNING: Model got unexpected kwargs ', kwargs)
@@ -55,7 +57,7 @@ class Sg2ImModel(nn.Module):
     self.rel_aux_net = build_mlp([2 * embedding_dim + 8, gconv_hidden_dim, num_preds],
                                  batch_norm=mlp_normalization)
     self.refinement_net = RefinementNetwork(dims=(gconv_dim + layout_noise_dim,) + tuple(refinement_dims),
-                                            normalization=normalization, activation=activation)
+                                            normalization=normalization, activation=activation, checkpoint8=checkpoint8)
 
   def _build_mask_net(self, num_objs, dim, mask_size):
     """Container with the Sequential indices of reference sg2im/model.py:94-106."""
