@@ -29,6 +29,21 @@ template <> __device__ __forceinline__ void store1<bf16_s>(bf16_s* p, float v) {
 template <typename T, int NV> struct RawVec { unsigned short h[NV]; };
 template <int NV> struct RawVec<float, NV> { float h[NV]; };
 
+typedef unsigned u32x4_u __attribute__((ext_vector_type(4), aligned(1)));
+typedef unsigned u32x2_u __attribute__((ext_vector_type(2), aligned(1)));
+typedef unsigned u32_u __attribute__((aligned(1)));
+template <int BYTES> __device__ __forceinline__ void store_bytes_nt(void* p, const void* from) {
+  static_assert(BYTES == 16 || BYTES == 8 || BYTES == 4, "one store");
+  if constexpr (BYTES == 16) { u32x4_u w; __builtin_memcpy(&w, from, 16); __builtin_nontemporal_store(w, reinterpret_cast<u32x4_u*>(p)); }
+  else if constexpr (BYTES == 8) { u32x2_u w; __builtin_memcpy(&w, from, 8); __builtin_nontemporal_store(w, reinterpret_cast<u32x2_u*>(p)); }
+  else { u32_u w; __builtin_memcpy(&w, from, 4); __builtin_nontemporal_store(w, reinterpret_cast<u32_u*>(p)); }
+}
+template <int BYTES> __device__ __forceinline__ void load_bytes_nt(void* to, const void* p) {
+  static_assert(BYTES == 16 || BYTES == 8, "one load");
+  if constexpr (BYTES == 16) { const u32x4_u w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_u*>(p)); __builtin_memcpy(to, &w, 16); }
+  else { const u32x2_u w = __builtin_nontemporal_load(reinterpret_cast<const u32x2_u*>(p)); __builtin_memcpy(to, &w, 8); }
+}
+
 template <typename T, int NV> __device__ __forceinline__ RawVec<T, NV> load_raw(const T* p) {
   RawVec<T, NV> r;
   __builtin_memcpy(&r, p, sizeof(r));
@@ -52,6 +67,16 @@ template <typename T, int NV> __device__ __forceinline__ void store_vec(T* p, co
     if constexpr (sizeof(T) == 4) r.h[j] = v[j]; else r.h[j] = f32_to_bf16_bits(v[j]);
   }
   __builtin_memcpy(p, &r, sizeof(r));
+}
+
+// the same past the caches: for what is larger than they are, or not read again soon
+template <typename T, int NV> __device__ __forceinline__ void store_vec_nt(T* p, const float (&v)[NV]) {
+  RawVec<T, NV> r;
+  #pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if constexpr (sizeof(T) == 4) r.h[j] = v[j]; else r.h[j] = f32_to_bf16_bits(v[j]);
+  }
+  store_bytes_nt<sizeof(r)>(p, &r);
 }
 
 // the parameters (affine, bias) are float32 or bfloat16: a wave-uniform choice
