@@ -49,8 +49,12 @@ struct Params {
   int grad_bf16, accumulate;
   long long E;
   int N, C, G, D, L, rows, full_rows, chunks, rows_per_chunk, slabs, TV, TP, nblk;
-  int S;                             // resident kernels: positions per workgroup
+  int S;                             // slab kernels: positions per workgroup
+  int merged;                        // the normalising pass joins the chunks' sums itself
+  int bypass;                        // the backward statistics read dy past the caches
 };
+
+template <bool V> struct Flag { static constexpr bool value = V; };
 
 // the lane's place: position q0 of its piece in a row, the pixel lane, and this workgroup's image / rows
 struct Place { int q0, pl, n, row0, row1; bool on; };
@@ -169,7 +173,8 @@ __device__ __forceinline__ void each_row(const Params& p, const Place& w, int NV
 
 // ---- forward ------------------------------------------------------------------------------------------------------
 
-// sums over the pixel lanes of NV values per thread: out(position of the slab, sum); buf: THREADS * NV values
+// sums over the pixel lanes of NV values per thread: out(position of the slab, sum); buf: THREADS * NV values.  (One thread
+// per position: spreading a position over idle threads, as the slab kernels do, measured 0.5 - 1 us slower here.)
 template <typename V, int NV, typename F>
 __device__ __forceinline__ void sum_pixel_lanes(const V (&s)[NV], V* buf, int TV, int TP, int pl, F out) {
   if (pl < TP) {
@@ -229,12 +234,15 @@ __device__ __forceinline__ void block_sum2(double& a, double& b, double (*red)[2
   for (int i = 0; i < waves; ++i) { a += red[i][0]; b += red[i][1]; }
 }
 
-__device__ __forceinline__ void write_stats(const Params& p, long long group, double s, double q, double& mean, double& rstd) {
+__device__ __forceinline__ void stats_of(const Params& p, double s, double q, double& mean, double& rstd) {
   const double cnt = (double)(p.E / p.C) * p.D;
   mean = s / cnt;
   double var = q / cnt - mean * mean;
   if (var < 0.0) var = 0.0;                                        // (a NaN stays one)
   rstd = 1.0 / sqrt(var + (double)p.eps);
+}
+__device__ __forceinline__ void write_stats(const Params& p, long long group, double s, double q, double& mean, double& rstd) {
+  stats_of(p, s, q, mean, rstd);
   p.stats[group * 2] = mean;
   p.stats[group * 2 + 1] = rstd;
 }
@@ -302,16 +310,57 @@ __device__ __forceinline__ void write_codes(const Params& p, int n, int row, int
   if (q0 % C8_BLOCK == 0) p.exps_out[pix * p.nblk + q0 / C8_BLOCK] = (unsigned char)e;
 }
 
+// Statistics of the groups that the slab's channels [c0, c0 + width) belong to, from the chunks' sums, into st[group][2];
+// returns the first group.  Every workgroup of an image does it over again: a few KB from the L2 against a launch of its own
+// between the two passes (32 x 64 x 64 x 64 float 24.4 -> 21.7 us, 32 x 128 x 128 x 64 72 -> 69).
+constexpr int MERGE_SPAN = 512;
+__device__ __forceinline__ int merged_stats(const Params& p, const Place& w, int c0, int width, double* st) {
+  __shared__ double red[2 * MERGE_SPAN];
+  const int g0 = c0 / p.D, g1 = (min(p.C, c0 + width) - 1) / p.D + 1, span = (g1 - g0) * p.D, parts = max(1, THREADS / span);
+  const double* part = reinterpret_cast<const double*>(p.part) + (long long)w.n * p.chunks * 2 * p.L + g0 * p.D;
+  for (int i = threadIdx.x; i < span * parts; i += THREADS) {
+    const int c = i % span;
+    double s = 0.0, q = 0.0;
+    #pragma unroll 4
+    for (int k = i / span; k < p.chunks; k += parts) { s += part[(long long)k * 2 * p.L + c]; q += part[(long long)k * 2 * p.L + p.L + c]; }
+    red[2 * i] = s;
+    red[2 * i + 1] = q;
+  }
+  __syncthreads();
+  // lanes per group: as many of 1, 4, 16, 64 as its sums keep busy
+  const int items = p.D * parts, lanes = items <= 16 ? 1 : items <= 64 ? 4 : items <= 256 ? 16 : 64;
+  for (int g = threadIdx.x / lanes; g < g1 - g0; g += THREADS / lanes) {
+    double s = 0.0, q = 0.0;
+    for (int i = threadIdx.x % lanes; i < items; i += lanes) {
+      const int at = i / p.D * span + g * p.D + i % p.D;
+      s += red[2 * at];
+      q += red[2 * at + 1];
+    }
+    for (int o = 1; o < lanes; o <<= 1) { s += __shfl_xor(s, o); q += __shfl_xor(q, o); }
+    if (threadIdx.x % lanes == 0) stats_of(p, s, q, st[2 * g], st[2 * g + 1]);
+  }
+  __syncthreads();
+  if (w.row0 == 0)
+    for (int i = threadIdx.x; i < 2 * (g1 - g0); i += THREADS) p.stats[((long long)w.n * p.G + g0) * 2 + i] = st[i];
+  return g0;
+}
+
 template <typename TX, typename TY, bool PACK>
 __global__ __launch_bounds__(THREADS) void fwd_apply_kernel(const Params p) {
   constexpr int NV = VecOf<TX>::n, U = 4;
   const Place w = place_of(p, NV, blockIdx.x);
+  __shared__ double st[2 * MERGE_SPAN];
+  int first = 0;
+  if (p.merged) first = merged_stats(p, w, w.q0 - (int)(threadIdx.x % p.TV) * NV, p.TV * NV, st);
   if (!w.on) return;
   const Source<TX, NV, true> src(p, w.n, w.q0);
   TY* y = reinterpret_cast<TY*>(p.out) + (long long)w.n * p.E + w.q0;
   Affine f[NV];
   #pragma unroll
-  for (int j = 0; j < NV; ++j) f[j] = affine_at(p, w.n, w.q0 + j);
+  for (int j = 0; j < NV; ++j) {
+    const int c = w.q0 + j, g = c / p.D - first;
+    f[j] = p.merged ? affine_of(p, c, st[2 * g], st[2 * g + 1]) : affine_at(p, w.n, c);
+  }
   each_row<U>(p, w, NV,
     [&](int r) {
       RawVec<TX, NV> raw[U];
@@ -400,17 +449,24 @@ __global__ __launch_bounds__(THREADS) void bwd_partial_kernel(const Params p) {
       #pragma unroll
       for (int j = 0; j < NV; ++j) { s[j] += g[j]; q[j] = fmaf(g[j], v[j], q[j]); }
     };
-    each_row<U>(p, w, NV,
-      [&](int r) {
-        typename X::Raw rx[U];
-        RawVec<TY, NV> rg[U];
-        #pragma unroll
-        for (int k = 0; k < U; ++k) { rx[k] = src.load(p, r + k * p.TP); rg[k] = load_raw<TY, NV>(dy + (long long)(r + k * p.TP) * p.L); }
-        #pragma unroll
-        for (int k = 0; k < U; ++k) add(rx[k], rg[k]);
-      },
-      // (behind the image dy reads as 0, and 0 times a finite x - m adds nothing)
-      [&](int r, int have) { add(src.load_tail(p, r, have), load_some<TY, NV>(dy + (long long)r * p.L, have)); });
+    auto rows = [&](auto bypass) {
+      each_row<U>(p, w, NV,
+        [&](int r) {
+          typename X::Raw rx[U];
+          RawVec<TY, NV> rg[U];
+          #pragma unroll
+          for (int k = 0; k < U; ++k) {
+            const TY* at = dy + (long long)(r + k * p.TP) * p.L;
+            rx[k] = src.load(p, r + k * p.TP);
+            if constexpr (bypass.value) load_bytes_nt<sizeof(rg[k])>(&rg[k], at); else rg[k] = load_raw<TY, NV>(at);
+          }
+          #pragma unroll
+          for (int k = 0; k < U; ++k) add(rx[k], rg[k]);
+        },
+        // (behind the image dy reads as 0, and 0 times a finite x - m adds nothing)
+        [&](int r, int have) { add(src.load_tail(p, r, have), load_some<TY, NV>(dy + (long long)r * p.L, have)); });
+    };
+    if (p.bypass) rows(Flag<true>()); else rows(Flag<false>());
   }
   float* out = reinterpret_cast<float*>(p.part) + ((long long)w.n * p.chunks + w.row0 / p.rows_per_chunk) * 2 * p.L;
   const int base = w.q0 - (int)(threadIdx.x % p.TV) * NV;
@@ -540,7 +596,7 @@ __global__ __launch_bounds__(THREADS) void bwd_apply_kernel(const Params p, long
       typename X::Raw rx[U];
       RawVec<TY, NV> rg[U];
       #pragma unroll
-      for (int u = 0; u < U; ++u) { rx[u] = src.load(p, r + u * p.TP); rg[u] = load_raw<TY, NV>(dy + (long long)(r + u * p.TP) * p.L); }
+      for (int u = 0; u < U; ++u) { rx[u] = src.load(p, r + u * p.TP); load_bytes_nt<sizeof(rg[u])>(&rg[u], dy + (long long)(r + u * p.TP) * p.L); }
       #pragma unroll
       for (int u = 0; u < U; ++u) {
         float v[NV];
@@ -577,10 +633,11 @@ __device__ __forceinline__ int piece_length(const Params& p, const Slab& w, int 
   return left >= NV ? NV : left > 0 ? (int)left : 0;
 }
 
-// sums of NV values per thread over the pixel lanes, into sums[0 .. S) (double); buf: blockDim * NV values of V
+// sums of NV values per thread over the pixel lanes, into sums[0 .. S); a thread's values are those of position
+// threadIdx % (S / NV) * NV on.  buf: blockDim * NV values of V
 template <typename V, int NV>
-__device__ __forceinline__ void slab_sums(const V (&s)[NV], V* buf, double* sums, const Slab& w, int S) {
-  if (w.pl < w.TP) {
+__device__ __forceinline__ void pixel_sums(const V (&s)[NV], V* buf, double* sums, int pl, int TP, int S) {
+  if (pl < TP) {
     #pragma unroll
     for (int j = 0; j < NV; ++j) buf[threadIdx.x * NV + j] = s[j];
   }
@@ -589,7 +646,7 @@ __device__ __forceinline__ void slab_sums(const V (&s)[NV], V* buf, double* sums
   if (S >= B) {
     for (int i = threadIdx.x; i < S; i += B) {
       double a = 0.0;
-      for (int t = 0; t < w.TP; ++t) a += buf[t * S + i];
+      for (int t = 0; t < TP; ++t) a += buf[t * S + i];
       sums[i] = a;
     }
     __syncthreads();
@@ -598,7 +655,7 @@ __device__ __forceinline__ void slab_sums(const V (&s)[NV], V* buf, double* sums
   // more threads than positions: `parts` threads per position, then one
   const int parts = B / S, i = threadIdx.x % S, part = threadIdx.x / S;
   double a = 0.0;
-  if (part < parts) for (int t = part; t < w.TP; t += parts) a += buf[t * S + i];
+  if (part < parts) for (int t = part; t < TP; t += parts) a += buf[t * S + i];
   __syncthreads();
   double* mid = reinterpret_cast<double*>(buf);              // (B doubles; buf holds at least that: NV * sizeof(V) >= 8)
   if (part < parts) mid[part * S + i] = a;
@@ -665,8 +722,8 @@ __global__ __launch_bounds__(B) void fwd_slab_kernel(const Params p) {
     for (int j = 0; j < NV; ++j) { const double d = v[j]; s[j] += d; q[j] = fma(d, d, q[j]); }
     forget(raw[k]);
   }
-  slab_sums<double, NV>(s, buf, s0, w, p.S);
-  slab_sums<double, NV>(q, buf, s1, w, p.S);
+  pixel_sums<double, NV>(s, buf, s0, w.pl, w.TP, p.S);
+  pixel_sums<double, NV>(q, buf, s1, w.pl, w.TP, p.S);
   // (a group's results take the place of its first position, which only its own wave has read)
   const int first = p.L > p.C ? 0 : w.base / p.D;
   slab_groups(p, w, s0, s1, [&](int g, double a, double b) {
@@ -735,8 +792,8 @@ __global__ __launch_bounds__(B) void bwd_slab_kernel(const Params p) {
     forget(rx[k]);
     forget(rg[k]);
   }
-  slab_sums<float, NV>(s, buf, s0, w, p.S);
-  slab_sums<float, NV>(q, buf, s1, w, p.S);
+  pixel_sums<float, NV>(s, buf, s0, w.pl, w.TP, p.S);
+  pixel_sums<float, NV>(q, buf, s1, w.pl, w.TP, p.S);
   // positions -> channels (dz, dz xh) for the parameters; then weighted, for the groups
   const int reps = p.L / p.C, span = min(p.S, p.L - w.base);
   for (int i = threadIdx.x; i < (reps > 1 ? p.C : span); i += B) {
@@ -971,9 +1028,11 @@ void launch_forward(const Params& p0, hipStream_t stream) {
   }
   const unsigned blocks = (unsigned)((long long)p.N * p.chunks * p.slabs);
   SG2IM_LAUNCH(fwd_partial_kernel<TX>, dim3(blocks), dim3(THREADS), 0, stream, p);
+  // (a slab's groups reach over it by less than a group on either side)
+  p.merged = p.L == p.C && p.chunks <= 64 && p.TV * VecOf<TX>::n + 2 * (p.D - 1) <= MERGE_SPAN && (p.TV * VecOf<TX>::n + 2 * p.D) * p.chunks <= 16384;
   const long long per = (long long)p.chunks * (p.L / p.C) * p.D;
   const int threads = per <= 256 ? 64 : per <= 4096 ? 256 : 1024;
-  SG2IM_LAUNCH(fwd_finish_kernel, dim3((unsigned)((long long)p.N * p.G)), dim3(threads), 0, stream, p);
+  if (!p.merged) SG2IM_LAUNCH(fwd_finish_kernel, dim3((unsigned)((long long)p.N * p.G)), dim3(threads), 0, stream, p);
   if (p.codes_out) SG2IM_LAUNCH((fwd_apply_kernel<TX, TY, true>), dim3(blocks), dim3(THREADS), 0, stream, p);
   else SG2IM_LAUNCH((fwd_apply_kernel<TX, TY, false>), dim3(blocks), dim3(THREADS), 0, stream, p);
 }
@@ -993,6 +1052,9 @@ void launch_backward(const Params& p0, bool need_dx, bool need_params, hipStream
     return;
   }
   const long long blocks = (long long)p.N * p.chunks * p.slabs;
+  // Where x and dy together are far beyond the 256 MB cache, one of them can stay in it between the two passes if the other
+  // goes past: 32 x 256 x 256 x 64 bfloat16 263 -> 217 us.  Where most of both stays anyway that costs (268 MB: 111 -> 114).
+  p.bypass = (double)p.N * p.E * (sizeof(SRC) + sizeof(TY)) > 384e6;
   SG2IM_LAUNCH((bwd_partial_kernel<SRC, TX, TY, EVEN>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
   const int gpb = p.D >= FIN_CH ? 1 : FIN_CH / p.D;
   SG2IM_LAUNCH(bwd_finish_kernel, dim3((unsigned)((long long)p.N * ((p.G + gpb - 1) / gpb))), dim3(FIN_CH * FIN_LANES), 0,
