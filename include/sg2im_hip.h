@@ -671,7 +671,8 @@ int sg2im_adam_apply_guarded(float* param, const float* grad, float* exp_avg, fl
  *   backward: from x, or - codes / exps given - from its 8-bit form; dy has out's type, dx has x_dtype.  dx, dgamma, dbeta may
  *             be NULL.  accumulate: dgamma / dbeta += .  The side of the LeakyReLU is decided in 64 bits where the
  *             32-bit value is within its rounding of zero; at exactly zero the gradient takes `slope`.
- * workspace: sg2im_groupnorm_workspace bytes, used by this call only.  No alignment beyond an element's is assumed.
+ * workspace: sg2im_groupnorm_workspace bytes, 16-byte aligned, used by this call only.  No alignment beyond an element's is
+ * assumed of the tensors.  Statistics are summed in 64 bits, in a fixed order: the same call gives the same bits.
  * SG2IM_ERR_ARG: channels % groups, hw < 1, a NULL that is needed, a workspace that is too small. */
 size_t sg2im_groupnorm_workspace(int batch, long long hw, int channels, int groups, int x_dtype, int backward);
 int sg2im_groupnorm_act_forward(const void* x, int x_dtype, int batch, long long hw, int channels, int groups,
@@ -706,7 +707,8 @@ int sg2im_unpack8(const signed char* codes, const unsigned char* exps, long long
  *                     (+)= column sums of dz.  signs given to either: `dz` is dy, and dz = dy * (sign ? 1 : slope), rounded to
  *                     `dtype`, is formed on its way into the product (the same numbers as backward_act's).
  * workspace: sg2im_linear_workspace bytes for `which` = 0 forward, 1 backward_data, 2 backward_weight, 3 backward_act.
- * Rows below 2^31 - 256; k, n and the operands' leading dimensions (in elements) at most 2^22; no alignment beyond an element's is assumed. */
+ * Rows below 2^31 - 256; k, n and the operands' leading dimensions (in elements) at most 2^22; no alignment
+ * beyond an element's is assumed (workspace: 16 bytes).  Fixed summation orders: the same call gives the same bits. */
 /* 1: backward_act first and plain products are the faster way for these sizes, 0: the products' own signs / dbias */
 int sg2im_linear_backward_act_first(long long rows, int k, int n, int dtype, int gated, int bias, int need_dx, int need_dw);
 size_t sg2im_linear_workspace(long long rows, int k, int n, int dtype, int which);

@@ -961,7 +961,8 @@ bool cut(Params& p, int N, long long hw, int C, int G, int x_bf16) {
   rpc = std::min(rpc, std::max(1LL, rows));
   p.rows_per_chunk = (int)rpc;
   p.chunks = (int)((rows + rpc - 1) / rpc);
-  return (long long)N * p.chunks * p.slabs + (C + 31) / 32 <= 0x7fffffffLL && (long long)N * G <= 0x7fffffffLL;
+  // (a launch has fewer than 2^32 threads)
+  return ((long long)N * p.chunks * p.slabs + (C + 31) / 32) * THREADS <= 0xffffffffLL && (long long)N * G * 1024 <= 0xffffffffLL;
 }
 
 // The slab kernels' cut: the fewest positions that hold whole groups, whole pieces (`unit`) and 32 channels, more of them where
@@ -980,7 +981,8 @@ bool slab_plan(const Params& p, int nv, int most, SlabPlan& q) {
   static const int forms[4][2] = {{256, 1}, {256, 4}, {512, 8}, {1024, 4}};      // (as many pieces in registers as spill nothing)
   for (int k = 0; k < 4; ++k) {
     const int tp = forms[k][0] / (S / nv);
-    if (k < 2 || k == most) if (tp > 0 && (long long)tp * forms[k][1] >= p.rows) { q.threads = forms[k][0]; q.iter = forms[k][1]; return true; }
+    if (k >= 2 && k != most) continue;
+    if (tp > 0 && (long long)tp * forms[k][1] >= p.rows && (long long)p.N * q.slabs * forms[k][0] <= 0xffffffffLL) { q.threads = forms[k][0]; q.iter = forms[k][1]; return true; }
   }
   return false;
 }

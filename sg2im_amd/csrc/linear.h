@@ -720,7 +720,7 @@ int run(Product& p, const Plan& q, void* workspace, size_t workspace_bytes, hipS
   p.tiles_i = (p.I + q.tile - 1) / q.tile;
   p.tiles_j = (p.J + q.tile - 1) / q.tile;
   const long long blocks = (long long)p.tiles_j * p.tiles_i * q.splits;
-  if (blocks > 0x7fffffffLL) return SG2IM_ERR_ARG;
+  if (blocks * (q.tile == 256 ? 512 : 256) > 0xffffffffLL) return SG2IM_ERR_ARG;      // (a launch has fewer than 2^32 threads)
   const dim3 grid((unsigned)blocks);
   if constexpr (!GATE && !SUM) if (q.tile == 256) SG2IM_LAUNCH((product_kernel<T, 256, 256, 512, AMODE, BMODE, GATE, SUM, false>), grid, dim3(512), 0, stream, p);
   if (q.tile == 128) SG2IM_LAUNCH((product_kernel<T, 128, 128, 256, AMODE, BMODE, GATE, SUM, true>), grid, dim3(256), 0, stream, p);

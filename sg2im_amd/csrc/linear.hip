@@ -179,7 +179,7 @@ int sg2im_linear_backward_act(const void* dy, int dy_dtype, long long ld_dy, con
   p.part = dbias ? reinterpret_cast<float*>(workspace) : nullptr;
   p.db = dbias; p.db_bf16 = bias_dtype; p.accumulate = accumulate;
   const long long blocks = (long long)p.chunks * p.slabs;
-  if (blocks > 0x7fffffffLL) return SG2IM_ERR_ARG;
+  if (blocks * THREADS > 0xffffffffLL) return SG2IM_ERR_ARG;
   if (rows > 0 && (dz || dbias)) {
     const dim3 grid((unsigned)blocks);
     if (dy_dtype == 0 && dz_dtype == 0) SG2IM_LAUNCH((act_backward_kernel<float, float>), grid, dim3(THREADS), 0, stream, p);

@@ -1,7 +1,8 @@
 // The host side of group norm + activation, linear + activation + residual and the 8-bit activation checkpoints: argument
 // checks, outputs, work buffers and the autograd nodes around the C ABI of libsg2im_hip.so.  These calls are short - a few
 // microseconds on the GPU for a graph's objects - and from Python their checks, allocations and the backward pass' way
-// through the interpreter took 24 us (forward) and 150 - 190 us (forward and backward); from here 9 and 45 - 60.
+// through the interpreter took 24 us (forward) and 150 - 190 us (forward and backward); from here 6 and 65 - 75, of which
+// torch.autograd.grad itself is some 35.
 //
 // Work buffers come from torch's allocator per call (inside a capture: from the graph's own pool), so neither two streams
 // nor two captured graphs share one.  The library's entry points are bound by address (bind), so that this module uses
@@ -172,7 +173,7 @@ GnResult gn_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, i
   TORCH_CHECK_VALUE(x.is_contiguous(), "group norm: the input must be dense");
   if (out_type < 0) out_type = code(x);
   TORCH_CHECK_TYPE(out_type == 1 || !is_bf16(x), "group norm: a float32 output of a bfloat16 input");
-  TORCH_CHECK_VALUE(eps >= 0, "group norm: eps = ", eps);
+  TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(slope), "group norm: eps = ", eps, ", slope = ", slope);
   const int pc = params(weight, bias, s.c, "group norm parameters");
   const size_t bytes = api.groupnorm_workspace(s.n, s.hw, s.c, s.g, code(x), 0);
   TORCH_CHECK_VALUE(bytes, "group norm: ", x.sizes(), " is too large");
@@ -295,6 +296,7 @@ std::tuple<Tensor, Tensor> lin_forward(const Tensor& x, const Tensor& weight, co
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == K, "linear: input ", x.sizes(), " and weight ", weight.sizes());
   if (out_type < 0) out_type = code(x);
   TORCH_CHECK_TYPE(out_type == 0 || is_bf16(x), "linear: a bfloat16 output of float32 operands");
+  TORCH_CHECK_VALUE(std::isfinite(slope), "linear: slope = ", slope);
   const int bc = params(Tensor(), bias, N, "linear bias");
   const Rows r = rows_of(x, "linear input");
   auto shape = x.sizes().vec();

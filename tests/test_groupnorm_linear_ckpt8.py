@@ -478,6 +478,64 @@ def test_gradients_go_into_registered_sinks():
     flat.close()
 
 
+# ---- more than 2^31 values --------------------------------------------------------------------------------------------
+
+@gpu
+def test_group_norm_and_pack_past_32_bit_offsets():
+  """the same image over and over: every image is computed alike, whatever its offset"""
+  from sg2im_amd import ops
+  r = gen(40)
+  one = r(1, 1024, 1024, 64).to(BF16)
+  n = 33                                                   # 33 * 2^26 values = 2.2e9
+  x = one.expand(n, -1, -1, -1).contiguous()
+  w, b = (1 + 0.1 * r(64)).to(BF16), (0.1 * r(64)).to(BF16)
+  y, st, p = ops.group_norm_act_forward(x, w, b, 8, 0.2, 1e-5, pack=True)
+  assert torch.equal(y[n - 1], y[0]) and torch.equal(st[n - 1], st[0])
+  assert torch.equal(p.codes[n - 1], p.codes[0]) and torch.equal(p.exps[n - 1], p.exps[0])
+  assert torch.equal(ops.unpack8(p)[n - 1], eight(one[0])[0].to(BF16))
+  q = ops.pack8(x)
+  assert torch.equal(q.codes[n - 1], p.codes[0]) and torch.equal(q.exps[n - 1], p.exps[0])
+  dy = r(1, 1024, 1024, 64).to(BF16).expand(n, -1, -1, -1).contiguous()
+  for src in (x, p):
+    dx = ops.group_norm_act_backward(dy, src, w, b, 8, 0.2, st)
+    assert torch.equal(dx[n - 1], dx[0]) and bool(dx[n - 1].isfinite().all())
+    del dx
+
+
+@gpu
+def test_linear_past_32_bit_offsets():
+  """rows repeated with a period: every row is computed alike, whatever its offset"""
+  from sg2im_amd import ops
+  r = gen(41)
+  period = 4096
+  rows = r(period, 64).to(BF16)
+  times = 8448                                             # 8448 * 4096 * 64 = 2.2e9 values
+  x = rows.repeat(times, 1)
+  w, b = (r(64, 64) / 8).to(BF16), r(64).to(BF16)
+  y, signs = ops.linear_forward(x, w, b, x, 0.2, signs=True)
+  z, s0 = ops.linear_forward(rows, w, b, rows, 0.2, signs=True)
+  assert torch.equal(y[-period:], z) and torch.equal(signs[-period:], s0)
+  for gate in (None, signs):
+    dx = ops.linear_backward_data(y, w, gate, 0.2)
+    assert torch.equal(dx[-period:], dx[:period])
+  # the last rows' part of dW and db, added to those of everything before them
+  cut = x.size(0) - period
+  dw, db = torch.empty(64, 64, device='cuda'), torch.empty(64, device='cuda')
+  ops.linear_backward_weight(y, ops.pack8(x), dw, dbias=db, signs=signs, slope=0.2)
+  d2, b2 = torch.empty_like(dw), torch.empty_like(db)
+  ops.linear_backward_weight(y[:cut], ops.pack8(x[:cut]), d2, dbias=b2, signs=signs[:cut], slope=0.2)
+  ops.linear_backward_weight(y[cut:], ops.pack8(x[cut:]), d2, accumulate=True, dbias=b2, bias_accumulate=True, signs=signs[cut:], slope=0.2)
+  one = torch.where(sides(s0, 64), z.to(F64), (z.to(F64) * 0.2).to(BF16).to(F64))
+  want = times * (one.t() @ eight(rows)[0])
+  mag = times * (one.abs().t() @ eight(rows)[0].abs())
+  # (a chunk of 64 rows at a time in float32 along a split of at most rows / 64: r / 64 + 64 additions)
+  tol = (x.size(0) / 64 + 64 + 256) * u32 * mag
+  check(dw, want, tol, 'dweight')
+  check(d2, want, tol, 'dweight in two parts')
+  unrounded = torch.where(sides(s0, 64), z.to(F64), z.to(F64) * 0.2)
+  check(db, times * unrounded.sum(0), (x.size(0) / 64 + 256) * u32 * times * unrounded.abs().sum(0), 'dbias')
+
+
 # ---- what is refused ------------------------------------------------------------------------------------------------
 
 def test_entry_points_refuse_without_a_gpu():
@@ -543,6 +601,8 @@ def test_wrappers_refuse():
     lambda: HF.GroupNormAct.apply(x.bfloat16(), None, None, 2, 0.2, 1e-5, False, F32),
     lambda: HF.GroupNormAct.apply(x, None, None, 2, 0.2, -1.0),
     lambda: HF.GroupNormAct.apply(x[0], None, None, 2),
+    lambda: HF.GroupNormAct.apply(x, None, None, 2, math.inf),
+    lambda: HF.LinearResidual.apply(x, w, None, None, math.nan),
     lambda: HF.GroupNormAct.apply(torch.empty(2, 0, 3, 8, device=d), None, None, 2),
     lambda: HF.LinearResidual.apply(x, w[:, :7], None, None),
     lambda: HF.LinearResidual.apply(x, w.bfloat16(), None, None),
