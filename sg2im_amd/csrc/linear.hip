@@ -13,6 +13,90 @@
 namespace sg2im {
 namespace lin {
 
+// ---- small forward products ------------------------------------------------------------------------------------------
+// Few tiles and a long reduction is a chain of waits: a workgroup takes 16 x 16 outputs and its NW waves split the reduction;
+// operands go from memory straight into the matrix instructions' registers (r contiguous: a lane's 16 bytes are its operand
+// of v_mfma_f32_16x16x32_bf16, or of four v_mfma_f32_16x16x4_f32), U pieces of each in flight, and the waves' sums meet in
+// LDS.  One launch instead of a split product and its join.  (32 x 32 outputs per workgroup were slower: a CU is then
+// busy with the products themselves, and few CUs are used.)
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 multiply16(const bf16x8& a, const bf16x8& b, const f32x4& c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 multiply16(const float4& a, const float4& b, f32x4 c) {
+  c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x, b.x, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.y, b.y, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.z, b.z, c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a.w, b.w, c, 0, 0, 0);
+}
+
+template <typename T, int NW>
+__global__ __launch_bounds__(NW * 64) void short_kernel(const Product p) {
+  constexpr int NV = Geo<T>::NV, RS = 4 * NV, U = 4, LD = 20;
+  __shared__ __attribute__((aligned(16))) float red[NW * 16 * LD];
+  const int tiles_j = (p.J + 15) / 16, i0 = (int)(blockIdx.x / tiles_j) * 16, j0 = (int)(blockIdx.x % tiles_j) * 16;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = (lane >> 4) * NV;
+  const T* a = reinterpret_cast<const T*>(p.a) + (long long)min(i0 + (lane & 15), p.I - 1) * p.lda + h;
+  const T* b = reinterpret_cast<const T*>(p.b) + (long long)min(j0 + (lane & 15), p.J - 1) * p.ldb + h;
+  const int steps = (p.R + RS - 1) / RS, per = (steps + NW - 1) / NW, s1 = min(steps, (wave + 1) * per), full = min(s1, p.R / RS);
+  typedef decltype(operand<32, RC>((const T*)nullptr, 0, 0, 0)) Op;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  int s = wave * per;
+  for (; s + U <= full; s += U) {
+    Op oa[U], ob[U];
+    #pragma unroll
+    for (int k = 0; k < U; ++k) {
+      __builtin_memcpy(&oa[k], a + (long long)(s + k) * RS, 16);
+      __builtin_memcpy(&ob[k], b + (long long)(s + k) * RS, 16);
+    }
+    #pragma unroll
+    for (int k = 0; k < U; ++k) acc = multiply16(ob[k], oa[k], acc);
+  }
+  for (; s < s1; ++s) {
+    // (a piece over the end: from where it fits, moved into place, as in Feeder)
+    const int over = max(0, s * RS + h + NV - p.R);
+    uint4 wa, wb;
+    __builtin_memcpy(&wa, a + (long long)s * RS - over, 16);
+    __builtin_memcpy(&wb, b + (long long)s * RS - over, 16);
+    wa = moved(wa, over * (int)sizeof(T) * 8);
+    wb = moved(wb, over * (int)sizeof(T) * 8);
+    acc = multiply16(__builtin_bit_cast(Op, wb), __builtin_bit_cast(Op, wa), acc);
+  }
+  *reinterpret_cast<float4*>(red + (wave * 16 + (lane & 15)) * LD + 4 * (lane >> 4)) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  __syncthreads();
+  if (wave) return;
+  const int row = lane >> 2, col = (lane & 3) * 4, i = i0 + row, j = j0 + col;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  #pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const float4 u = *reinterpret_cast<const float4*>(red + (w * 16 + row) * LD + col);
+    v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w;
+  }
+  unsigned bits = 0;
+  if (i < p.I && j + 4 <= p.J) bits = finish<4>(p, i, j, v);
+  else if (i < p.I) {
+    if (j < p.J) bits = finish_one(p, i, j, v[0]);
+    if (j + 1 < p.J) bits |= finish_one(p, i, j + 1, v[1]) << 1;
+    if (j + 2 < p.J) bits |= finish_one(p, i, j + 2, v[2]) << 2;
+  }
+  if (p.signs) {                                     // (half a word; the upper half of a row's last one may have no columns)
+    bits <<= col;
+    bits |= __shfl_xor(bits, 1);
+    bits |= __shfl_xor(bits, 2);
+    unsigned short* half = reinterpret_cast<unsigned short*>(p.signs) + (long long)i * p.sign_words * 2 + j0 / 16;
+    if (col == 0 && i < p.I) {
+      half[0] = (unsigned short)bits;
+      if (j0 + 16 >= p.J && (j0 / 16 & 1) == 0) half[1] = 0;
+    }
+  }
+}
+
+template <typename T>
+static int run_short(const Product& p, hipStream_t stream) {
+  const dim3 grid((unsigned)(((long long)p.I + 15) / 16 * ((p.J + 15) / 16)));
+  if (p.R <= 16 * 4 * Geo<T>::NV) SG2IM_LAUNCH((short_kernel<T, 4>), grid, dim3(256), 0, stream, p);
+  else SG2IM_LAUNCH((short_kernel<T, 8>), grid, dim3(512), 0, stream, p);
+  return status();
+}
+
 // ---- dz and the bias gradient -------------------------------------------------------------------------------------
 
 struct ActParams {
@@ -107,6 +191,16 @@ constexpr int LD_MAX = 1 << 22;      // (a tile's 256 rows stay within 32-bit by
 bool ld_ok(long long ld, int cols) { return ld >= cols && ld <= LD_MAX; }
 bool sizes_ok(long long rows, int k, int n) { return rows >= 0 && rows <= 0x7fffffffLL - 256 && k >= 1 && n >= 1 && k <= LD_MAX && n <= LD_MAX; }
 
+// The whole reduction in one workgroup's waves, where that is estimated faster than the tiles (whose estimate leaves the
+// launch out).  Fitted to 24 shapes; microseconds, tiles / short, rows x n x k:
+//   float     342 x 384 x 512 11.8 / 8.5, 1 x 4096 x 4096 27.7 / 14.0, 1000 x 300 x 300 12.6 / 9.6; 342 x 512 x 1152 14.4 / 16.6
+//   bfloat16  29 x 23 x 1823 7.0 / 5.0, 1 x 4096 x 4096 11.5 / 8.8, 64 x 2048 x 512 9.2 / 7.6; 512 x 1024 x 1024 9.2 / 18.8
+bool short_form(long long I, long long J, long long R, int bf16, const Plan& q) {
+  const double tiles = (double)((I + 15) / 16) * (double)((J + 15) / 16), chunks = (double)R / (bf16 ? 64 : 32);
+  const double us = 4.5 + tiles / 256 * (0.3 + chunks * (bf16 ? 0.12 : 0.11));
+  return R >= (bf16 ? 8 : 4) && us < q.us + (bf16 ? 3.0 : 3.5) && tiles < 65536;   // (a lane's 16 bytes have to fit in a row)
+}
+
 ActParams act_plan(long long rows, int n) {
   ActParams p = {};
   p.M = rows; p.N = n;
@@ -164,6 +258,7 @@ int sg2im_linear_forward(const void* x, int dtype, long long ld_x, const void* w
   p.bias = bias; p.bias_bf16 = bias_dtype; p.residual = residual; p.ld_res = ld_res; p.slope = slope;
   p.signs = signs; p.sign_words = (n + 31) / 32; p.out = out; p.out_bf16 = out_dtype; p.ld_out = ld_out;
   const Plan q = plan(0, rows, n, k, dtype);
+  if (short_form(rows, n, k, dtype, q)) return dtype == 0 ? run_short<float>(p, stream) : run_short<bf16_s>(p, stream);
   return dtype == 0 ? run<float, RC, RC, false, false>(p, q, workspace, workspace_bytes, stream)
                     : run<bf16_s, RC, RC, false, false>(p, q, workspace, workspace_bytes, stream);
 }

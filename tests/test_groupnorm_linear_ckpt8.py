@@ -317,6 +317,26 @@ def test_linear_forward_and_backward(size, types):
 
 
 @gpu
+@pytest.mark.parametrize('ty', [F32, BF16])
+@pytest.mark.parametrize('K', [3, 4, 8, 9, 31, 33, 100, 257, 516, 1100])
+def test_small_forward_products(K, ty):
+  """few outputs, every remainder of a row's end, strided rows; signs of rows' half words"""
+  from sg2im_amd import ops
+  for M, N in ((1, 1), (7, 18), (16, 16), (17, 35), (33, 61), (50, 96)):
+    r = gen(100 * K + M + N)
+    x, w = r(M, K + 5).to(ty)[:, 3:3 + K], (r(N, K) / math.sqrt(K)).to(ty)
+    b, res = r(N).to(ty), r(M, N).to(ty)
+    y, signs = ops.linear_forward(x, w, b, res, 0.2, ty, signs=True)
+    f = lin_bounds(x, x, w, b, res, 0.2, res, sides(signs, N), ty, ty)
+    check(y, f['y'], f['y_tol'] + half_step(ty) * f['y'].abs(), 'y')
+    wrong = sides(signs, N) != (f['z'] > 0)
+    assert not bool((wrong & (f['z'].abs() > f['z_tol'])).any()), 'sides'
+    assert signs.shape == (M, (N + 31) // 32)
+    if N % 32:
+      assert not bool((signs[:, -1].long() & 0xffffffff >> N % 32 << N % 32).any()), 'bits past the last column'
+
+
+@gpu
 def test_linear_gradient_against_differences():
   """the loss is linear in each of x, W, b and the residual away from the kink: a difference of the definition is exact"""
   from sg2im_amd import functional as HF
