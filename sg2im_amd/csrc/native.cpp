@@ -173,7 +173,7 @@ GnResult gn_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, i
   TORCH_CHECK_VALUE(x.is_contiguous(), "group norm: the input must be dense");
   if (out_type < 0) out_type = code(x);
   TORCH_CHECK_TYPE(out_type == 1 || !is_bf16(x), "group norm: a float32 output of a bfloat16 input");
-  TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(slope), "group norm: eps = ", eps, ", slope = ", slope);
+  TORCH_CHECK_VALUE(eps >= 0 && std::isfinite((float)slope), "group norm: eps = ", eps, ", slope = ", slope);
   const int pc = params(weight, bias, s.c, "group norm parameters");
   const size_t bytes = api.groupnorm_workspace(s.n, s.hw, s.c, s.g, code(x), 0);
   TORCH_CHECK_VALUE(bytes, "group norm: ", x.sizes(), " is too large");
@@ -199,7 +199,8 @@ Tensor gn_backward(const Tensor& dy, const Tensor& x, const Packed& packed, int 
   TORCH_CHECK_TYPE(x_type == 0 || is_bf16(dy), "group norm backward: a float32 gradient of a bfloat16 input");
   const GnShape s = gn_shape(dy, groups);
   const int pc = params(weight, bias, s.c, "group norm parameters"), gc = params(dweight, dbias, s.c, "group norm gradients");
-  TORCH_CHECK_VALUE(stats.is_cuda() && stats.scalar_type() == at::kDouble && stats.is_contiguous() && stats.numel() == (int64_t)s.n * s.g * 2,
+  TORCH_CHECK_VALUE(stats.is_cuda() && stats.scalar_type() == at::kDouble && stats.is_contiguous() && stats.device() == dy.device() &&
+                    stats.numel() == (int64_t)s.n * s.g * 2,
                     "group norm backward: not the statistics of this input");
   const size_t bytes = api.groupnorm_workspace(s.n, s.hw, s.c, s.g, x_type, 1);
   Tensor dx = need_dx ? at::empty(dy.sizes(), dy.options().dtype(type_of(x_type)).memory_format(c10::nullopt)) : Tensor();
@@ -272,12 +273,30 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
 
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// A leaf's gradient is handed over on the stream on which its accumulation node was made, and that node lives as long as any
+// graph of the leaf does.  Made on the default stream, which cannot take part in a capture, it would end the process in the
+// captured backward pass: such a call is refused while it is recorded.  (With a sink nothing is handed over.)
+void check_capture(std::initializer_list<std::pair<const Tensor*, const Tensor*>> leaves) {
+  const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream(), usual = c10::hip::getDefaultHIPStream();
+  hipStreamCaptureStatus status;
+  if (now == usual || hipStreamIsCapturing(now.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  for (const auto& [t, sink] : leaves) {
+    if (!wants(*t) || !t->is_leaf() || (sink && sink->defined())) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : c10::nullopt;
+    TORCH_CHECK(!stream.has_value() || stream->id() != usual.id(),
+                "captured into a graph while a gradient graph of the same leaf, made on the default stream, is alive: release it before the "
+                "capture, or record with a detached copy of the leaf");
+  }
+}
+
 Tensor group_norm_act(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, int64_t groups, double slope, double eps, bool checkpoint8,
                       int64_t out_type, const MaybeTensor& sink_w, const MaybeTensor& sink_b) {
   const Tensor w = given(weight), b = given(bias);
   if (!(at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))))
     return gn_forward(x.contiguous(), w, b, groups, slope, eps, (int)out_type, false).y;
   const Sinks sinks{given(sink_w), given(sink_b)};
+  check_capture({{&x, nullptr}, {&w, &sinks.w}, {&b, &sinks.b}});
   return GroupNormAct::apply(x.contiguous(), maybe(w), maybe(b), groups, slope, eps, checkpoint8, out_type, &sinks);
 }
 
@@ -296,7 +315,7 @@ std::tuple<Tensor, Tensor> lin_forward(const Tensor& x, const Tensor& weight, co
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == K, "linear: input ", x.sizes(), " and weight ", weight.sizes());
   if (out_type < 0) out_type = code(x);
   TORCH_CHECK_TYPE(out_type == 0 || is_bf16(x), "linear: a bfloat16 output of float32 operands");
-  TORCH_CHECK_VALUE(std::isfinite(slope), "linear: slope = ", slope);
+  TORCH_CHECK_VALUE(std::isfinite((float)slope), "linear: slope = ", slope);
   const int bc = params(Tensor(), bias, N, "linear bias");
   const Rows r = rows_of(x, "linear input");
   auto shape = x.sizes().vec();
@@ -320,7 +339,7 @@ std::tuple<Tensor, Tensor> lin_forward(const Tensor& x, const Tensor& weight, co
 
 void check_signs(const Tensor& signs, const Rows& dy) {
   TORCH_CHECK_VALUE(!signs.defined() || (signs.is_cuda() && signs.scalar_type() == at::kInt && signs.is_contiguous() && signs.dim() == 2 &&
-                                         signs.size(0) == dy.rows && signs.size(1) == (dy.cols + 31) / 32), "linear backward: not the signs of this output");
+                                         signs.device() == dy.m.device() && signs.size(0) == dy.rows && signs.size(1) == (dy.cols + 31) / 32), "linear backward: not the signs of this output");
 }
 const unsigned* signs_ptr(const Tensor& t) { return reinterpret_cast<const unsigned*>(ptr(t)); }
 
@@ -444,6 +463,7 @@ Tensor linear_residual(const Tensor& x, const Tensor& weight, const MaybeTensor&
     return std::get<0>(lin_forward(x, w, b, r, slope, (int)out_type, false));
   }
   const Sinks sinks{given(sink_w), given(sink_b)};
+  check_capture({{&x, nullptr}, {&weight, &sinks.w}, {&b, &sinks.b}, {&r, nullptr}});
   return LinearResidual::apply(x, weight, maybe(b), maybe(r), slope, checkpoint8, out_type, &sinks);
 }
 

@@ -469,6 +469,38 @@ def test_the_three_together_on_streams_and_in_graphs(dtype, ckpt):
 
 
 @gpu
+def test_capture_next_to_a_living_graph_of_the_same_leaves_is_refused():
+  """the leaf's accumulation node would be one of the default stream; released, or with a sink, the capture goes through"""
+  from sg2im_amd import functional as HF
+  r = gen(33)
+  x, w, b = r(6, 32).requires_grad_(True), r(32, 32).requires_grad_(True), r(32).requires_grad_(True)
+  dy = r(6, 32)
+  calls = {'group norm': (lambda x, w, b: HF.GroupNormAct.apply(x, b, None, 4, 0.2), (x, b)),
+           'linear': (lambda x, w, b: HF.LinearResidual.apply(x, w, b, x, 0.2), (x, w, b))}
+  for name, (call, leaves) in calls.items():
+    y = call(x, w, b)
+    want = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+      with pytest.raises(RuntimeError, match='same leaf'):
+        call(x, w, b)
+      with torch.no_grad():
+        z = call(x, w, b)                                                # (nothing to hand over)
+    g.replay()
+    assert torch.equal(z, y), name
+    del y
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+      got = torch.autograd.grad(call(x, w, b), leaves, dy)
+    for _ in range(2):
+      for t in got:
+        t.fill_(7.0)
+      g.replay()
+      torch.cuda.synchronize()
+      assert all(torch.equal(p, q) for p, q in zip(got, want)), name
+
+
+@gpu
 def test_gradients_go_into_registered_sinks():
   from sg2im_amd import functional as HF
   from sg2im_amd.optim import FlatParams
@@ -623,6 +655,7 @@ def test_wrappers_refuse():
     lambda: HF.GroupNormAct.apply(x[0], None, None, 2),
     lambda: HF.GroupNormAct.apply(x, None, None, 2, math.inf),
     lambda: HF.LinearResidual.apply(x, w, None, None, math.nan),
+    lambda: HF.LinearResidual.apply(x, w, None, None, 1e300),                      # (infinite in float)
     lambda: HF.GroupNormAct.apply(torch.empty(2, 0, 3, 8, device=d), None, None, 2),
     lambda: HF.LinearResidual.apply(x, w[:, :7], None, None),
     lambda: HF.LinearResidual.apply(x, w.bfloat16(), None, None),
