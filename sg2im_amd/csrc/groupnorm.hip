@@ -722,16 +722,44 @@ __global__ __launch_bounds__(B) void fwd_slab_kernel(const Params p) {
     for (int j = 0; j < NV; ++j) { const double d = v[j]; s[j] += d; q[j] = fma(d, d, q[j]); }
     forget(raw[k]);
   }
-  pixel_sums<double, NV>(s, buf, s0, w.pl, w.TP, p.S);
-  pixel_sums<double, NV>(q, buf, s1, w.pl, w.TP, p.S);
-  // (a group's results take the place of its first position, which only its own wave has read)
   const int first = p.L > p.C ? 0 : w.base / p.D;
-  slab_groups(p, w, s0, s1, [&](int g, double a, double b) {
-    double mean, rstd;
-    write_stats(p, (long long)w.n * p.G + g, a, b, mean, rstd);
-    s0[(g - first) * p.D] = mean;
-    s1[(g - first) * p.D] = rstd;
-  });
+  if (p.L == p.C && p.D % NV == 0) {
+    // a piece lies in one group: a thread has one sum, and a wave joins a group's (32 x 8 x 8 x 512 bfloat16 8.2 us; by
+    // positions first, as below, 10.7)
+    double a = 0.0, b = 0.0;
+    #pragma unroll
+    for (int j = 0; j < NV; ++j) { a += s[j]; b += q[j]; }
+    buf[threadIdx.x] = a;
+    buf[B + threadIdx.x] = b;
+    __syncthreads();
+    const int lane = threadIdx.x & 63, per = p.D / NV, entries = w.TP * per, ng = min(p.S, p.L - w.base) / p.D;
+    for (int g = threadIdx.x >> 6; g < ng; g += B / 64) {
+      a = b = 0.0;
+      for (int i = lane; i < entries; i += 64) {
+        const int t = i / per * w.TV + g * per + i % per;
+        a += buf[t];
+        b += buf[B + t];
+      }
+      #pragma unroll
+      for (int o = 32; o; o >>= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
+      if (lane == 0) {
+        double mean, rstd;
+        write_stats(p, (long long)w.n * p.G + first + g, a, b, mean, rstd);
+        s0[g * p.D] = mean;
+        s1[g * p.D] = rstd;
+      }
+    }
+  } else {
+    pixel_sums<double, NV>(s, buf, s0, w.pl, w.TP, p.S);
+    pixel_sums<double, NV>(q, buf, s1, w.pl, w.TP, p.S);
+    // (a group's results take the place of its first position, which only its own wave has read)
+    slab_groups(p, w, s0, s1, [&](int g, double a, double b) {
+      double mean, rstd;
+      write_stats(p, (long long)w.n * p.G + g, a, b, mean, rstd);
+      s0[(g - first) * p.D] = mean;
+      s1[(g - first) * p.D] = rstd;
+    });
+  }
   __syncthreads();
   if (!w.on) return;
   Affine f[NV];
