@@ -173,21 +173,26 @@ __device__ __forceinline__ void each_row(const Params& p, const Place& w, int NV
 
 // ---- forward ------------------------------------------------------------------------------------------------------
 
-// sums over the pixel lanes of NV values per thread: out(position of the slab, sum); buf: THREADS * NV values.  (One thread
-// per position: spreading a position over idle threads, as the slab kernels do, measured 0.5 - 1 us slower here.)
+// sums over the pixel lanes of two times NV values per thread: out(which, position of the slab, sum); buf: 2 * THREADS * NV
+// values.  (One thread per sum: spreading a sum over idle threads, as the slab kernels do, measured 0.5 - 1 us slower here.)
 template <typename V, int NV, typename F>
-__device__ __forceinline__ void sum_pixel_lanes(const V (&s)[NV], V* buf, int TV, int TP, int pl, F out) {
+__device__ __forceinline__ void sum_pixel_lanes(const V (&s)[NV], const V (&q)[NV], V* buf, int TV, int TP, int pl, F out) {
+  constexpr int HALF = THREADS * NV;
   if (pl < TP) {
     #pragma unroll
-    for (int j = 0; j < NV; ++j) buf[threadIdx.x * NV + j] = s[j];
+    for (int j = 0; j < NV; ++j) {
+      buf[threadIdx.x * NV + j] = s[j];
+      buf[HALF + threadIdx.x * NV + j] = q[j];
+    }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < TV * NV; i += blockDim.x) {
+  const int S = TV * NV;
+  for (int i = threadIdx.x; i < 2 * S; i += THREADS) {
+    const int which = i >= S, at = which * (HALF - S) + i;
     double a = 0.0;
-    for (int t = 0; t < TP; ++t) a += buf[t * TV * NV + i];
-    out(i, a);
+    for (int t = 0; t < TP; ++t) a += buf[t * S + at];
+    out(which, i - which * S, a);
   }
-  __syncthreads();
 }
 
 // sums of x and x^2 of every position over a chunk of rows.  Bound by memory: 32 x 256 x 256 x 64 bfloat16 46 us, 5.8 TB/s (the part
@@ -195,7 +200,7 @@ __device__ __forceinline__ void sum_pixel_lanes(const V (&s)[NV], V* buf, int TV
 template <typename TX>
 __global__ __launch_bounds__(THREADS) void fwd_partial_kernel(const Params p) {
   constexpr int NV = VecOf<TX>::n, U = 4;
-  __shared__ double buf[THREADS * NV];
+  __shared__ double buf[2 * THREADS * NV];
   const Place w = place_of(p, NV, blockIdx.x);
   double s[NV], q[NV];
   #pragma unroll
@@ -220,8 +225,7 @@ __global__ __launch_bounds__(THREADS) void fwd_partial_kernel(const Params p) {
   }
   double* out = reinterpret_cast<double*>(p.part) + ((long long)w.n * p.chunks + w.row0 / p.rows_per_chunk) * 2 * p.L;
   const int base = w.q0 - (int)(threadIdx.x % p.TV) * NV;
-  sum_pixel_lanes<double, NV>(s, buf, p.TV, p.TP, w.pl, [&](int i, double a) { if (base + i < p.L) out[base + i] = a; });
-  sum_pixel_lanes<double, NV>(q, buf, p.TV, p.TP, w.pl, [&](int i, double a) { if (base + i < p.L) out[p.L + base + i] = a; });
+  sum_pixel_lanes<double, NV>(s, q, buf, p.TV, p.TP, w.pl, [&](int k, int i, double a) { if (base + i < p.L) out[k * p.L + base + i] = a; });
 }
 
 __device__ __forceinline__ void block_sum2(double& a, double& b, double (*red)[2]) {
@@ -432,7 +436,7 @@ __device__ __forceinline__ void back_values(const Params& p, int n, int q0, floa
 template <typename SRC, typename TX, typename TY, bool EVEN>
 __global__ __launch_bounds__(THREADS) void bwd_partial_kernel(const Params p) {
   constexpr int NV = VecOf<TX>::n, U = 2;
-  __shared__ float buf[THREADS * NV];
+  __shared__ float buf[2 * THREADS * NV];
   const Place w = place_of(p, NV, blockIdx.x);
   float s[NV], q[NV];
   #pragma unroll
@@ -474,8 +478,7 @@ __global__ __launch_bounds__(THREADS) void bwd_partial_kernel(const Params p) {
   }
   float* out = reinterpret_cast<float*>(p.part) + ((long long)w.n * p.chunks + w.row0 / p.rows_per_chunk) * 2 * p.L;
   const int base = w.q0 - (int)(threadIdx.x % p.TV) * NV;
-  sum_pixel_lanes<float, NV>(s, buf, p.TV, p.TP, w.pl, [&](int i, double a) { if (base + i < p.L) out[base + i] = (float)a; });
-  sum_pixel_lanes<float, NV>(q, buf, p.TV, p.TP, w.pl, [&](int i, double a) { if (base + i < p.L) out[p.L + base + i] = (float)a; });
+  sum_pixel_lanes<float, NV>(s, q, buf, p.TV, p.TP, w.pl, [&](int k, int i, double a) { if (base + i < p.L) out[k * p.L + base + i] = (float)a; });
 }
 
 // a channel's sum of dz xh from those of dz (x - m) and dz:  xh = (x - m) rstd + (m - mean) rstd
