@@ -28,7 +28,24 @@ __device__ __forceinline__ f32x4 multiply16(const float4& a, const float4& b, f3
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a.w, b.w, c, 0, 0, 0);
 }
 
-template <typename T, int NW>
+// 16 bytes at p.  HALF: p may lie in the middle of a word; the five words that hold them are loaded and moved (a 16-byte load at
+// such an address takes several times as long: 16 x 128 x 2001 bfloat16 12.2 us with it, 7.3 so)
+template <bool HALF, typename T> __device__ __forceinline__ uint4 piece_at(const T* p) {
+  uint4 w;
+  if constexpr (!HALF) __builtin_memcpy(&w, p, 16);
+  else {
+    const unsigned long long at = reinterpret_cast<unsigned long long>(p);
+    const unsigned by = (unsigned)at & 2;
+    const unsigned* word = reinterpret_cast<const unsigned*>(at - by);
+    const unsigned w4 = word[by ? 4 : 3];                            // (a word that holds some of the 16 bytes)
+    __builtin_memcpy(&w, word, 16);
+    w = make_uint4(__builtin_amdgcn_alignbyte(w.y, w.x, by), __builtin_amdgcn_alignbyte(w.z, w.y, by),
+                   __builtin_amdgcn_alignbyte(w.w, w.z, by), __builtin_amdgcn_alignbyte(w4, w.w, by));
+  }
+  return w;
+}
+
+template <typename T, int NW, bool HALF>
 __global__ __launch_bounds__(NW * 64) void short_kernel(const Product p) {
   constexpr int NV = Geo<T>::NV, RS = 4 * NV, U = 4, LD = 20;
   __shared__ __attribute__((aligned(16))) float red[NW * 16 * LD];
@@ -44,8 +61,8 @@ __global__ __launch_bounds__(NW * 64) void short_kernel(const Product p) {
     Op oa[U], ob[U];
     #pragma unroll
     for (int k = 0; k < U; ++k) {
-      __builtin_memcpy(&oa[k], a + (long long)(s + k) * RS, 16);
-      __builtin_memcpy(&ob[k], b + (long long)(s + k) * RS, 16);
+      oa[k] = __builtin_bit_cast(Op, piece_at<HALF>(a + (long long)(s + k) * RS));
+      ob[k] = __builtin_bit_cast(Op, piece_at<HALF>(b + (long long)(s + k) * RS));
     }
     #pragma unroll
     for (int k = 0; k < U; ++k) acc = multiply16(ob[k], oa[k], acc);
@@ -53,11 +70,8 @@ __global__ __launch_bounds__(NW * 64) void short_kernel(const Product p) {
   for (; s < s1; ++s) {
     // (a piece over the end: from where it fits, moved into place, as in Feeder)
     const int over = max(0, s * RS + h + NV - p.R);
-    uint4 wa, wb;
-    __builtin_memcpy(&wa, a + (long long)s * RS - over, 16);
-    __builtin_memcpy(&wb, b + (long long)s * RS - over, 16);
-    wa = moved(wa, over * (int)sizeof(T) * 8);
-    wb = moved(wb, over * (int)sizeof(T) * 8);
+    const uint4 wa = moved(piece_at<HALF>(a + (long long)s * RS - over), over * (int)sizeof(T) * 8);
+    const uint4 wb = moved(piece_at<HALF>(b + (long long)s * RS - over), over * (int)sizeof(T) * 8);
     acc = multiply16(__builtin_bit_cast(Op, wb), __builtin_bit_cast(Op, wa), acc);
   }
   *reinterpret_cast<float4*>(red + (wave * 16 + (lane & 15)) * LD + 4 * (lane >> 4)) = make_float4(acc[0], acc[1], acc[2], acc[3]);
@@ -89,12 +103,18 @@ __global__ __launch_bounds__(NW * 64) void short_kernel(const Product p) {
   }
 }
 
+template <typename T, bool HALF>
+static int run_short_as(const Product& p, hipStream_t stream) {
+  const dim3 grid((unsigned)(((long long)p.I + 15) / 16 * ((p.J + 15) / 16)));
+  if (p.R <= 16 * 4 * Geo<T>::NV) SG2IM_LAUNCH((short_kernel<T, 4, HALF>), grid, dim3(256), 0, stream, p);
+  else SG2IM_LAUNCH((short_kernel<T, 8, HALF>), grid, dim3(512), 0, stream, p);
+  return status();
+}
 template <typename T>
 static int run_short(const Product& p, hipStream_t stream) {
-  const dim3 grid((unsigned)(((long long)p.I + 15) / 16 * ((p.J + 15) / 16)));
-  if (p.R <= 16 * 4 * Geo<T>::NV) SG2IM_LAUNCH((short_kernel<T, 4>), grid, dim3(256), 0, stream, p);
-  else SG2IM_LAUNCH((short_kernel<T, 8>), grid, dim3(512), 0, stream, p);
-  return status();
+  const auto odd = [](const void* at, long long ld) { return (reinterpret_cast<unsigned long long>(at) & 2) || (ld & 1); };
+  if constexpr (sizeof(T) == 2) if (odd(p.a, p.lda) || odd(p.b, p.ldb) || p.R % 2) return run_short_as<T, true>(p, stream);
+  return run_short_as<T, false>(p, stream);
 }
 
 // ---- dz and the bias gradient -------------------------------------------------------------------------------------
