@@ -8,8 +8,10 @@
 // nor two captured graphs share one.  The library's entry points are bound by address (bind), so that this module uses
 // whichever build of it the process has loaded.
 #include <torch/extension.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <cmath>
 #include <string>
 #include <tuple>
@@ -74,6 +76,18 @@ void on_device(const Tensor& t, const char* what) {
   TORCH_CHECK_VALUE(t.device() == gpu().getDevice(), what, " lies on ", t.device(), " but the current device is ", gpu().getDevice());
 }
 Tensor given(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
+
+// These calls read and write memory below torch's dispatcher, so what follows operators there does not see them: a forward
+// gradient would come back as none, that is as a derivative of zero, and a recorded program would hold the empty outputs and
+// nothing that fills them.  Both are refused, before anything else is looked at.
+void eager_only(const char* what, std::initializer_list<Tensor> tensors) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() &&
+                              !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                              what, ": called while torch.jit.trace or make_fx records, which would not see it");
+  for (const Tensor& t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(),
+                                what, ": no forward-mode derivative (an argument carries a forward gradient)");
+}
 const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* out_ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
@@ -141,9 +155,14 @@ Packed pack(const Tensor& x) {
   done(api.pack8(ptr(r.m), code(x), r.rows, int_of(r.cols, "pack8"), r.ld, codes_ptr(p.codes), exps_ptr(p.exps), stream_of(x)), "sg2im_pack8");
   return p;
 }
-std::tuple<Tensor, Tensor> pack8(const Tensor& x) { const Packed p = pack(x); return {p.codes, p.exps}; }
+std::tuple<Tensor, Tensor> pack8(const Tensor& x) {
+  eager_only("pack8", {x});
+  const Packed p = pack(x);
+  return {p.codes, p.exps};
+}
 
 Tensor unpack8(const Tensor& codes, const Tensor& exps, int type) {
+  eager_only("unpack8", {});
   check_packed(codes, exps, "unpack8");
   TORCH_CHECK_TYPE(type == 0 || type == 1, "unpack8: float32 or bfloat16");
   Tensor out = at::empty(codes.sizes(), codes.options().dtype(type_of(type)).memory_format(c10::nullopt));
@@ -222,8 +241,9 @@ struct Target {
   Tensor grad() const { return own ? buf : Tensor(); }
 };
 
-void once() {
+void once(const char* what, const Tensor& grad) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "this operator has no second derivative (create_graph=True reached its backward pass)");
+  eager_only(what, {grad});
 }
 
 // the registered gradient buffers of a layer's two parameters (undefined: none); autograd does not see them
@@ -253,7 +273,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
     return r.y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once();
+    once("group norm backward", grads[0]);
     const variable_list s = ctx->get_saved_variables();
     // (edges are numbered over the tensors that are there)
     const bool nw = s[3].defined() && ctx->needs_input_grad(1), nb = s[4].defined() && ctx->needs_input_grad(s[3].defined() ? 2 : 1);
@@ -293,6 +313,7 @@ void check_capture(std::initializer_list<std::pair<const Tensor*, const Tensor*>
 Tensor group_norm_act(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, int64_t groups, double slope, double eps, bool checkpoint8,
                       int64_t out_type, const MaybeTensor& sink_w, const MaybeTensor& sink_b) {
   const Tensor w = given(weight), b = given(bias);
+  eager_only("group norm", {x, w, b});
   if (!(at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))))
     return gn_forward(x.contiguous(), w, b, groups, slope, eps, (int)out_type, false).y;
   const Sinks sinks{given(sink_w), given(sink_b)};
@@ -417,7 +438,7 @@ struct LinearResidual : torch::autograd::Function<LinearResidual> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once();
+    once("linear backward", grads[0]);
     const variable_list s = ctx->get_saved_variables();
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = s[5].defined() && ctx->needs_input_grad(2);
     const bool nr = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(s[5].defined() ? 3 : 2);
@@ -457,6 +478,7 @@ struct LinearResidual : torch::autograd::Function<LinearResidual> {
 Tensor linear_residual(const Tensor& x, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual, double slope, bool checkpoint8,
                        int64_t out_type, const MaybeTensor& sink_w, const MaybeTensor& sink_b) {
   const Tensor b = given(bias), r = given(residual);
+  eager_only("linear", {x, weight, b, r});
   if (!(at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(b) || wants(r)))) {
     Tensor w = weight.contiguous();
     if (is_bf16(x) && w.scalar_type() == at::kFloat) w = w.to(at::kBFloat16);
@@ -478,29 +500,35 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // the passes on their own (missing tensors: None)
   m.def("group_norm_act_forward", [](const Tensor& x, const MaybeTensor& w, const MaybeTensor& b, int64_t groups, double slope, double eps,
                                      int64_t out_type, bool pack) {
+    eager_only("group norm", {x, given(w), given(b)});
     const GnResult r = gn_forward(x, given(w), given(b), groups, slope, eps, (int)out_type, pack);
     return std::make_tuple(r.y, r.stats, r.packed.codes, r.packed.exps);
   });
   m.def("group_norm_act_backward", [](const Tensor& dy, const MaybeTensor& x, const MaybeTensor& codes, const MaybeTensor& exps, int64_t x_type,
                                       const MaybeTensor& w, const MaybeTensor& b, int64_t groups, double slope, const Tensor& stats, bool need_dx,
                                       const MaybeTensor& dw, const MaybeTensor& db, bool accumulate) {
+    eager_only("group norm backward", {dy, given(x), given(w), given(b), stats, given(dw), given(db)});
     return gn_backward(dy, given(x), Packed{given(codes), given(exps)}, (int)x_type, given(w), given(b), groups, slope, stats, need_dx, given(dw),
                        given(db), accumulate);
   });
   m.def("linear_forward", [](const Tensor& x, const Tensor& w, const MaybeTensor& b, const MaybeTensor& r, double slope, int64_t out_type, bool signs) {
+    eager_only("linear", {x, w, given(b), given(r)});
     return lin_forward(x, w, given(b), given(r), slope, (int)out_type, signs);
   });
   m.def("linear_backward_act", [](const Tensor& dy, const MaybeTensor& signs, double slope, int64_t dz_type, const MaybeTensor& db, bool accumulate) {
+    eager_only("linear backward", {dy, given(db)});
     on_device(dy, "linear gradient");
     return lin_backward_act(rows_of(dy, "linear gradient"), given(signs), slope, (int)dz_type, given(db), accumulate);
   });
   m.def("linear_backward_data", [](const Tensor& dz, const Tensor& w, const MaybeTensor& signs, double slope) {
+    eager_only("linear backward", {dz, w});
     on_device(dz, "linear gradient");
     const Rows r = rows_of(dz, "linear gradient");
     return lin_backward_data(r, given(signs), slope, w, {r.rows, w.size(-1)});
   });
   m.def("linear_backward_weight", [](const Tensor& dz, const MaybeTensor& x, const MaybeTensor& codes, const MaybeTensor& exps, const Tensor& dw,
                                      bool accumulate, const MaybeTensor& db, bool bias_accumulate, const MaybeTensor& signs, double slope) {
+    eager_only("linear backward", {dz, given(x), dw, given(db)});
     on_device(dz, "linear gradient");
     lin_backward_weight(rows_of(dz, "linear gradient"), given(signs), slope, given(x), Packed{given(codes), given(exps)}, dw, accumulate, given(db),
                         bias_accumulate);

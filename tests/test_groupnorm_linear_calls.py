@@ -1,0 +1,93 @@
+"""What may and may not be called on group norm + activation, linear + activation + residual and the 8-bit checkpoints: calls
+that record or transform operators instead of running them, the framework's own bookkeeping of launches, and calls
+at the limits of a launch."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+gpu = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def entry_points():
+  """every entry point by name: (call, its float arguments)"""
+  from sg2im_amd import functional as HF, ops
+  t = lambda *s: torch.ones(*s)  # noqa: E731
+  stats, signs = torch.ones(2, 4, 2, dtype=torch.float64), torch.zeros(6, 1, dtype=torch.int32)
+  return {
+    'group norm': (lambda x, w, b: HF.GroupNormAct.apply(x, w, b, 4, 0.2), [t(2, 3, 8), t(8), t(8)]),
+    'group norm, 8 bits': (lambda x, w, b: HF.GroupNormAct.apply(x, w, b, 4, 0.2, 1e-5, True), [t(2, 3, 8), t(8), t(8)]),
+    'linear': (lambda x, w, b, r: HF.LinearResidual.apply(x, w, b, r, 0.2), [t(6, 8), t(5, 8), t(5), t(6, 5)]),
+    'pack8': (lambda x: ops.pack8(x).codes, [t(6, 8)]),
+    'group norm forward': (lambda x, w, b: ops.group_norm_act_forward(x, w, b, 4, 0.2, 1e-5)[0], [t(2, 3, 8), t(8), t(8)]),
+    'group norm backward': (lambda dy, x, w, b: ops.group_norm_act_backward(dy, x, w, b, 4, 0.2, stats),
+                            [t(2, 3, 8), t(2, 3, 8), t(8), t(8)]),
+    'linear forward': (lambda x, w, b, r: ops.linear_forward(x, w, b, r, 0.2)[0], [t(6, 8), t(5, 8), t(5), t(6, 5)]),
+    'linear backward act': (lambda dy, db: ops.linear_backward_act(dy, signs, 0.2, F32, db), [t(6, 5), t(5)]),
+    'linear backward data': (lambda dz, w: ops.linear_backward_data(dz, w, signs, 0.2), [t(6, 5), t(5, 8)]),
+    'linear backward weight': (lambda dz, x, dw, db: ops.linear_backward_weight(dz, x, dw, dbias=db),
+                               [t(6, 5), t(6, 8), t(5, 8), t(5)]),
+  }
+
+
+# ---- calls that are followed, not only run ------------------------------------------------------------------------------
+# (refused before a device is looked at, so on CPU tensors too; those without a forward gradient get the TypeError of a CPU tensor)
+
+NAMES = ['group norm', 'group norm, 8 bits', 'linear', 'pack8', 'group norm forward', 'group norm backward', 'linear forward',
+         'linear backward act', 'linear backward data', 'linear backward weight']
+
+
+@pytest.mark.parametrize('name', NAMES)
+def test_a_forward_gradient_is_refused(name):
+  call, args = entry_points()[name]
+  assert list(entry_points()) == NAMES
+  with pytest.raises(TypeError):
+    call(*args)
+  for k in range(len(args)):
+    for needs in (False, True):
+      with fwAD.dual_level():
+        a = [t.clone() for t in args]
+        a[k] = fwAD.make_dual(a[k].requires_grad_(needs and 'ward' not in name and name != 'pack8'), torch.ones_like(a[k]))
+        with pytest.raises(NotImplementedError, match='forward'):
+          call(*a)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match='forward'):
+          call(*a)
+
+
+@pytest.mark.parametrize('name', NAMES)
+def test_a_recorded_call_is_refused(name):
+  from torch.fx.experimental.proxy_tensor import make_fx
+  call, args = entry_points()[name]
+  with pytest.raises(NotImplementedError, match='records'):
+    torch.jit.trace(call, tuple(args))
+  with pytest.raises(NotImplementedError, match='records'):
+    make_fx(call)(*args)
+  with pytest.raises(TypeError):                          # (and nothing of it stays behind)
+    call(*args)
+
+
+def test_unpack8_is_refused_in_a_recording():
+  from torch.fx.experimental.proxy_tensor import make_fx
+  from sg2im_amd import ops
+  call = lambda c, e: ops.unpack8(ops.Packed8(c, e, F32))  # noqa: E731
+  args = (torch.zeros(2, 8, dtype=torch.int8), torch.zeros(2, 1, dtype=torch.uint8))
+  for record in (lambda: torch.jit.trace(call, args), lambda: make_fx(call)(*args)):
+    with pytest.raises(NotImplementedError, match='records'):
+      record()
+
+
+@gpu
+def test_forward_gradients_and_recordings_are_refused_on_the_gpu():
+  from sg2im_amd import functional as HF
+  x, w = torch.randn(6, 32, device='cuda'), torch.randn(32, 32, device='cuda')
+  calls = (lambda x, w: HF.GroupNormAct.apply(x, None, None, 4, 0.2), lambda x, w: HF.LinearResidual.apply(x, w, None, x, 0.2))
+  for call in calls:
+    with fwAD.dual_level(), pytest.raises(NotImplementedError):
+      call(fwAD.make_dual(x, w[:6].contiguous()), w)
+    with pytest.raises(NotImplementedError):
+      torch.jit.trace(call, (x, w))
+    # forward over reverse: the gradient that comes in carries one
+    xr = x.clone().requires_grad_(True)
+    y = call(xr, w)
+    with fwAD.dual_level(), pytest.raises(NotImplementedError):
+      torch.autograd.grad(y, (xr,), fwAD.make_dual(torch.ones_like(y), torch.ones_like(y)))
