@@ -91,3 +91,32 @@ def test_forward_gradients_and_recordings_are_refused_on_the_gpu():
     y = call(xr, w)
     with fwAD.dual_level(), pytest.raises(NotImplementedError):
       torch.autograd.grad(y, (xr,), fwAD.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@gpu
+def test_a_pending_negation_is_carried_out():
+  """the imaginary part of a conjugate is a view of the numbers before their sign is turned"""
+  from sg2im_amd import functional as HF, ops
+  z = torch.complex(torch.randn(64, 2, device='cuda'), torch.randn(64, 2, device='cuda')).conj()
+  v = z.imag
+  real = -(-v).clone()
+  neg = torch._neg_view
+  assert v.is_neg() and not real.is_neg() and torch.equal(v, real)
+  for f in (lambda t: ops.unpack8(ops.pack8(t)), lambda t: HF.GroupNormAct.apply(t, None, None, 1, 0.2)):
+    for take in (lambda t: t, lambda t: t[:, :1], lambda t: t[:1]):
+      assert torch.equal(f(take(v)), f(take(real)))
+    assert torch.equal(f(neg(-real)), f(real))
+  w = torch.randn(3, 1, device='cuda')
+  res = torch.randn(64, 3, device='cuda')
+  dy = torch.randn(64, 3, device='cuda')
+  outs = []
+  for x, a, r, g in ((real[:, :1], w, res, dy), (v[:, :1], neg(-w), neg(-res), neg(-dy))):
+    leaves = [t.detach().requires_grad_(True) for t in (x, a, r)]
+    y = HF.LinearResidual.apply(leaves[0], leaves[1], None, leaves[2], 0.2)
+    outs.append([y.detach()] + [t.clone() for t in torch.autograd.grad(y, leaves, g)])
+  assert all(torch.equal(p, q) for p, q in zip(*outs))
+  # (the single passes take tensors as they lie in memory)
+  with pytest.raises(ValueError, match='negation'):
+    ops.linear_forward(neg(real), w[:, :1].expand(3, 2).contiguous(), None, None, 1.0)
+  with pytest.raises(ValueError, match='negation'):
+    HF.GroupNormAct.apply(real, neg(torch.ones(2, device='cuda')), None, 1)
