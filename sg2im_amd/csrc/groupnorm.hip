@@ -51,6 +51,7 @@ struct Params {
   int N, C, G, D, L, rows, full_rows, chunks, rows_per_chunk, slabs, TV, TP, nblk;
   int S;                             // slab kernels: positions per workgroup
   int merged;                        // the normalising pass joins the chunks' sums itself
+  int span;                          // of the channels of the groups that a slab touches, the most
   int bypass;                        // the backward statistics read dy past the caches
 };
 
@@ -316,12 +317,13 @@ __device__ __forceinline__ void write_codes(const Params& p, int n, int row, int
 }
 
 // Statistics of the groups that the slab's channels [c0, c0 + width) belong to, from the chunks' sums, into st[group][2];
-// returns the first group.  Every workgroup of an image does it over again: a few KB from the L2 against a launch of its own
+// returns the first group.  A group that reaches over a slab's border is joined by two slabs: in the same order, since how many
+// threads share a sum goes by the widest slab, and written by the one that holds its first channel.  Every workgroup of an image does it over again: a few KB from the L2 against a launch of its own
 // between the two passes (32 x 64 x 64 x 64 float 24.4 -> 21.7 us, 32 x 128 x 128 x 64 72 -> 69).
 constexpr int MERGE_SPAN = 512;
 __device__ __forceinline__ int merged_stats(const Params& p, const Place& w, int c0, int width, double* st) {
   __shared__ double red[2 * MERGE_SPAN];
-  const int g0 = c0 / p.D, g1 = (min(p.C, c0 + width) - 1) / p.D + 1, span = (g1 - g0) * p.D, parts = max(1, THREADS / span);
+  const int g0 = c0 / p.D, g1 = (min(p.C, c0 + width) - 1) / p.D + 1, span = (g1 - g0) * p.D, parts = max(1, THREADS / p.span);
   const double* part = reinterpret_cast<const double*>(p.part) + (long long)w.n * p.chunks * 2 * p.L + g0 * p.D;
   for (int i = threadIdx.x; i < span * parts; i += THREADS) {
     const int c = i % span;
@@ -346,7 +348,8 @@ __device__ __forceinline__ int merged_stats(const Params& p, const Place& w, int
   }
   __syncthreads();
   if (w.row0 == 0)
-    for (int i = threadIdx.x; i < 2 * (g1 - g0); i += THREADS) p.stats[((long long)w.n * p.G + g0) * 2 + i] = st[i];
+    for (int i = threadIdx.x; i < 2 * (g1 - g0); i += THREADS)
+      if ((g0 + i / 2) * p.D >= c0) p.stats[((long long)w.n * p.G + g0) * 2 + i] = st[i];
   return g0;
 }
 
@@ -1026,6 +1029,13 @@ bool slab_plan(const Params& p, int nv, int most, SlabPlan& q) {
   return false;
 }
 
+// channels of the groups that a slab of `width` channels touches, the most over the slabs
+int slab_span(const Params& p, int width) {
+  int most = 0;
+  for (int c0 = 0; c0 < p.C; c0 += width) most = std::max(most, ((std::min(p.C, c0 + width) - 1) / p.D + 1 - c0 / p.D) * p.D);
+  return most;
+}
+
 size_t part_bytes(const Params& p, bool backward) {
   return (size_t)p.N * p.chunks * 2 * p.L * (backward ? 4 : 8);
 }
@@ -1071,6 +1081,7 @@ void launch_forward(const Params& p0, hipStream_t stream) {
   SG2IM_LAUNCH(fwd_partial_kernel<TX>, dim3(blocks), dim3(THREADS), 0, stream, p);
   // (a slab's groups reach over it by less than a group on either side)
   p.merged = p.L == p.C && p.chunks <= 64 && p.TV * VecOf<TX>::n + 2 * (p.D - 1) <= MERGE_SPAN && (p.TV * VecOf<TX>::n + 2 * p.D) * p.chunks <= 16384;
+  if (p.merged) p.span = slab_span(p, p.TV * VecOf<TX>::n);
   const long long per = (long long)p.chunks * (p.L / p.C) * p.D;
   const int threads = per <= 256 ? 64 : per <= 4096 ? 256 : 1024;
   if (!p.merged) SG2IM_LAUNCH(fwd_finish_kernel, dim3((unsigned)((long long)p.N * p.G)), dim3(threads), 0, stream, p);

@@ -120,3 +120,41 @@ def test_a_pending_negation_is_carried_out():
     ops.linear_forward(neg(real), w[:, :1].expand(3, 2).contiguous(), None, None, 1.0)
   with pytest.raises(ValueError, match='negation'):
     HF.GroupNormAct.apply(real, neg(torch.ones(2, device='cuda')), None, 1)
+
+
+# ---- one group, several workgroups ----------------------------------------------------------------------------------------
+
+# (channels, groups): widths at which groups reach over the border of the channels that one workgroup takes, a narrow last run
+# of channels among them (1600 and 1824 float: the last workgroups' groups are fewer than half of the others'), and one at
+# which none does
+CROSSING = [(1600, 32, F32), (1632, 32, F32), (1824, 32, F32), (1856, 32, F32), (640, 32, F32), (900, 20, F32), (1040, 16, BF16),
+            (2080, 32, BF16), (1024, 32, F32)]
+
+
+@gpu
+@pytest.mark.parametrize('channels,groups,dtype', CROSSING)
+def test_groups_that_cross_workgroups_have_one_statistic(channels, groups, dtype):
+  """every group holds the same numbers: its statistics, and what is normalised with them, have to be the same bits whichever
+  workgroup joined the sums; and the same call gives the same bits"""
+  from sg2im_amd import ops
+  g = torch.Generator(device='cuda').manual_seed(channels)
+  D = channels // groups
+  one = (torch.randn(4, 32, 32, D, device='cuda', generator=g) * 3 + 1).to(dtype)
+  x = one.repeat(1, 1, 1, groups)
+  dy = torch.randn(4, 32, 32, channels, device='cuda', generator=g).to(dtype)
+  first = None
+  for _ in range(8):
+    y, stats, _ = ops.group_norm_act_forward(x, None, None, groups, 0.2, 1e-5)
+    dx = ops.group_norm_act_backward(dy, x, None, None, groups, 0.2, stats)
+    assert torch.equal(stats, stats[:, :1].expand_as(stats))
+    assert torch.equal(y, y[..., :D].repeat(1, 1, 1, groups))
+    if first is None:
+      first = (y, stats, dx)
+    assert all(torch.equal(a, b) for a, b in zip(first, (y, stats, dx)))
+  v = one.to(torch.float64)
+  mean, rstd = v.mean((1, 2, 3)), (v.var((1, 2, 3), unbiased=False) + 1e-5).rsqrt()
+  # (n values summed in 64 bits: n 2^-53 of the absolute sums, the mean's square taken from the square's mean)
+  n, eps = 1024 * D, 2.0 ** -53
+  scale = v.square().mean((1, 2, 3))
+  assert bool(((first[1][:, 0, 0] - mean).abs() <= n * eps * v.abs().mean((1, 2, 3))).all())
+  assert bool(((first[1][:, 0, 1] - rstd).abs() <= 4 * n * eps * scale * rstd ** 3).all())
