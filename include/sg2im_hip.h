@@ -673,7 +673,9 @@ int sg2im_adam_apply_guarded(float* param, const float* grad, float* exp_avg, fl
  *             32-bit value is within its rounding of zero; at exactly zero the gradient takes `slope`.
  * workspace: sg2im_groupnorm_workspace bytes, 16-byte aligned, used by this call only.  No alignment beyond an element's is
  * assumed of the tensors.  Statistics are summed in 64 bits, in a fixed order: the same call gives the same bits.
- * SG2IM_ERR_ARG: channels % groups, hw < 1, a NULL that is needed, a workspace that is too small. */
+ * Any batch is taken: where one launch does not hold it, several do.  SG2IM_ERR_ARG: channels % groups, hw < 1 or >= 2^30,
+ * 2^28 (bfloat16) / 2^29 (float) channels and more, more groups than a launch takes (fewer than 2^22 always fit), a NULL that is
+ * needed, a workspace that is too small.  The workspace query answers 0 for sizes that are refused. */
 size_t sg2im_groupnorm_workspace(int batch, long long hw, int channels, int groups, int x_dtype, int backward);
 int sg2im_groupnorm_act_forward(const void* x, int x_dtype, int batch, long long hw, int channels, int groups,
                                 const void* gamma, const void* beta, int param_dtype, float slope, float eps, void* out,

@@ -13,6 +13,7 @@
 // the 32-bit z unless |z| is within that value's rounding of zero, and then from z in 64 bits.
 #include <hip/hip_runtime.h>
 #include <algorithm>
+#include <type_traits>
 #include "sg2im_hip.h"
 #include "launch_count.h"
 #include "vecio.h"
@@ -980,6 +981,16 @@ unsigned piece_blocks(long long pieces) { return (unsigned)std::max(1LL, std::mi
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
+constexpr long long LAUNCH_THREADS = 0xffffffffLL;
+
+// the finish launches: threads of a workgroup per (image, group) forward, workgroups per image backward
+int finish_threads(const Params& p) {
+  const long long per = (long long)p.chunks * (p.L / p.C) * p.D;
+  return per <= 256 ? 64 : per <= 4096 ? 256 : 1024;
+}
+int groups_per_block(const Params& p) { return p.D >= FIN_CH ? 1 : FIN_CH / p.D; }
+int finish_blocks(const Params& p) { return (p.G + groups_per_block(p) - 1) / groups_per_block(p); }
+
 // How an image is cut: slabs of at most 64 pieces across a row, and chunks of rows so that there are about 1 024
 // workgroups (4 per CU; 2 048 and more cost 3 % and up on the largest map, in partial sums) - but never less than four rows per lane, where a workgroup would be all set-up.
 bool cut(Params& p, int N, long long hw, int C, int G, int x_bf16) {
@@ -1003,8 +1014,33 @@ bool cut(Params& p, int N, long long hw, int C, int G, int x_bf16) {
   rpc = std::min(rpc, std::max(1LL, rows));
   p.rows_per_chunk = (int)rpc;
   p.chunks = (int)((rows + rpc - 1) / rpc);
-  // (a launch has fewer than 2^32 threads)
-  return ((long long)N * p.chunks * p.slabs + (C + 31) / 32) * THREADS <= 0xffffffffLL && (long long)N * G * 1024 <= 0xffffffffLL;
+  // (each launch of one image)
+  return ((long long)p.chunks * p.slabs + (C + 31) / 32) * THREADS <= LAUNCH_THREADS && (long long)G * finish_threads(p) <= LAUNCH_THREADS &&
+         (long long)finish_blocks(p) * FIN_CH * FIN_LANES <= LAUNCH_THREADS;
+}
+
+// A launch has fewer than 2^32 threads, so a batch of many small images takes several: launch(parameters of the images from
+// n on, how many, whether they are all).  TX, TY, TP: x; dy; the chunks' sums, OUT: y or dx.
+template <typename TX, typename TY, typename OUT, typename TP, typename F>
+void over_images(const Params& p, long long blocks_per_image, int threads, F launch) {
+  const long long most = std::max(1LL, LAUNCH_THREADS / (blocks_per_image * threads));
+  for (long long n = 0; n < p.N; n += most) {
+    Params q = p;
+    auto move = [](auto*& at, long long bytes) { if (at) at = reinterpret_cast<std::remove_reference_t<decltype(at)>>((unsigned long long)at + bytes); };
+    move(q.x, n * p.E * (int)sizeof(TX));
+    move(q.codes, n * p.E);
+    move(q.exps, n * (p.E / p.C) * p.nblk);
+    move(q.codes_out, n * p.E);
+    move(q.exps_out, n * (p.E / p.C) * p.nblk);
+    move(q.dy, n * p.E * (int)sizeof(TY));
+    move(q.out, n * p.E * (int)sizeof(OUT));
+    move(q.stats, n * p.G * 2 * 8);
+    move(q.part, n * p.chunks * 2 * p.L * (int)sizeof(TP));
+    move(q.chan, n * p.C * 2 * 8);
+    move(q.coef, n * p.G * 2 * 4);
+    const long long count = std::min(most, p.N - n);
+    launch(q, count, count == p.N);
+  }
 }
 
 // The slab kernels' cut: the fewest positions that hold whole groups, whole pieces (`unit`) and 32 channels, more of them where
@@ -1024,7 +1060,7 @@ bool slab_plan(const Params& p, int nv, int most, SlabPlan& q) {
   for (int k = 0; k < 4; ++k) {
     const int tp = forms[k][0] / (S / nv);
     if (k >= 2 && k != most) continue;
-    if (tp > 0 && (long long)tp * forms[k][1] >= p.rows && (long long)p.N * q.slabs * forms[k][0] <= 0xffffffffLL) { q.threads = forms[k][0]; q.iter = forms[k][1]; return true; }
+    if (tp > 0 && (long long)tp * forms[k][1] >= p.rows) { q.threads = forms[k][0]; q.iter = forms[k][1]; return true; }
   }
   return false;
 }
@@ -1056,14 +1092,18 @@ int pack(const void* x, long long rows, int C, int nblk, long long ld, signed ch
 }
 
 template <typename TX, typename TY, int B, int ITER>
-void forward_slabs(const Params& p, hipStream_t stream) {
-  const dim3 grid((unsigned)((long long)p.N * p.slabs));
-  if (p.codes_out) SG2IM_LAUNCH((fwd_slab_kernel<TX, TY, true, B, ITER>), grid, dim3(B), 0, stream, p);
-  else SG2IM_LAUNCH((fwd_slab_kernel<TX, TY, false, B, ITER>), grid, dim3(B), 0, stream, p);
+void forward_slabs(const Params& p0, hipStream_t stream) {
+  over_images<TX, char, TY, double>(p0, p0.slabs, B, [&](const Params& p, long long images, bool) {
+    const dim3 grid((unsigned)(images * p.slabs));
+    if (p.codes_out) SG2IM_LAUNCH((fwd_slab_kernel<TX, TY, true, B, ITER>), grid, dim3(B), 0, stream, p);
+    else SG2IM_LAUNCH((fwd_slab_kernel<TX, TY, false, B, ITER>), grid, dim3(B), 0, stream, p);
+  });
 }
 template <typename SRC, typename TX, typename TY, bool EVEN, int B, int ITER>
-void backward_slabs(const Params& p, hipStream_t stream) {
-  SG2IM_LAUNCH((bwd_slab_kernel<SRC, TX, TY, EVEN, B, ITER>), dim3((unsigned)((long long)p.N * p.slabs)), dim3(B), 0, stream, p);
+void backward_slabs(const Params& p0, hipStream_t stream) {
+  over_images<TX, TY, TX, float>(p0, p0.slabs, B, [&](const Params& p, long long images, bool) {
+    SG2IM_LAUNCH((bwd_slab_kernel<SRC, TX, TY, EVEN, B, ITER>), dim3((unsigned)(images * p.slabs)), dim3(B), 0, stream, p);
+  });
 }
 
 template <typename TX, typename TY>
@@ -1077,16 +1117,23 @@ void launch_forward(const Params& p0, hipStream_t stream) {
     else forward_slabs<TX, TY, 1024, 4>(p, stream);
     return;
   }
-  const unsigned blocks = (unsigned)((long long)p.N * p.chunks * p.slabs);
-  SG2IM_LAUNCH(fwd_partial_kernel<TX>, dim3(blocks), dim3(THREADS), 0, stream, p);
+  const long long per_image = (long long)p.chunks * p.slabs;
+  over_images<TX, char, TY, double>(p, per_image, THREADS, [&](const Params& s, long long images, bool) {
+    SG2IM_LAUNCH(fwd_partial_kernel<TX>, dim3((unsigned)(images * per_image)), dim3(THREADS), 0, stream, s);
+  });
   // (a slab's groups reach over it by less than a group on either side)
   p.merged = p.L == p.C && p.chunks <= 64 && p.TV * VecOf<TX>::n + 2 * (p.D - 1) <= MERGE_SPAN && (p.TV * VecOf<TX>::n + 2 * p.D) * p.chunks <= 16384;
   if (p.merged) p.span = slab_span(p, p.TV * VecOf<TX>::n);
-  const long long per = (long long)p.chunks * (p.L / p.C) * p.D;
-  const int threads = per <= 256 ? 64 : per <= 4096 ? 256 : 1024;
-  if (!p.merged) SG2IM_LAUNCH(fwd_finish_kernel, dim3((unsigned)((long long)p.N * p.G)), dim3(threads), 0, stream, p);
-  if (p.codes_out) SG2IM_LAUNCH((fwd_apply_kernel<TX, TY, true>), dim3(blocks), dim3(THREADS), 0, stream, p);
-  else SG2IM_LAUNCH((fwd_apply_kernel<TX, TY, false>), dim3(blocks), dim3(THREADS), 0, stream, p);
+  const int threads = finish_threads(p);
+  if (!p.merged)
+    over_images<TX, char, TY, double>(p, p.G, threads, [&](const Params& s, long long images, bool) {
+      SG2IM_LAUNCH(fwd_finish_kernel, dim3((unsigned)(images * s.G)), dim3(threads), 0, stream, s);
+    });
+  over_images<TX, char, TY, double>(p, per_image, THREADS, [&](const Params& s, long long images, bool) {
+    const dim3 blocks((unsigned)(images * per_image));
+    if (s.codes_out) SG2IM_LAUNCH((fwd_apply_kernel<TX, TY, true>), blocks, dim3(THREADS), 0, stream, s);
+    else SG2IM_LAUNCH((fwd_apply_kernel<TX, TY, false>), blocks, dim3(THREADS), 0, stream, s);
+  });
 }
 
 template <typename SRC, typename TX, typename TY, bool EVEN>
@@ -1103,19 +1150,27 @@ void launch_backward(const Params& p0, bool need_dx, bool need_params, hipStream
     if (p.N > 1 && need_params) SG2IM_LAUNCH(param_grads_kernel, dim3((p.C + 31) / 32), dim3(THREADS), 0, stream, p);
     return;
   }
-  const long long blocks = (long long)p.N * p.chunks * p.slabs;
+  const long long per_image = (long long)p.chunks * p.slabs;
   // Where x and dy together are far beyond the 256 MB cache, one of them can stay in it between the two passes if the other
   // goes past: 32 x 256 x 256 x 64 bfloat16 263 -> 217 us.  Where most of both stays anyway that costs (268 MB: 111 -> 114).
   p.bypass = (double)p.N * p.E * (sizeof(SRC) + sizeof(TY)) > 384e6;
-  SG2IM_LAUNCH((bwd_partial_kernel<SRC, TX, TY, EVEN>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
-  const int gpb = p.D >= FIN_CH ? 1 : FIN_CH / p.D;
-  SG2IM_LAUNCH(bwd_finish_kernel, dim3((unsigned)((long long)p.N * ((p.G + gpb - 1) / gpb))), dim3(FIN_CH * FIN_LANES), 0,
-               stream, p, gpb);
+  over_images<TX, TY, TX, float>(p, per_image, THREADS, [&](const Params& s, long long images, bool) {
+    SG2IM_LAUNCH((bwd_partial_kernel<SRC, TX, TY, EVEN>), dim3((unsigned)(images * per_image)), dim3(THREADS), 0, stream, s);
+  });
+  const int gpb = groups_per_block(p), fin = finish_blocks(p);
+  over_images<TX, TY, TX, float>(p, fin, FIN_CH * FIN_LANES, [&](const Params& s, long long images, bool) {
+    SG2IM_LAUNCH(bwd_finish_kernel, dim3((unsigned)(images * fin)), dim3(FIN_CH * FIN_LANES), 0, stream, s, gpb);
+  });
+  // (the parameters' sums run over all images: behind the map of a launch that has them all, or in one of their own)
   const int tail = need_params ? (p.C + 31) / 32 : 0;
+  bool summed = false;
   if (need_dx)
-    SG2IM_LAUNCH((bwd_apply_kernel<SRC, TX, TY, EVEN>), dim3((unsigned)(blocks + tail)), dim3(THREADS), 0, stream, p, blocks);
-  else if (tail)
-    SG2IM_LAUNCH(param_grads_kernel, dim3(tail), dim3(THREADS), 0, stream, p);
+    over_images<TX, TY, TX, float>(p, per_image + tail, THREADS, [&](const Params& s, long long images, bool all) {
+      const long long blocks = images * per_image;
+      summed = all;
+      SG2IM_LAUNCH((bwd_apply_kernel<SRC, TX, TY, EVEN>), dim3((unsigned)(blocks + (all ? tail : 0))), dim3(THREADS), 0, stream, s, blocks);
+    });
+  if (tail && !summed) SG2IM_LAUNCH(param_grads_kernel, dim3(tail), dim3(THREADS), 0, stream, p);
 }
 template <typename TX, typename TY>
 void launch_backward(const Params& p, bool need_dx, bool need_params, hipStream_t stream) {

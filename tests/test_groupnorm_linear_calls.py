@@ -158,3 +158,56 @@ def test_groups_that_cross_workgroups_have_one_statistic(channels, groups, dtype
   scale = v.square().mean((1, 2, 3))
   assert bool(((first[1][:, 0, 0] - mean).abs() <= n * eps * v.abs().mean((1, 2, 3))).all())
   assert bool(((first[1][:, 0, 1] - rstd).abs() <= 4 * n * eps * scale * rstd ** 3).all())
+
+
+# ---- many small images ----------------------------------------------------------------------------------------------------
+
+def test_row_wise_batches_are_not_refused():
+  """(the workspace query answers 0 for a size that the passes refuse)"""
+  from sg2im_amd import _lib
+  lib = _lib.load()
+  for backward in (0, 1):
+    for batch, hw, channels, groups, bf16 in ((131072, 1, 128, 32, 0), (131072, 1, 64, 32, 1), (1 << 24, 1, 32, 4, 1), (1 << 20, 4, 256, 256, 0),
+                                              (300000, 1, 4096, 1, 1), (0x7fffffff, 1, 8, 8, 0)):
+      assert lib.sg2im_groupnorm_workspace(batch, hw, channels, groups, bf16, backward) > 0, (batch, channels, groups)
+    for batch, hw, channels, groups, bf16 in ((1, 1 << 30, 8, 1, 0), (1, 1, 1 << 28, 1, 1), (1, 1, 1 << 28, 1 << 28, 0), (-1, 1, 8, 1, 0), (1, 0, 8, 1, 0)):
+      assert lib.sg2im_groupnorm_workspace(batch, hw, channels, groups, bf16, backward) == 0, (batch, channels, groups)
+
+
+@gpu
+@pytest.mark.parametrize('batch,channels,groups,dtype', [(131072, 128, 32, F32), (131072, 64, 4, BF16), (140000, 96, 32, BF16),
+                                                         ((1 << 24) + 4096, 32, 2, BF16)])      # (the last: two launches)
+def test_row_wise_batches(batch, channels, groups, dtype):
+  """rows repeated with a period, against the period's values in 64 bits"""
+  from sg2im_amd import ops
+  from tests.test_groupnorm_linear_ckpt8 import check, eight, gen, gn_reference, half_step, u32
+  period = 4096
+  r = gen(channels)
+  rows, d = (2 * r(period, channels) + r(channels)).to(dtype), r(period, channels).to(dtype)
+  w, b = (1 + 0.2 * r(channels)).to(dtype), (0.2 * r(channels)).to(dtype)
+  times, rest = batch // period, batch % period
+  x, dy = torch.empty(batch, channels, device='cuda', dtype=dtype), torch.empty(batch, channels, device='cuda', dtype=dtype)
+  for full, one in ((x, rows), (dy, d)):
+    full[:times * period].view(times, period, channels).copy_(one)
+    full[times * period:] = one[:rest]
+  for pack in (False, True):
+    y, stats, packed = ops.group_norm_act_forward(x, w, b, groups, 0.2, 1e-5, pack=pack)
+    dw, db = torch.empty(channels, device='cuda'), torch.empty(channels, device='cuda')
+    if dtype == BF16:
+      dw, db = dw.to(dtype), db.to(dtype)
+    dx = ops.group_norm_act_backward(dy, packed if pack else x, w, b, groups, 0.2, stats, True, dw, db)
+    f = gn_reference(rows, eight(rows)[0] if pack else rows, w, b, groups, 0.2, 1e-5, d)
+    for got, name, t in ((y, 'y', dtype), (dx, 'dx', dtype)):
+      tol = f[name + '_tol'] + half_step(t) * f[name].abs()
+      for at in range(0, times, max(1, times // 7)):
+        check(got[at * period:(at + 1) * period], f[name], tol, name)
+      check(got[(times - 1) * period:times * period], f[name], tol, name)
+      check(got[times * period:], f[name][:rest], tol[:rest] if tol.dim() else tol, name)
+      # every period is the same bits
+      whole = got[:times * period].view(times, -1)
+      assert torch.equal(whole, whole[:1].expand_as(whole)), name
+    tail = gn_reference(rows[:rest], eight(rows[:rest])[0] if pack else rows[:rest], w, b, groups, 0.2, 1e-5, d[:rest]) if rest else None
+    for got, name in ((dw, 'dw'), (db, 'db')):
+      want = times * f[name] + (tail[name] if rest else 0)
+      tol = times * f[name + '_tol'] + (tail[name + '_tol'] if rest else 0)
+      check(got, want, tol + (half_step(dtype) + u32) * want.abs(), name)
