@@ -237,12 +237,13 @@ def native():
     spec.loader.exec_module(mod)
     mod.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in _SIGNATURES
               if name.startswith(('sg2im_init', 'sg2im_groupnorm', 'sg2im_linear', 'sg2im_pack8', 'sg2im_unpack8'))})
+    mod.observe(_observe)
     _native = mod
   return _native
 
 
 _TRACE = os.environ.get('SG2IM_TRACE', '') == '1'
-EAGER_EPOCH = 0      # number of EAGER launches made through this binding (captured ones do not count)
+EAGER_EPOCH = 0      # number of EAGER launches made through call() (captured ones do not count); see eager_epoch()
 CAPTURING = False    # set by the Trainer around a stream capture: launches are recorded, not executed
 _inited = False
 
@@ -257,12 +258,46 @@ def init():
     _inited = True
 
 
+def eager_epoch():
+  """number of EAGER launches of the library so far, those of the host module among them (also from its backward passes)"""
+  return EAGER_EPOCH + (_native.eager_launches() if _native is not None else 0)
+
+
+timed = None         # ops._native_timed: times the host module's launches
+_watching = False
+
+
+def _observe(name, kind, amount, token):
+  """called by the host module before (token: None) and after each of its launches, while it is watched"""
+  if token is None and timed is None:
+    return (None,)
+  if token is None:
+    return (timed(kind, amount, None),)
+  if token[0] is not None:
+    timed(kind, amount, token[0])
+  if _TRACE:
+    _trace(name)
+  return token
+
+
 def eager():
-  """the host module, for a call that launches: counted as eager outside a capture, like those of call()"""
-  global EAGER_EPOCH
-  if not CAPTURING:
-    EAGER_EPOCH += 1
-  return _native or native()
+  """the host module, for a call that launches; watched while launches are traced or timed"""
+  global _watching
+  mod = _native or native()
+  watch = _TRACE or (timed is not None and timed.active())
+  if watch is not _watching:
+    mod.watch(watch)
+    _watching = watch
+  return mod
+
+
+def _trace(name):
+  import sys
+  import torch
+  sys.stderr.write('[sg2im] %s\n' % name)
+  sys.stderr.flush()
+  if not torch.cuda.is_current_stream_capturing():
+    torch.cuda.synchronize()
 
 
 def call(name, *args):
@@ -275,12 +310,7 @@ def call(name, *args):
     EAGER_EPOCH += 1          # see sg2im_amd/trainer.py::_graph_step (graph invalidation)
   rc = getattr(load(), name)(*args)
   if _TRACE:
-    import sys
-    import torch
-    sys.stderr.write('[sg2im] %s\n' % name)
-    sys.stderr.flush()
-    if not torch.cuda.is_current_stream_capturing():
-      torch.cuda.synchronize()
+    _trace(name)
   if rc != SG2IM_OK:
     kind = {SG2IM_ERR_ARG: 'invalid argument', SG2IM_ERR_HIP: 'HIP runtime error'}.get(rc, 'error %d' % rc)
     raise Sg2imHipError('%s failed: %s' % (name, kind))

@@ -12,6 +12,7 @@
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/jit/frontend/tracer.h>
+#include <atomic>
 #include <cmath>
 #include <string>
 #include <tuple>
@@ -57,11 +58,40 @@ const c10::impl::VirtualGuardImpl& gpu() {
   static const c10::impl::VirtualGuardImpl impl(c10::DeviceType::CUDA);
   return impl;
 }
-// (the last thing before a launch: the library's one-time set-up comes first)
+
+// ---- launches ---------------------------------------------------------------------------------------------------------
+// The framework follows its launches: it counts the eager ones, times them by kind and prints them (_lib.call, ops._timed).  Those of
+// this module are counted here - the backward passes' too, which no Python sees - and, while it is watched, announced to the
+// observer before and after: observer(name, kind, amount, None) -> token, observer(name, kind, amount, token).
+std::atomic<long long> eager_launches{0};
+std::atomic<bool> watched{false};
+PyObject* observer = nullptr;            // (held until the process ends)
+
+void notify(const char* name, const char* kind, double amount, py::object& token) {
+  token = py::reinterpret_borrow<py::object>(observer)(name, kind, amount, token);
+}
+
+// t's current stream, for a launch (the library's one-time set-up comes first)
 hipStream_t stream_of(const Tensor& t) {
   static const int ready = api.init();
   done(ready, "sg2im_init");
-  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
+  const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream(t.device().index());
+  hipStreamCaptureStatus status;               // (the default stream takes part in no capture, and is not to be asked during one)
+  if (now == c10::hip::getDefaultHIPStream(t.device().index()) || hipStreamIsCapturing(now.stream(), &status) != hipSuccess ||
+      status == hipStreamCaptureStatusNone) ++eager_launches;
+  return now.stream();
+}
+
+// kind, amount: as ops._timed's (flops of the products, bytes of the others)
+template <typename F> void launch(const char* name, const char* kind, double amount, const Tensor& on, F call) {
+  const hipStream_t stream = stream_of(on);
+  if (!watched) { done(call(stream), name); return; }
+  py::gil_scoped_acquire gil;
+  py::object token = py::none();
+  notify(name, kind, amount, token);
+  const int result = call(stream);
+  notify(name, kind, amount, token);
+  done(result, name);
 }
 
 // ---- checks -----------------------------------------------------------------------------------------------------------
@@ -153,7 +183,9 @@ Packed pack(const Tensor& x) {
   on_device(x, "pack8");
   const Rows r = rows_of(x, "pack8");
   Packed p = packed_like(x);
-  done(api.pack8(ptr(r.m), code(x), r.rows, int_of(r.cols, "pack8"), r.ld, codes_ptr(p.codes), exps_ptr(p.exps), stream_of(x)), "sg2im_pack8");
+  launch("sg2im_pack8", "hbm_pack8", x.numel() * (x.element_size() + 33.0 / 32), x, [&](hipStream_t stream) {
+    return api.pack8(ptr(r.m), code(x), r.rows, int_of(r.cols, "pack8"), r.ld, codes_ptr(p.codes), exps_ptr(p.exps), stream);
+  });
   return p;
 }
 std::tuple<Tensor, Tensor> pack8(const Tensor& x) {
@@ -168,7 +200,9 @@ Tensor unpack8(const Tensor& codes, const Tensor& exps, int type) {
   TORCH_CHECK_TYPE(type == 0 || type == 1, "unpack8: float32 or bfloat16");
   Tensor out = at::empty(codes.sizes(), codes.options().dtype(type_of(type)).memory_format(c10::nullopt));
   const int64_t C = codes.size(-1);
-  done(api.unpack8(codes_ptr(codes), exps_ptr(exps), codes.numel() / C, int_of(C, "unpack8"), out_ptr(out), type, C, stream_of(codes)), "sg2im_unpack8");
+  launch("sg2im_unpack8", "hbm_unpack8", codes.numel() * (out.element_size() + 33.0 / 32), codes, [&](hipStream_t stream) {
+    return api.unpack8(codes_ptr(codes), exps_ptr(exps), codes.numel() / C, int_of(C, "unpack8"), out_ptr(out), type, C, stream);
+  });
   return out;
 }
 
@@ -202,9 +236,11 @@ GnResult gn_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, i
   r.stats = at::empty({s.n, s.g, 2}, x.options().dtype(at::kDouble).memory_format(c10::nullopt));
   if (pack) r.packed = packed_like(x);
   const Tensor w = work(x, bytes);
-  done(api.groupnorm_act_forward(ptr(x), code(x), s.n, s.hw, s.c, s.g, ptr(weight), ptr(bias), pc, (float)slope, (float)eps, out_ptr(r.y), out_type,
-                                 reinterpret_cast<double*>(out_ptr(r.stats)), codes_ptr(r.packed.codes), exps_ptr(r.packed.exps), out_ptr(w), bytes,
-                                 stream_of(x)), "sg2im_groupnorm_act_forward");
+  launch("sg2im_groupnorm_act_forward", "hbm_group_norm_fwd", x.numel() * (x.element_size() + r.y.element_size() + (pack ? 33.0 / 32 : 0.0)), x, [&](hipStream_t stream) {
+    return api.groupnorm_act_forward(ptr(x), code(x), s.n, s.hw, s.c, s.g, ptr(weight), ptr(bias), pc, (float)slope, (float)eps, out_ptr(r.y), out_type,
+         reinterpret_cast<double*>(out_ptr(r.stats)), codes_ptr(r.packed.codes), exps_ptr(r.packed.exps), out_ptr(w), bytes,
+         stream);
+  });
   return r;
 }
 
@@ -225,9 +261,11 @@ Tensor gn_backward(const Tensor& dy, const Tensor& x, const Packed& packed, int 
   const size_t bytes = api.groupnorm_workspace(s.n, s.hw, s.c, s.g, x_type, 1);
   Tensor dx = need_dx ? at::empty(dy.sizes(), dy.options().dtype(type_of(x_type)).memory_format(c10::nullopt)) : Tensor();
   const Tensor w = work(dy, bytes);
-  done(api.groupnorm_act_backward(ptr(dy), code(dy), ptr(x), x_type, codes_ptr(packed.codes), exps_ptr(packed.exps), s.n, s.hw, s.c, s.g, ptr(weight),
-                                  ptr(bias), pc, (float)slope, reinterpret_cast<const double*>(ptr(stats)), out_ptr(dx), out_ptr(dweight),
-                                  out_ptr(dbias), gc, accumulate, out_ptr(w), bytes, stream_of(dy)), "sg2im_groupnorm_act_backward");
+  launch("sg2im_groupnorm_act_backward", "hbm_group_norm_bwd", dy.numel() * (dy.element_size() + (x.defined() ? x.element_size() : 33.0 / 32) + (need_dx ? dx.element_size() : 0.0)), dy, [&](hipStream_t stream) {
+    return api.groupnorm_act_backward(ptr(dy), code(dy), ptr(x), x_type, codes_ptr(packed.codes), exps_ptr(packed.exps), s.n, s.hw, s.c, s.g, ptr(weight),
+         ptr(bias), pc, (float)slope, reinterpret_cast<const double*>(ptr(stats)), out_ptr(dx), out_ptr(dweight),
+         out_ptr(dbias), gc, accumulate, out_ptr(w), bytes, stream);
+  });
   return dx;
 }
 
@@ -354,8 +392,10 @@ std::tuple<Tensor, Tensor> lin_forward(const Tensor& x, const Tensor& weight, co
   if (want_signs) signs = at::empty({r.rows, (N + 31) / 32}, x.options().dtype(at::kInt).memory_format(c10::nullopt));
   const size_t bytes = api.linear_workspace(r.rows, K, N, code(x), 0);
   const Tensor w = work(x, bytes);
-  done(api.linear_forward(ptr(r.m), code(x), r.ld, ptr(weight), ptr(bias), bc, ptr(res.m), res.ld, (float)slope, out_ptr(y), out_type, N,
-                          reinterpret_cast<unsigned*>(out_ptr(signs)), r.rows, K, N, out_ptr(w), bytes, stream_of(x)), "sg2im_linear_forward");
+  launch("sg2im_linear_forward", "igemm_fwd", 2.0 * r.rows * K * N, x, [&](hipStream_t stream) {
+    return api.linear_forward(ptr(r.m), code(x), r.ld, ptr(weight), ptr(bias), bc, ptr(res.m), res.ld, (float)slope, out_ptr(y), out_type, N,
+         reinterpret_cast<unsigned*>(out_ptr(signs)), r.rows, K, N, out_ptr(w), bytes, stream);
+  });
   return {y, signs};
 }
 
@@ -375,9 +415,10 @@ Tensor lin_backward_act(const Rows& dy, const Tensor& signs, double slope, int d
   if (dz_type >= 0) dz = at::empty({dy.rows, dy.cols}, dy.m.options().dtype(type_of(dz_type)).memory_format(c10::nullopt));
   const size_t bytes = api.linear_workspace(dy.rows, 1, N, 0, 3);
   const Tensor w = work(dy.m, bytes);
-  done(api.linear_backward_act(ptr(dy.m), code(dy.m), dy.ld, reinterpret_cast<const unsigned*>(ptr(signs)), (float)slope, out_ptr(dz),
-                               dz_type < 0 ? code(dy.m) : dz_type, out_ptr(dbias), bc, accumulate, dy.rows, N, out_ptr(w), bytes, stream_of(dy.m)),
-       "sg2im_linear_backward_act");
+  launch("sg2im_linear_backward_act", "hbm_linear_act_bwd", (double)dy.rows * N * (dy.m.element_size() + (dz.defined() ? dz.element_size() : 0.0)), dy.m, [&](hipStream_t stream) {
+    return api.linear_backward_act(ptr(dy.m), code(dy.m), dy.ld, reinterpret_cast<const unsigned*>(ptr(signs)), (float)slope, out_ptr(dz),
+         dz_type < 0 ? code(dy.m) : dz_type, out_ptr(dbias), bc, accumulate, dy.rows, N, out_ptr(w), bytes, stream);
+  });
   return dz;
 }
 
@@ -389,8 +430,9 @@ Tensor lin_backward_data(const Rows& dz, const Tensor& signs, double slope, cons
   Tensor dx = at::empty(shape, dz.m.options().memory_format(c10::nullopt));
   const size_t bytes = api.linear_workspace(dz.rows, K, N, code(dz.m), 1);
   const Tensor w = work(dz.m, bytes);
-  done(api.linear_backward_data(ptr(dz.m), code(dz.m), dz.ld, signs_ptr(signs), (float)slope, ptr(weight), out_ptr(dx), K, dz.rows, K, N, out_ptr(w), bytes, stream_of(dz.m)),
-       "sg2im_linear_backward_data");
+  launch("sg2im_linear_backward_data", "igemm_dgrad", 2.0 * dz.rows * K * N, dz.m, [&](hipStream_t stream) {
+    return api.linear_backward_data(ptr(dz.m), code(dz.m), dz.ld, signs_ptr(signs), (float)slope, ptr(weight), out_ptr(dx), K, dz.rows, K, N, out_ptr(w), bytes, stream);
+  });
   return dx;
 }
 
@@ -416,8 +458,10 @@ void lin_backward_weight(const Rows& dz, const Tensor& signs, double slope, cons
                     r.rows, " x ", r.cols, ", weight gradient ", dweight.scalar_type(), " ", dweight.sizes());
   const size_t bytes = api.linear_workspace(dz.rows, K, N, code(dz.m), 2);
   const Tensor w = work(dz.m, bytes);
-  done(api.linear_backward_weight(ptr(dz.m), code(dz.m), dz.ld, signs_ptr(signs), (float)slope, ptr(r.m), r.ld, codes_ptr(packed.codes),
-                                  exps_ptr(packed.exps), out_ptr(dweight), code(dweight), accumulate, out_ptr(dbias), bc, bias_accumulate, dz.rows, K, N, out_ptr(w), bytes, stream_of(dz.m)), "sg2im_linear_backward_weight");
+  launch("sg2im_linear_backward_weight", "igemm_wgrad", 2.0 * dz.rows * K * N, dz.m, [&](hipStream_t stream) {
+    return api.linear_backward_weight(ptr(dz.m), code(dz.m), dz.ld, signs_ptr(signs), (float)slope, ptr(r.m), r.ld, codes_ptr(packed.codes),
+         exps_ptr(packed.exps), out_ptr(dweight), code(dweight), accumulate, out_ptr(dbias), bc, bias_accumulate, dz.rows, K, N, out_ptr(w), bytes, stream);
+  });
 }
 
 struct LinearResidual : torch::autograd::Function<LinearResidual> {
@@ -497,6 +541,9 @@ Tensor linear_residual(const Tensor& x_, const Tensor& weight_, const MaybeTenso
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind", &bind);
+  m.def("observe", [](py::object f) { observer = f.release().ptr(); });
+  m.def("watch", [](bool on) { watched = on && observer; });
+  m.def("eager_launches", [] { return eager_launches.load(); });
   m.def("pack8", &pack8);
   m.def("unpack8", &unpack8);
   m.def("group_norm_act", &group_norm_act);

@@ -409,6 +409,22 @@ def _timed(kind, flops, fn, bn_finish=False, finish_bytes=0.0):
     TIMER.records.append((kind, flops, e0, e1, TIMER_TAG))
 
 
+def _native_timed(kind, amount, token):
+  """_timed for the launches of the host module (see _lib._observe): before them with token None, then with what that returned"""
+  if TIMER is None:
+    return None
+  if token is None:
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    e0.record()
+    return e0, e1
+  token[1].record()
+  TIMER.records.append((kind, amount, token[0], token[1], TIMER_TAG))
+
+
+_native_timed.active = lambda: TIMER is not None
+_lib.timed = _native_timed
+
+
 def _desc_k(desc):
   return desc.kh * desc.kw * sum(desc.src[i].channels for i in range(desc.nsrc))
 

@@ -682,14 +682,14 @@ class Trainer(object):
     Safety net: round 1 reported that an EAGER launch from this library after a graph was instantiated
     made the next replay of that graph fault; 26 probe variants in round 2 could not reproduce it
     (profiles/r2_graph_fault_probes.log), so it is NOT a known property of the runtime.  The check stays
-    because it is free on the training path: eager launches through the binding bump ``_lib.EAGER_EPOCH``
+    because it is free on the training path: eager launches through the binding move ``_lib.eager_epoch()``
     (captured ones do not); a graph whose epoch is stale is dropped and re-captured at its next use, so a
     validation pass between training steps costs one re-capture per bucket and nothing otherwise."""
     imgs, objs, masks, triples = batch[0], batch[1], batch[3], batch[4]
     o_pad, t_pad = self.bucketer.bucket(objs.numel(), triples.size(0))
     key = (o_pad, t_pad, tuple(imgs.shape), None if masks is None else (masks.dtype,) + tuple(masks.shape[1:]))
     if self._graphs:
-      stale = [k for k, e in self._graphs.items() if e[3] != _lib.EAGER_EPOCH]
+      stale = [k for k, e in self._graphs.items() if e[3] != _lib.eager_epoch()]
       for k in stale:                # the library ran eagerly since these were instantiated
         del self._graphs[k]
       self.graph_stats['invalidated'] += len(stale)
@@ -785,7 +785,7 @@ class Trainer(object):
     # zeroing - not counted): all / implicit-GEMM family incl. split-K finishes
     self.launch_stats = {'launches_per_step': int(lib.sg2im_launch_count(0) - n0),
                          'gemm_launches_per_step': int(lib.sg2im_launch_count(1) - g0)}
-    return (sb, graphs, st, _lib.EAGER_EPOCH)
+    return (sb, graphs, st, _lib.eager_epoch())
 
   def _generator_buckets(self):
     """the early buckets of the generator's gradient arena, see generator_buckets"""

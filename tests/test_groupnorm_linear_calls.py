@@ -211,3 +211,75 @@ def test_row_wise_batches(batch, channels, groups, dtype):
       want = times * f[name] + (tail[name] if rest else 0)
       tol = times * f[name + '_tol'] + (tail[name + '_tol'] if rest else 0)
       check(got, want, tol + (half_step(dtype) + u32) * want.abs(), name)
+
+
+# ---- launches are followed ------------------------------------------------------------------------------------------------
+
+def block():
+  """a group norm and a linear layer with everything trained: (call, leaves, gradient that comes in)"""
+  from sg2im_amd import functional as HF
+  g = torch.Generator(device='cuda').manual_seed(5)
+  r = lambda *s: torch.randn(*s, device='cuda', generator=g)  # noqa: E731
+  leaves = [t.requires_grad_(True) for t in (r(2, 4, 4, 32), r(32), r(32), r(48, 32), r(48))]
+
+  def call(x, gw, gb, w, b):
+    return HF.LinearResidual.apply(HF.GroupNormAct.apply(x, gw, gb, 4, 0.2, 1e-5, True), w, b, None, 0.2)
+  return call, leaves, r(2, 4, 4, 48)
+
+
+@gpu
+def test_eager_launches_are_counted_in_both_directions_and_captured_ones_are_not():
+  from sg2im_amd import _lib
+  call, leaves, dy = block()
+  seen = [_lib.eager_epoch()]
+  y = call(*leaves)
+  seen.append(_lib.eager_epoch())
+  torch.autograd.grad(y, leaves, dy)
+  seen.append(_lib.eager_epoch())
+  # (group norm and product; then at least dx, dW and the norm's pass)
+  assert seen[1] - seen[0] == 2 and seen[2] - seen[1] >= 3
+  del y
+  g = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(g):
+    torch.autograd.grad(call(*leaves), leaves, dy)
+  g.replay()
+  torch.cuda.synchronize()
+  assert _lib.eager_epoch() == seen[2]
+
+
+@gpu
+def test_launches_are_timed_by_kind():
+  from sg2im_amd import ops
+  call, leaves, dy = block()
+  want = [t.clone() for t in torch.autograd.grad(call(*leaves), leaves, dy)]
+  ops.TIMER, ops.TIMER_TAG = ops.KernelTimer(), 'mine'
+  try:
+    got = torch.autograd.grad(call(*leaves), leaves, dy)
+    ops.unpack8(ops.pack8(leaves[0].detach()))
+    s, tagged = ops.TIMER.summary(), ops.TIMER.summary('mine')
+  finally:
+    ops.TIMER = ops.TIMER_TAG = None
+  assert all(torch.equal(a, b) for a, b in zip(got, want)) and s == tagged
+  rows, k, n, e = 32, 32, 48, 2 * 4 * 4 * 32
+  for kind in ('igemm_fwd', 'igemm_dgrad', 'igemm_wgrad'):
+    assert s[kind]['launches'] == 1 and s[kind]['flops'] == 2.0 * rows * k * n, kind
+  bytes8 = e * 33 / 32
+  for kind, amount in (('hbm_group_norm_fwd', 8 * e + bytes8), ('hbm_group_norm_bwd', 8 * e + bytes8), ('hbm_pack8', 4 * e + bytes8),
+                       ('hbm_unpack8', 4 * e + bytes8)):
+    assert s[kind]['launches'] == 1 and s[kind]['flops'] == amount and s[kind]['ms'] > 0, kind
+  # and no longer, once nobody asks
+  torch.autograd.grad(call(*leaves), leaves, dy)
+
+
+@gpu
+def test_launches_are_printed_while_they_are_traced(monkeypatch, capfd):
+  from sg2im_amd import _lib
+  call, leaves, dy = block()
+  monkeypatch.setattr(_lib, '_TRACE', True)
+  torch.autograd.grad(call(*leaves), leaves, dy)
+  names = [l.split()[-1] for l in capfd.readouterr().err.splitlines() if l.startswith('[sg2im]')]
+  assert names[:2] == ['sg2im_groupnorm_act_forward', 'sg2im_linear_forward'] and names[-1] == 'sg2im_groupnorm_act_backward'
+  assert {'sg2im_linear_backward_data', 'sg2im_linear_backward_weight'} <= set(names)
+  monkeypatch.setattr(_lib, '_TRACE', False)
+  torch.autograd.grad(call(*leaves), leaves, dy)
+  assert '[sg2im]' not in capfd.readouterr().err
