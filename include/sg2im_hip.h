@@ -26,7 +26,7 @@ extern "C" {
 #define SG2IM_ERR_ARG 1   /* invalid argument (the reference would raise / assert) */
 #define SG2IM_ERR_HIP 2   /* a HIP runtime call failed; see hipGetLastError() */
 
-int sg2im_abi_version(void);   /* 12 (12: + group norm, linear with residual, 8-bit checkpoints; 11: + sg2im_csr_build_triples; 10: bfloat16 storage, weight mirror) */
+int sg2im_abi_version(void);   /* 13 (13: + sg2im_linear_plan; 12: + group norm, linear with residual, 8-bit checkpoints; 11: + sg2im_csr_build_triples; 10: bfloat16 storage, weight mirror) */
 
 /* Statistics: kernels this library has launched (or recorded into a stream capture) so far in this process;
  * which = 0: all of them, 1: the implicit-GEMM family incl. its split-K finishes.  bench.py reads it around the
@@ -714,6 +714,9 @@ int sg2im_unpack8(const signed char* codes, const unsigned char* exps, long long
 /* 1: backward_act first and plain products are the faster way for these sizes, 0: the products' own signs / dbias */
 int sg2im_linear_backward_act_first(long long rows, int k, int n, int dtype, int gated, int bias, int need_dx, int need_dw);
 size_t sg2im_linear_workspace(long long rows, int k, int n, int dtype, int which);
+/* which kernel a product takes (`which` = 0, 1, 2 as above; gated: signs are given, bias: dbias is): its square tile of 64, 128 or 256 - or
+ * 16: a small forward product in one launch - and into how many parts its reduction is split */
+int sg2im_linear_plan(long long rows, int k, int n, int dtype, int which, int gated, int bias, int* tile, int* splits);
 int sg2im_linear_forward(const void* x, int dtype, long long ld_x, const void* weight, const void* bias, int bias_dtype,
                          const void* residual, long long ld_res, float slope, void* out, int out_dtype, long long ld_out,
                          unsigned* signs, long long rows, int k, int n, void* workspace, size_t workspace_bytes,

@@ -181,6 +181,7 @@ _SIGNATURES = {
   'sg2im_unpack8': [_P, _P, _L, _I, _P, _I, _L, _P],
   'sg2im_linear_workspace': [_L, _I, _I, _I, _I],
   'sg2im_linear_backward_act_first': [_L, _I, _I, _I, _I, _I, _I, _I],
+  'sg2im_linear_plan': [_L, _I, _I, _I, _I, _I, _I, _P, _P],
   'sg2im_linear_forward': [_P, _I, _L, _P, _P, _I, _P, _L, _F, _P, _I, _L, _P, _L, _I, _I, _P, _Z, _P],
   'sg2im_linear_backward_act': [_P, _I, _L, _P, _F, _P, _I, _P, _I, _I, _L, _I, _P, _Z, _P],
   'sg2im_linear_backward_data': [_P, _I, _L, _P, _F, _P, _P, _L, _L, _I, _I, _P, _Z, _P],

@@ -222,6 +222,13 @@ bool short_form(long long I, long long J, long long R, int bf16, const Plan& q) 
   return R >= (bf16 ? 8 : 4) && us < q.us + (bf16 ? 3.0 : 3.5) && tiles < 65536;   // (a lane's 16 bytes have to fit in a row)
 }
 
+// which: 0 forward, 1 dx, 2 dW, as in the workspace query; gated, summed: Product's fields
+Plan plan_of(int which, long long rows, int k, int n, int dtype, bool gated, bool summed) {
+  if (which == 0) return plan(0, rows, n, k, dtype);
+  if (which == 1) return plan(1, rows, k, n, dtype, gated ? GATED[dtype] : 0.0);
+  return plan(2, n, k, std::max(1LL, rows), dtype, gated ? GATED[dtype] : summed ? SUMMED[dtype] : 0.0);      // (no row: one empty sum, zeros or what was there)
+}
+
 ActParams act_plan(long long rows, int n) {
   ActParams p = {};
   p.M = rows; p.N = n;
@@ -246,10 +253,10 @@ extern "C" {
 size_t sg2im_linear_workspace(long long rows, int k, int n, int dtype, int which) {
   if (!sizes_ok(rows, k, n) || !type_ok(dtype) || rows == 0) return 16;
   if (which == 3) return std::max((size_t)16, (size_t)act_plan(rows, n).chunks * n * 4);
-  if (which == 0) return plan_bytes(plan(0, rows, n, k, dtype), rows, n, false);
-  if (which == 1) return std::max(plan_bytes(plan(1, rows, k, n, dtype), rows, k, false), plan_bytes(plan(1, rows, k, n, dtype, GATED[dtype]), rows, k, false));
-  return std::max({plan_bytes(plan(2, n, k, rows, dtype), n, k, false), plan_bytes(plan(2, n, k, rows, dtype, GATED[dtype]), n, k, true),
-                   plan_bytes(plan(2, n, k, rows, dtype, SUMMED[dtype]), n, k, true)});
+  const auto form = [&](bool gated, bool summed) { return plan_of(which, rows, k, n, dtype, gated, summed); };
+  if (which == 0) return plan_bytes(form(false, false), rows, n, false);
+  if (which == 1) return std::max(plan_bytes(form(false, false), rows, k, false), plan_bytes(form(true, false), rows, k, false));
+  return std::max({plan_bytes(form(false, false), n, k, false), plan_bytes(form(true, true), n, k, true), plan_bytes(form(false, true), n, k, true)});
 }
 
 int sg2im_linear_backward_act_first(long long rows, int k, int n, int dtype, int gated, int bias, int need_dx, int need_dw) {
@@ -258,12 +265,19 @@ int sg2im_linear_backward_act_first(long long rows, int k, int n, int dtype, int
   // one pass over dy (and dz to memory) at 4.5 TB/s and its last sum, then plain products; or products that do it themselves
   const double es = dtype ? 2 : 4;
   double first = 8.0 + es * rows * n * (gated ? 2 : 1) / 4.5e6, itself = 0.0;
-  if (need_dx && gated) { first += plan(1, rows, k, n, dtype).us; itself += plan(1, rows, k, n, dtype, GATED[dtype]).us; }
-  if (need_dw) {
-    first += plan(2, n, k, rows, dtype).us;
-    itself += plan(2, n, k, rows, dtype, gated ? GATED[dtype] : SUMMED[dtype]).us;
-  }
+  const auto us = [&](int which, bool by_itself) { return plan_of(which, rows, k, n, dtype, by_itself && gated, by_itself).us; };
+  if (need_dx && gated) { first += us(1, false); itself += us(1, true); }
+  if (need_dw) { first += us(2, false); itself += us(2, true); }
   return first < itself;
+}
+
+int sg2im_linear_plan(long long rows, int k, int n, int dtype, int which, int gated, int bias, int* tile, int* splits) {
+  if (!sizes_ok(rows, k, n) || rows == 0 || !type_ok(dtype) || which < 0 || which > 2 || !tile || !splits) return SG2IM_ERR_ARG;
+  const Plan q = plan_of(which, rows, k, n, dtype, gated != 0, bias != 0);
+  const bool small = which == 0 && short_form(rows, n, k, dtype, q);
+  *tile = small ? 16 : q.tile;
+  *splits = small ? 1 : q.splits;
+  return SG2IM_OK;
 }
 
 int sg2im_linear_forward(const void* x, int dtype, long long ld_x, const void* weight, const void* bias, int bias_dtype,
@@ -278,7 +292,7 @@ int sg2im_linear_forward(const void* x, int dtype, long long ld_x, const void* w
   p.a = x; p.lda = ld_x; p.b = weight; p.ldb = k; p.I = (int)rows; p.J = n; p.R = k;
   p.bias = bias; p.bias_bf16 = bias_dtype; p.residual = residual; p.ld_res = ld_res; p.slope = slope;
   p.signs = signs; p.sign_words = (n + 31) / 32; p.out = out; p.out_bf16 = out_dtype; p.ld_out = ld_out;
-  const Plan q = plan(0, rows, n, k, dtype);
+  const Plan q = plan_of(0, rows, k, n, dtype, false, false);
   if (short_form(rows, n, k, dtype, q)) return dtype == 0 ? run_short<float>(p, stream) : run_short<bf16_s>(p, stream);
   return dtype == 0 ? run<float, RC, RC, false, false>(p, q, workspace, workspace_bytes, stream)
                     : run<bf16_s, RC, RC, false, false>(p, q, workspace, workspace_bytes, stream);
@@ -316,7 +330,7 @@ int sg2im_linear_backward_data(const void* dz, int dtype, long long ld_dz, const
   p.a = dz; p.lda = ld_dz; p.b = weight; p.ldb = k; p.I = (int)rows; p.J = k; p.R = n;
   p.slope = 1.f; p.out = dx; p.out_bf16 = dtype; p.ld_out = ld_dx;
   p.gate = reinterpret_cast<const unsigned char*>(signs); p.gate_ld = (n + 31) / 32 * 4LL; p.gate_slope = slope;
-  const Plan q = plan(1, rows, k, n, dtype, signs ? GATED[dtype] : 0.0);
+  const Plan q = plan_of(1, rows, k, n, dtype, signs != nullptr, false);
   if (signs) return dtype == 0 ? run<float, RC, RM, true, false>(p, q, workspace, workspace_bytes, stream)
                                : run<bf16_s, RC, RM, true, false>(p, q, workspace, workspace_bytes, stream);
   return dtype == 0 ? run<float, RC, RM, false, false>(p, q, workspace, workspace_bytes, stream)
@@ -337,7 +351,7 @@ int sg2im_linear_backward_weight(const void* dz, int dtype, long long ld_dz, con
   p.sum = dbias; p.sum_bf16 = bias_dtype; p.sum_accumulate = bias_accumulate;
   if (codes) { p.b = codes; p.ldb = k; p.b_exps = exps; p.b_nblk = (k + C8_BLOCK - 1) / C8_BLOCK; }
   else { p.b = x; p.ldb = ld_x; }
-  const Plan q = plan(2, n, k, std::max(1LL, rows), dtype, signs ? GATED[dtype] : dbias ? SUMMED[dtype] : 0.0);   // (no row: one empty sum, zeros or what was there)
+  const Plan q = plan_of(2, rows, k, n, dtype, signs != nullptr, dbias != nullptr);
   return run_weight(p, dtype, codes != nullptr, q, workspace, workspace_bytes, stream);
 }
 
