@@ -670,7 +670,9 @@ int sg2im_adam_apply_guarded(float* param, const float* grad, float* exp_avg, fl
  *             codes / exps (both or neither): the 8-bit form of x is written too (sg2im_pack8).
  *   backward: from x, or - codes / exps given - from its 8-bit form; dy has out's type, dx has x_dtype.  dx, dgamma, dbeta may
  *             be NULL.  accumulate: dgamma / dbeta += .  The side of the LeakyReLU is decided in 64 bits where the
- *             32-bit value is within its rounding of zero; at exactly zero the gradient takes `slope`.
+ *             32-bit value is within its rounding of zero; at exactly zero the gradient takes `slope`.  From the 8-bit form:
+ *             xh = (rounded x - mean) * rstd with x's own mean and rstd, and the rounded value's side - which within half a
+ *             step of the kink may be another than the forward pass took.  An approximation of the gradient.
  * workspace: sg2im_groupnorm_workspace bytes, 16-byte aligned, used by this call only.  No alignment beyond an element's is
  * assumed of the tensors.  Statistics are summed in 64 bits, in a fixed order: the same call gives the same bits.
  * Any batch is taken: where one launch does not hold it, several do.  SG2IM_ERR_ARG: channels % groups, hw < 1 or >= 2^30,

@@ -1474,7 +1474,9 @@ class InstNormAct(Function):
 class GroupNormAct(object):
   """leaky_slope(group_norm(x)) of a channels-last map x (N, ..., C), float32 or bfloat16 (statistics in 64 bits):
   C / groups channels and all pixels of an image share a mean and a (biased) variance.  weight / bias: (C,) vectors of one
-  type, or None.  checkpoint8: the backward pass keeps x in 8 bits (ops.pack8) and is computed from that.
+  type, or None.  checkpoint8: the backward pass keeps x in 8 bits (ops.pack8) and evaluates the gradient's formula on that, with
+  the statistics of x itself: an approximation of the gradient.  An element within half an 8-bit step of the LeakyReLU's kink may
+  take the other side's slope there.
   out_dtype: x's type (None), or torch.bfloat16.  The autograd node is native (csrc/native.cpp); parameters with a
   registered gradient sink get their gradient there, as everywhere in this module."""
 

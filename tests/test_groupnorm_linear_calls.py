@@ -283,3 +283,40 @@ def test_launches_are_printed_while_they_are_traced(monkeypatch, capfd):
   monkeypatch.setattr(_lib, '_TRACE', False)
   torch.autograd.grad(call(*leaves), leaves, dy)
   assert '[sg2im]' not in capfd.readouterr().err
+
+
+# ---- sides of the kink ------------------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize('pack', [False, True])
+@pytest.mark.parametrize('channels', [512, 2048, 100])
+def test_which_side_of_the_kink_the_backward_pass_takes(channels, pack):
+  """slope 0 and a gradient of 2^p at pixel p: the bits of dbias are the sides.  From x they are the forward pass'; from the
+  8-bit form they are those of its values, so an element within half a step of the kink may be on the other one."""
+  from sg2im_amd import ops
+  from tests.test_groupnorm_linear_ckpt8 import eight, gen
+  r = gen(channels)
+  x, w, b, groups = r(1, 4, 4, channels), 1 + 0.2 * r(channels), 0.2 * r(channels), 4
+  dy = (2.0 ** torch.arange(16, device='cuda')).view(1, 4, 4, 1).expand(1, 4, 4, channels).contiguous()
+  y, stats, packed = ops.group_norm_act_forward(x, w, b, groups, 0.0, 1e-5, pack=pack)
+  db = torch.empty(channels, device='cuda')
+  ops.group_norm_act_backward(dy, packed if pack else x, w, b, groups, 0.0, stats, True, None, db)
+  got = (db.long().view(1, -1) >> torch.arange(16, device='cuda').view(16, 1) & 1).bool()
+  D = channels // groups
+  xd, (seen, exps) = x.double().view(16, channels), eight(x)
+  per = xd.view(16, groups, D)
+  mean, rstd = per.mean((0, 2)), (per.var((0, 2), unbiased=False) + 1e-5).rsqrt()
+  spread = lambda v: v.repeat_interleave(D).view(1, channels)  # noqa: E731
+  z = lambda v: (v - spread(mean)) * spread(rstd) * w.double() + b.double()  # noqa: E731
+  forward = y.view(16, channels) > 0
+  assert torch.equal(forward, z(xd) > 0)
+  if not pack:
+    assert torch.equal(got, forward)
+    return
+  assert torch.equal(got, z(seen.view(16, channels)) > 0)
+  half_step = torch.pow(2.0, exps.double().view(16, -1) - 128).repeat_interleave(32, 1)[:, :channels]
+  near = z(xd).abs() <= half_step * spread(rstd) * w.double().abs() * (1 + 1e-12)
+  other = got != forward
+  assert not bool((other & ~near).any())
+  if channels > 100:
+    assert bool(other.any())                        # (it does happen: the two passes are not one function's)
