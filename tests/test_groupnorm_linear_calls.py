@@ -285,7 +285,34 @@ def test_launches_are_printed_while_they_are_traced(monkeypatch, capfd):
   assert '[sg2im]' not in capfd.readouterr().err
 
 
-# ---- sides of the kink ------------------------------------------------------------------------------------------------------
+# ---- maps larger than the caches; sides of the kink -------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('pack', [False, True])
+def test_group_norm_beyond_the_caches(pack, dtype, monkeypatch):
+  """x and dy of 400 - 550 MB, from 32 times one image: every image like the first, that one against 64 bits, the parameters'
+  gradients against 32 times its sums.  A thread adds up rows / 32 chunks / 32 pixel lanes (16 float) in float32 before they
+  are joined in 64 bits: 64 (128) values."""
+  from sg2im_amd import ops
+  from tests import test_groupnorm_linear_ckpt8 as base
+  monkeypatch.setattr(base, 'T', 64 if dtype == BF16 else 128)
+  r = base.gen(60)
+  n, shape, groups = 32, (1, 256, 256, 64), 8
+  one, d = (2 * r(*shape) + r(64)).to(dtype), r(*shape).to(dtype)
+  w, b = (1 + 0.2 * r(64)).to(dtype), (0.2 * r(64)).to(dtype)
+  x, dy = one.expand(n, -1, -1, -1).contiguous(), d.expand(n, -1, -1, -1).contiguous()
+  y, stats, packed = ops.group_norm_act_forward(x, w, b, groups, 0.2, 1e-5, pack=pack)
+  dw, db = torch.empty(64, device='cuda', dtype=dtype), torch.empty(64, device='cuda', dtype=dtype)
+  dx = ops.group_norm_act_backward(dy, packed if pack else x, w, b, groups, 0.2, stats, True, dw, db)
+  assert torch.equal(y, y[:1].expand_as(y)) and torch.equal(dx, dx[:1].expand_as(dx)) and torch.equal(stats, stats[:1].expand_as(stats))
+  f = base.gn_reference(one, base.eight(one)[0] if pack else one, w, b, groups, 0.2, 1e-5, d)
+  half = base.half_step(dtype)
+  base.check(y[:1], f['y'], f['y_tol'] + half * f['y'].abs(), 'y')
+  base.check(dx[:1], f['dx'], f['dx_tol'] + half * f['dx'].abs(), 'dx')
+  base.check(dw, n * f['dw'], n * f['dw_tol'] + (half + base.u32) * n * f['dw'].abs(), 'dweight')
+  base.check(db, n * f['db'], n * f['db_tol'] + (half + base.u32) * n * f['db'].abs(), 'dbias')
+
 
 @gpu
 @pytest.mark.parametrize('pack', [False, True])
