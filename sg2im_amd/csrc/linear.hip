@@ -4,7 +4,8 @@
 //   dz = dy (z > 0 ? 1 : slope),  dresidual = dy,  db = sum_m dz
 //   dx = dz W,   dW = dz^T x        (x, or its 8-bit form)
 //
-// The forward pass keeps one bit per element, z > 0, for the backward pass.
+// The forward pass keeps one bit per element, z > 0, for the backward pass.  Next to a bfloat16 x the backward products take dz in
+// bfloat16 (a matrix operand is; linear.h at the gate says what that costs), db sums it unrounded.
 //
 // The products are linear.h's.
 #define SG2IM_GEMM_TU 1

@@ -1491,7 +1491,8 @@ class GroupNormAct(object):
 
 class LinearResidual(object):
   """y = leaky_slope(x W^T + b) + residual for x (..., K), W (N, K); float32, or bfloat16 operands with float32
-  accumulation.  W has x's type, or is float32 next to a bfloat16 x (it is rounded for the product; its gradient is
+  accumulation.  The backward products of a bfloat16 x take dz = dy leaky'(z), and a float32 dy, rounded to bfloat16; the
+  bias gradient sums dz unrounded.  W has x's type, or is float32 next to a bfloat16 x (it is rounded for the product; its gradient is
   float32).  bias (N,) and residual (..., N) may be None; the residual has the output's type and shape.  checkpoint8: the
   weight's gradient is computed from x in 8 bits (ops.pack8), which is what the backward pass keeps of x.  out_dtype: x's
   type (None), or torch.float32."""
