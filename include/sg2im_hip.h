@@ -712,7 +712,9 @@ int sg2im_unpack8(const signed char* codes, const unsigned char* exps, long long
  *                     `dtype`, is formed on its way into the product (the same numbers as backward_act's).
  * workspace: sg2im_linear_workspace bytes for `which` = 0 forward, 1 backward_data, 2 backward_weight, 3 backward_act.
  * Rows below 2^31 - 256; k, n and the operands' leading dimensions (in elements) at most 2^22; no alignment
- * beyond an element's is assumed (workspace: 16 bytes).  Fixed summation orders: the same call gives the same bits. */
+ * beyond an element's is assumed (workspace: 16 bytes).  A bfloat16 x or weight of the forward product whose rows start in the middle of a
+ * 4-byte word may be read by whole words, that is by one element before and behind it, inside words that hold some of it; what
+ * lies there does not count.  Fixed summation orders: the same call gives the same bits. */
 /* 1: backward_act first and plain products are the faster way for these sizes, 0: the products' own signs / dbias */
 int sg2im_linear_backward_act_first(long long rows, int k, int n, int dtype, int gated, int bias, int need_dx, int need_dw);
 size_t sg2im_linear_workspace(long long rows, int k, int n, int dtype, int which);

@@ -146,10 +146,9 @@ __device__ __forceinline__ float load1_bf(const ConvGeom& g, const Src& S, bool 
 // instead of compare + multiply + select, bit-identical (v > 0: v * slope <= v; v < 0: v * slope >= v)
 __device__ __forceinline__ float leaky01(float v, float slope) { return __builtin_fmaxf(v, v * slope); }
 
-// Pending affine + LeakyReLU + validity mask of one float4, on the packed-fp32 VALU (v_pk_fma_f32 /
-// v_pk_mul_f32: two lanes of work per instruction): 2 fma + 2 mul + 4 max + 2 mul(mask) instead of
-// 4 + 4 + 4 + 4 selects.  The mask is a multiplication by 0 / 1 (the masked-off load fetched element 0
-// of its tensor, finite).
+// Pending affine + LeakyReLU + validity mask of one float4, written on pairs: 4 fma + 4 mul + 4 max + 4 mul(mask).  (Packed fp32
+// instructions would take the pairs two at a time; they are switched off for every file.)  The mask is a multiplication by 0 / 1
+// (the masked-off load fetched element 0 of its tensor, finite).
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float4 apply_aff(float4 v, const Aff& a, bool ok) {
   const f32x2 mk = ok ? f32x2{1.f, 1.f} : f32x2{0.f, 0.f};
