@@ -31,7 +31,7 @@ def build_native(force=False, verbose=True):
   """lib/sg2im_native.so with the host compiler (csrc/native.cpp holds no device code)"""
   import sysconfig
   src = os.path.join(CSRC, 'native.cpp')
-  if not (force or _stale(NATIVE, [src, os.path.join(ROOT, 'include', 'sg2im_hip.h')])):
+  if not (force or _stale(NATIVE, [src, os.path.join(ROOT, 'include', 'sg2im_hip.h'), os.path.abspath(__file__)])):
     return None
   import torch
   inc = os.path.join(os.path.dirname(torch.__file__), 'include')
@@ -52,7 +52,7 @@ def build(force=False, verbose=True, cflags=(), tag=''):
   os.makedirs(LIBDIR, exist_ok=True)
   lib_path = LIB.replace('.so', tag + '.so')
   headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith('.h')]
-  headers.append(os.path.join(ROOT, 'include', 'sg2im_hip.h'))
+  headers += [os.path.join(ROOT, 'include', 'sg2im_hip.h'), os.path.abspath(__file__)]      # (the flags are here)
   objs, procs = [], []
   for src in SOURCES:
     sp = os.path.join(CSRC, src)
