@@ -322,9 +322,9 @@ __device__ __forceinline__ void write_codes(const Params& p, int n, int row, int
 }
 
 // Statistics of the groups that the slab's channels [c0, c0 + width) belong to, from the chunks' sums, into st[group][2];
-// returns the first group.  A group that reaches over a slab's border is joined by two slabs: in the same order, since how many
-// threads share a sum goes by the widest slab, and written by the one that holds its first channel.  Every workgroup of an image does it over again: a few KB from the L2 against a launch of its own
-// between the two passes (32 x 64 x 64 x 64 float 24.4 -> 21.7 us, 32 x 128 x 128 x 64 72 -> 69).
+// returns the first group.  Every workgroup of an image does it over again: a few KB from the L2 against a launch of its own
+// between the two passes (figures where it is chosen).  A group that reaches over a slab's border is joined by both slabs - in
+// the same order, since how many threads share a sum goes by the widest slab - and written by the one that holds its first channel.
 constexpr int MERGE_SPAN = 512;
 __device__ __forceinline__ int merged_stats(const Params& p, const Place& w, int c0, int width, double* st) {
   __shared__ double red[2 * MERGE_SPAN];
@@ -1125,8 +1125,12 @@ void launch_forward(const Params& p0, hipStream_t stream) {
   over_images<TX, char, TY, double>(p, per_image, THREADS, [&](const Params& s, long long images, bool) {
     SG2IM_LAUNCH(fwd_partial_kernel<TX>, dim3((unsigned)(images * per_image)), dim3(THREADS), 0, stream, s);
   });
-  // (a slab's groups reach over it by less than a group on either side)
-  p.merged = p.L == p.C && p.chunks <= 64 && p.TV * VecOf<TX>::n + 2 * (p.D - 1) <= MERGE_SPAN && (p.TV * VecOf<TX>::n + 2 * p.D) * p.chunks <= 16384;
+  // A finish launch, or its work in every workgroup of the normalising pass: by the sums that such a workgroup would join (a
+  // slab's groups reach over it by less than a group on either side).  Forward, microseconds, with the launch / without, groups in
+  // 32: 544 sums 64 x 64 x 64 x 32 float 20.6 / 18.2; 1088 64 x 32 x 32 x 64 float 15.6 / 12.6; 2176 32 x 64 x 64 x 64 float 21.4 / 19.6,
+  // bfloat16 17.9 / 15.9; 4352 32 x 32 x 32 x 128 float 15.8 / 17.3, 32 x 64 x 64 x 128 float 38.7 / 38.1; 8704 32 x 32 x 32 x 256 float
+  // 22.7 / 25.6, 16 x 64 x 64 x 128 bfloat16 19.4 / 23.5; 17408 16 x 32 x 32 x 256 float 17.3 / 29.4.
+  p.merged = p.L == p.C && p.chunks <= 64 && p.TV * VecOf<TX>::n + 2 * (p.D - 1) <= MERGE_SPAN && (p.TV * VecOf<TX>::n + 2 * p.D) * p.chunks <= 4096;
   if (p.merged) p.span = slab_span(p, p.TV * VecOf<TX>::n);
   const int threads = finish_threads(p);
   if (!p.merged)

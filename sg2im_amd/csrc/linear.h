@@ -734,6 +734,9 @@ int run(Product& p, const Plan& q, void* workspace, size_t workspace_bytes, hipS
   if (q.tile == 64) SG2IM_LAUNCH((product_kernel<T, 64, 64, 256, AMODE, BMODE, GATE, SUM, true>), grid, dim3(256), 0, stream, p);
   if (q.splits > 1) {
     const long long pieces = (long long)p.I * ((p.J + 31) / 32) * 8;
+    // Eight threads to a piece where there are splits for each of them and too few pieces to fill the card.  dW with its join, microseconds,
+    // one thread / eight: 128 splits of 1024 pieces (65536 x 64 -> 64 bfloat16) 44.1 / 13.1, 128 of 4096 49.8 / 23.2, 32 of 16384 24.4 / 17.9,
+    // 8 of 24720 15.7 / 12.4; 16 of 65536 39.3 / 38.7; 4 of 262144 92 / 98, 3 of 147456 (float) 47.8 / 50.5.
     if (q.splits >= 8 && pieces < 1 << 16) SG2IM_LAUNCH(join_kernel<8>, dim3((unsigned)((pieces + 31) / 32)), dim3(THREADS), 0, stream, p);
     else SG2IM_LAUNCH(join_kernel<1>, dim3((unsigned)std::min((pieces + THREADS - 1) / THREADS, 1LL << 20)), dim3(THREADS), 0, stream, p);
   }

@@ -132,16 +132,17 @@ CROSSING = [(1600, 32, F32), (1632, 32, F32), (1824, 32, F32), (1856, 32, F32), 
 
 
 @gpu
+@pytest.mark.parametrize('images', [4, 32])             # (32: few sums per image, joined by the normalising pass itself)
 @pytest.mark.parametrize('channels,groups,dtype', CROSSING)
-def test_groups_that_cross_workgroups_have_one_statistic(channels, groups, dtype):
+def test_groups_that_cross_workgroups_have_one_statistic(channels, groups, dtype, images):
   """every group holds the same numbers: its statistics, and what is normalised with them, have to be the same bits whichever
   workgroup joined the sums; and the same call gives the same bits"""
   from sg2im_amd import ops
   g = torch.Generator(device='cuda').manual_seed(channels)
   D = channels // groups
-  one = (torch.randn(4, 32, 32, D, device='cuda', generator=g) * 3 + 1).to(dtype)
+  one = (torch.randn(images, 32, 32, D, device='cuda', generator=g) * 3 + 1).to(dtype)
   x = one.repeat(1, 1, 1, groups)
-  dy = torch.randn(4, 32, 32, channels, device='cuda', generator=g).to(dtype)
+  dy = torch.randn(images, 32, 32, channels, device='cuda', generator=g).to(dtype)
   first = None
   for _ in range(8):
     y, stats, _ = ops.group_norm_act_forward(x, None, None, groups, 0.2, 1e-5)
