@@ -106,6 +106,8 @@ void on_device(const Tensor& t, const char* what) {
   TORCH_CHECK_VALUE(!t.is_neg(), what, ": a view whose negation is pending (resolve_neg() makes it a tensor)");
   TORCH_CHECK_VALUE(t.device() == gpu().getDevice(), what, " lies on ", t.device(), " but the current device is ", gpu().getDevice());
 }
+// (a view whose negation is pending holds the numbers before it)
+Tensor settled(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 Tensor given(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
 
 // These calls read and write memory below torch's dispatcher, so what follows operators there does not see them: a forward
@@ -190,7 +192,7 @@ Packed pack(const Tensor& x) {
 }
 std::tuple<Tensor, Tensor> pack8(const Tensor& x) {
   eager_only("pack8", {x});
-  const Packed p = pack(x.resolve_neg());
+  const Packed p = pack(settled(x));
   return {p.codes, p.exps};
 }
 
@@ -320,7 +322,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
     // one launch adds to both or writes both: a sink next to a parameter without one is added to afterwards
     const bool all = (!nw || sw.defined()) && (!nb || sb.defined());
     const Target tw(nw, s[3], all ? sw : Tensor()), tb(nb, s[4], all ? sb : Tensor());
-    const Tensor dx = gn_backward(grads[0].resolve_neg().contiguous(), s[0], Packed{s[1], s[2]}, (int)ctx->saved_data["type"].toInt(), s[3], s[4],
+    const Tensor dx = gn_backward(settled(grads[0]).contiguous(), s[0], Packed{s[1], s[2]}, (int)ctx->saved_data["type"].toInt(), s[3], s[4],
                                   ctx->saved_data["groups"].toInt(), ctx->saved_data["slope"].toDouble(), s[5], ctx->needs_input_grad(0),
                                   tw.buf, tb.buf, all);
     Tensor dw = tw.grad(), db = tb.grad();
@@ -354,10 +356,10 @@ Tensor group_norm_act(const Tensor& x, const MaybeTensor& weight, const MaybeTen
   const Tensor w = given(weight), b = given(bias);
   eager_only("group norm", {x, w, b});
   if (!(at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))))
-    return gn_forward(x.resolve_neg().contiguous(), w, b, groups, slope, eps, (int)out_type, false).y;
+    return gn_forward(settled(x).contiguous(), w, b, groups, slope, eps, (int)out_type, false).y;
   const Sinks sinks{given(sink_w), given(sink_b)};
   check_capture({{&x, nullptr}, {&w, &sinks.w}, {&b, &sinks.b}});
-  return GroupNormAct::apply(x.resolve_neg().contiguous(), maybe(w), maybe(b), groups, slope, eps, checkpoint8, out_type, &sinks);
+  return GroupNormAct::apply(settled(x).contiguous(), maybe(w), maybe(b), groups, slope, eps, checkpoint8, out_type, &sinks);
 }
 
 // ---- linear + activation + residual -----------------------------------------------------------------------------------
@@ -491,7 +493,7 @@ struct LinearResidual : torch::autograd::Function<LinearResidual> {
     const Tensor& signs = s[6];
     Tensor dx, dw, db;
     if (nx || nw || nb) {
-      const Tensor given_dy = grads[0].resolve_neg();
+      const Tensor given_dy = settled(grads[0]);
       on_device(given_dy, "linear gradient");
       const Rows dy = rows_of(given_dy, "linear gradient");
       const double slope = ctx->saved_data["slope"].toDouble();
@@ -526,7 +528,7 @@ Tensor linear_residual(const Tensor& x_, const Tensor& weight_, const MaybeTenso
   const Tensor b = given(bias);
   Tensor x = x_, weight = weight_, r = given(residual);
   eager_only("linear", {x, weight, b, r});
-  for (Tensor* t : {&x, &weight, &r}) if (t->defined() && t->is_neg()) *t = t->resolve_neg();
+  for (Tensor* t : {&x, &weight, &r}) if (t->defined()) *t = settled(*t);
   if (!(at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(b) || wants(r)))) {
     Tensor w = weight.contiguous();
     if (is_bf16(x) && w.scalar_type() == at::kFloat) w = w.to(at::kBFloat16);
