@@ -264,7 +264,8 @@ def eager_epoch():
   return EAGER_EPOCH + (_native.eager_launches() if _native is not None else 0)
 
 
-timed = None         # ops._native_timed: times the host module's launches
+timed = None         # ops._native_timed: times the host module's launches ...
+timer = {}           # ... while its module's TIMER (this is that module's dictionary) is not None
 _watching = False
 
 
@@ -285,7 +286,7 @@ def eager():
   """the host module, for a call that launches; watched while launches are traced or timed"""
   global _watching
   mod = _native or native()
-  watch = _TRACE or (timed is not None and timed.active())
+  watch = _TRACE or timer.get('TIMER') is not None
   if watch is not _watching:
     mod.watch(watch)
     _watching = watch

@@ -1128,9 +1128,10 @@ void launch_forward(const Params& p0, hipStream_t stream) {
   // A finish launch, or its work in every workgroup of the normalising pass: by the sums that such a workgroup would join (a
   // slab's groups reach over it by less than a group on either side).  Forward, microseconds, with the launch / without, groups in
   // 32: 544 sums 64 x 64 x 64 x 32 float 20.6 / 18.2; 1088 64 x 32 x 32 x 64 float 15.6 / 12.6; 2176 32 x 64 x 64 x 64 float 21.4 / 19.6,
-  // bfloat16 17.9 / 15.9; 4352 32 x 32 x 32 x 128 float 15.8 / 17.3, 32 x 64 x 64 x 128 float 38.7 / 38.1; 8704 32 x 32 x 32 x 256 float
-  // 22.7 / 25.6, 16 x 64 x 64 x 128 bfloat16 19.4 / 23.5; 17408 16 x 32 x 32 x 256 float 17.3 / 29.4.
-  p.merged = p.L == p.C && p.chunks <= 64 && p.TV * VecOf<TX>::n + 2 * (p.D - 1) <= MERGE_SPAN && (p.TV * VecOf<TX>::n + 2 * p.D) * p.chunks <= 4096;
+  // bfloat16 17.9 / 15.9; 4352 (14 maps: 0.91 - 1.09, 0.99 on average) 16 x 128 x 128 x 64 bfloat16 23.7 / 22.6, 32 x 32 x 32 x 128 float
+  // 15.8 / 17.3; 8704 32 x 32 x 32 x 256 float 22.7 / 25.6, 16 x 64 x 64 x 128 bfloat16 19.4 / 23.5; 17408 16 x 32 x 32 x 256 float 17.3 / 29.4.
+  // (Where the host issues slower than the card works, the launch costs another 2 - 3.)
+  p.merged = p.L == p.C && p.chunks <= 64 && p.TV * VecOf<TX>::n + 2 * (p.D - 1) <= MERGE_SPAN && (p.TV * VecOf<TX>::n + 2 * p.D) * p.chunks <= 4608;
   if (p.merged) p.span = slab_span(p, p.TV * VecOf<TX>::n);
   const int threads = finish_threads(p);
   if (!p.merged)

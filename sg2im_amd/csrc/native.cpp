@@ -113,12 +113,12 @@ Tensor given(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
 // These calls read and write memory below torch's dispatcher, so what follows operators there does not see them: a forward
 // gradient would come back as none, that is as a derivative of zero, and a recorded program would hold the empty outputs and
 // nothing that fills them.  Both are refused, before anything else is looked at.
-void eager_only(const char* what, std::initializer_list<Tensor> tensors) {
+void eager_only(const char* what, std::initializer_list<const Tensor*> tensors) {
   TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() &&
                               !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
                               what, ": called while torch.jit.trace or make_fx records, which would not see it");
-  for (const Tensor& t : tensors)
-    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(),
+  for (const Tensor* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
                                 what, ": no forward-mode derivative (an argument carries a forward gradient)");
 }
 const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -191,7 +191,7 @@ Packed pack(const Tensor& x) {
   return p;
 }
 std::tuple<Tensor, Tensor> pack8(const Tensor& x) {
-  eager_only("pack8", {x});
+  eager_only("pack8", {&x});
   const Packed p = pack(settled(x));
   return {p.codes, p.exps};
 }
@@ -284,7 +284,7 @@ struct Target {
 
 void once(const char* what, const Tensor& grad) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "this operator has no second derivative (create_graph=True reached its backward pass)");
-  eager_only(what, {grad});
+  eager_only(what, {&grad});
 }
 
 // the registered gradient buffers of a layer's two parameters (undefined: none); autograd does not see them
@@ -354,7 +354,7 @@ void check_capture(std::initializer_list<std::pair<const Tensor*, const Tensor*>
 Tensor group_norm_act(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, int64_t groups, double slope, double eps, bool checkpoint8,
                       int64_t out_type, const MaybeTensor& sink_w, const MaybeTensor& sink_b) {
   const Tensor w = given(weight), b = given(bias);
-  eager_only("group norm", {x, w, b});
+  eager_only("group norm", {&x, &w, &b});
   if (!(at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))))
     return gn_forward(settled(x).contiguous(), w, b, groups, slope, eps, (int)out_type, false).y;
   const Sinks sinks{given(sink_w), given(sink_b)};
@@ -527,7 +527,7 @@ Tensor linear_residual(const Tensor& x_, const Tensor& weight_, const MaybeTenso
                        int64_t out_type, const MaybeTensor& sink_w, const MaybeTensor& sink_b) {
   const Tensor b = given(bias);
   Tensor x = x_, weight = weight_, r = given(residual);
-  eager_only("linear", {x, weight, b, r});
+  eager_only("linear", {&x, &weight, &b, &r});
   for (Tensor* t : {&x, &weight, &r}) if (t->defined()) *t = settled(*t);
   if (!(at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(b) || wants(r)))) {
     Tensor w = weight.contiguous();
@@ -553,37 +553,40 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // the passes on their own (missing tensors: None)
   m.def("group_norm_act_forward", [](const Tensor& x, const MaybeTensor& w, const MaybeTensor& b, int64_t groups, double slope, double eps,
                                      int64_t out_type, bool pack) {
-    eager_only("group norm", {x, given(w), given(b)});
-    const GnResult r = gn_forward(x, given(w), given(b), groups, slope, eps, (int)out_type, pack);
+    const Tensor wt = given(w), bt = given(b);
+    eager_only("group norm", {&x, &wt, &bt});
+    const GnResult r = gn_forward(x, wt, bt, groups, slope, eps, (int)out_type, pack);
     return std::make_tuple(r.y, r.stats, r.packed.codes, r.packed.exps);
   });
   m.def("group_norm_act_backward", [](const Tensor& dy, const MaybeTensor& x, const MaybeTensor& codes, const MaybeTensor& exps, int64_t x_type,
                                       const MaybeTensor& w, const MaybeTensor& b, int64_t groups, double slope, const Tensor& stats, bool need_dx,
                                       const MaybeTensor& dw, const MaybeTensor& db, bool accumulate) {
-    eager_only("group norm backward", {dy, given(x), given(w), given(b), stats, given(dw), given(db)});
-    return gn_backward(dy, given(x), Packed{given(codes), given(exps)}, (int)x_type, given(w), given(b), groups, slope, stats, need_dx, given(dw),
-                       given(db), accumulate);
+    const Tensor xt = given(x), wt = given(w), bt = given(b), dwt = given(dw), dbt = given(db);
+    eager_only("group norm backward", {&dy, &xt, &wt, &bt, &stats, &dwt, &dbt});
+    return gn_backward(dy, xt, Packed{given(codes), given(exps)}, (int)x_type, wt, bt, groups, slope, stats, need_dx, dwt, dbt, accumulate);
   });
   m.def("linear_forward", [](const Tensor& x, const Tensor& w, const MaybeTensor& b, const MaybeTensor& r, double slope, int64_t out_type, bool signs) {
-    eager_only("linear", {x, w, given(b), given(r)});
-    return lin_forward(x, w, given(b), given(r), slope, (int)out_type, signs);
+    const Tensor bt = given(b), rt = given(r);
+    eager_only("linear", {&x, &w, &bt, &rt});
+    return lin_forward(x, w, bt, rt, slope, (int)out_type, signs);
   });
   m.def("linear_backward_act", [](const Tensor& dy, const MaybeTensor& signs, double slope, int64_t dz_type, const MaybeTensor& db, bool accumulate) {
-    eager_only("linear backward", {dy, given(db)});
+    const Tensor dbt = given(db);
+    eager_only("linear backward", {&dy, &dbt});
     on_device(dy, "linear gradient");
-    return lin_backward_act(rows_of(dy, "linear gradient"), given(signs), slope, (int)dz_type, given(db), accumulate);
+    return lin_backward_act(rows_of(dy, "linear gradient"), given(signs), slope, (int)dz_type, dbt, accumulate);
   });
   m.def("linear_backward_data", [](const Tensor& dz, const Tensor& w, const MaybeTensor& signs, double slope) {
-    eager_only("linear backward", {dz, w});
+    eager_only("linear backward", {&dz, &w});
     on_device(dz, "linear gradient");
     const Rows r = rows_of(dz, "linear gradient");
     return lin_backward_data(r, given(signs), slope, w, {r.rows, w.size(-1)});
   });
   m.def("linear_backward_weight", [](const Tensor& dz, const MaybeTensor& x, const MaybeTensor& codes, const MaybeTensor& exps, const Tensor& dw,
                                      bool accumulate, const MaybeTensor& db, bool bias_accumulate, const MaybeTensor& signs, double slope) {
-    eager_only("linear backward", {dz, given(x), dw, given(db)});
+    const Tensor xt = given(x), dbt = given(db);
+    eager_only("linear backward", {&dz, &xt, &dw, &dbt});
     on_device(dz, "linear gradient");
-    lin_backward_weight(rows_of(dz, "linear gradient"), given(signs), slope, given(x), Packed{given(codes), given(exps)}, dw, accumulate, given(db),
-                        bias_accumulate);
+    lin_backward_weight(rows_of(dz, "linear gradient"), given(signs), slope, xt, Packed{given(codes), given(exps)}, dw, accumulate, dbt, bias_accumulate);
   });
 }

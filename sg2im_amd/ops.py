@@ -421,8 +421,7 @@ def _native_timed(kind, amount, token):
   TIMER.records.append((kind, amount, token[0], token[1], TIMER_TAG))
 
 
-_native_timed.active = lambda: TIMER is not None
-_lib.timed = _native_timed
+_lib.timed, _lib.timer = _native_timed, globals()
 
 
 def _desc_k(desc):
