@@ -33,6 +33,7 @@ namespace gn {
 
 constexpr int THREADS = 256;
 
+// (Times beside the kernels: medians of a profile, MI355X.)
 struct Params {
   const void* x;
   const signed char* codes;          // instead of x in the backward pass
@@ -201,8 +202,8 @@ __device__ __forceinline__ void sum_pixel_lanes(const V (&s)[NV], const V (&q)[N
   }
 }
 
-// sums of x and x^2 of every position over a chunk of rows.  Bound by memory: 32 x 256 x 256 x 64 bfloat16 46 us, 5.8 TB/s (the part
-// of x that a producer left in cache comes faster); 32 x 64 x 64 x 64 6.5 us.
+// sums of x and x^2 of every position over a chunk of rows.  Bound by memory: 32 x 256 x 256 x 64 bfloat16 47 us, 5.7 TB/s (the part
+// of x that a producer left in cache comes faster); 32 x 64 x 64 x 64 6.4 us.
 template <typename TX>
 __global__ __launch_bounds__(THREADS) void fwd_partial_kernel(const Params p) {
   constexpr int NV = VecOf<TX>::n, U = 4;
@@ -358,8 +359,8 @@ __device__ __forceinline__ int merged_stats(const Params& p, const Place& w, int
   return g0;
 }
 
-// the normalised, activated map (and x in 8 bits on the way).  Bound by memory: 32 x 128 x 128 x 64 float 45 us, 5.9 TB/s;
-// 32 x 256 x 256 x 64 bfloat16 with its codes 135 us, 5.0 TB/s.
+// the normalised, activated map (and x in 8 bits on the way).  Bound by memory: 32 x 128 x 128 x 64 float 44 us, 6.1 TB/s;
+// 32 x 256 x 256 x 64 bfloat16 with its codes 150 us, 4.5 TB/s.
 template <typename TX, typename TY, bool PACK>
 __global__ __launch_bounds__(THREADS) void fwd_apply_kernel(const Params p) {
   constexpr int NV = VecOf<TX>::n, U = 4;
@@ -440,7 +441,7 @@ __device__ __forceinline__ void back_values(const Params& p, int n, int q0, floa
 }
 
 // sums of dz and dz (x - m) of every position over a chunk of rows.  Bound by memory: 32 x 256 x 256 x 64 bfloat16 from the 8-bit
-// form 76 us, 5.3 TB/s.
+// form 80 us, 5.1 TB/s.
 template <typename SRC, typename TX, typename TY, bool EVEN>
 __global__ __launch_bounds__(THREADS) void bwd_partial_kernel(const Params p) {
   constexpr int NV = VecOf<TX>::n, U = 2;
@@ -581,7 +582,7 @@ __device__ __forceinline__ DxCoef dx_coef(double mean, double rstd, double m1, d
 }
 
 // dx; the workgroups behind the map's add up the parameters' gradients over the images (a launch less).  Bound by memory:
-// 32 x 256 x 256 x 64 bfloat16 from the 8-bit form 115 us, 5.9 TB/s.
+// 32 x 256 x 256 x 64 bfloat16 from the 8-bit form 117 us, 5.8 TB/s.
 template <typename SRC, typename TX, typename TY, bool EVEN>
 __global__ __launch_bounds__(THREADS) void bwd_apply_kernel(const Params p, long long main_blocks) {
   constexpr int NV = VecOf<TX>::n, U = 2;
@@ -633,7 +634,7 @@ __global__ __launch_bounds__(THREADS) void bwd_apply_kernel(const Params p, long
 // A slab is S positions of a row that hold whole groups, over all rows of one image.  Its pieces stay in registers (up to
 // ITER per thread) between the statistics and their use: x is read once and one launch does the forward pass, one (and one
 // for the parameters' sums over the images) the backward pass.  Bound by latency - load, join, join, store: 32 x 4 x 4 x 1024
-// float 6.1 us forward, 8.8 + 3.5 backward.
+// float 6.2 us forward, 9.0 + 3.8 backward.
 
 struct Slab { int q0, pl, n, base, TV, TP; bool on; };
 __device__ __forceinline__ Slab slab_of(const Params& p, int NV) {
@@ -743,7 +744,7 @@ __global__ __launch_bounds__(B) void fwd_slab_kernel(const Params p) {
   }
   const int first = p.L > p.C ? 0 : w.base / p.D;
   if (p.L == p.C && p.D % NV == 0) {
-    // a piece lies in one group: a thread has one sum, and a wave joins a group's (32 x 8 x 8 x 512 bfloat16 8.2 us; by
+    // a piece lies in one group: a thread has one sum, and a wave joins a group's (32 x 8 x 8 x 512 bfloat16 8.5 us; by
     // positions first, as below, 10.7)
     double a = 0.0, b = 0.0;
     #pragma unroll
@@ -900,7 +901,7 @@ __global__ __launch_bounds__(B) void bwd_slab_kernel(const Params p) {
 
 // A lane takes one 16-byte piece of x; 4 (bfloat16) or 8 (float) neighbouring lanes make a block of 32 channels.  Pieces are
 // numbered along the rows; a workgroup takes a run of U * 256 of them, U in flight per lane.  2097152 x 64 bfloat16: pack 83 us,
-// unpack 60 us (4.9 and 6.7 TB/s; with the grid's stride between a lane's pieces and cached stores 98 and 123).
+// unpack 64 us (4.9 and 6.4 TB/s; with the grid's stride between a lane's pieces and cached stores 98 and 123).
 template <typename T>
 __global__ __launch_bounds__(THREADS) void pack8_kernel(const T* __restrict__ x, long long rows, int C, int nblk, long long ld,
                                                         signed char* __restrict__ codes, unsigned char* __restrict__ exps) {
@@ -1049,7 +1050,10 @@ void over_images(const Params& p, long long blocks_per_image, int threads, F lau
 
 // The slab kernels' cut: the fewest positions that hold whole groups, whole pieces (`unit`) and 32 channels, more of them where
 // a thread would not have its first piece yet and there are workgroups to spare.  False: an image does not fit
-// the registers of a workgroup, and the chunked kernels take it.
+// the registers of a workgroup, and the chunked kernels take it.  Slab / chunks, microseconds: few images of small maps gain (float
+// forward 32 x 4 x 4 x 512 5.5 / 9.8, 32 x 16 x 16 x 256 9.4 / 14.0; bfloat16 32 x 16 x 16 x 512 11.3 / 18.9; backward 32 x 4 x 4 x 512 float
+// 10.5 / 13.3), many images and groups of one or two channels lose (float forward 32 x 8 x 8 x 32 14.7 / 9.3, 2048 x 4 x 4 x 256 51 / 24;
+// backward 256 x 16 x 16 x 256 99 / 73); over 214 maps the geometric mean is 2 % apart forward, 1 % backward.
 struct SlabPlan { int S, slabs, threads, iter; };
 bool slab_plan(const Params& p, int nv, int most, SlabPlan& q) {
   int unit = p.L > p.C ? p.L : p.D / gcd(p.D, nv) * nv;

@@ -12,8 +12,9 @@
 // barrier per chunk.
 //
 // Bound by the matrix cores where there is enough to do: bfloat16 8192^3 1.23 PFLOP/s (a library's product 1.5: its matrix cores
-// are busy 88 % of the time, these 71 %), 32768 x 4096 x 1024 with bias and activation 274 us; float 3200 x 1152 x 512 41 us, of
-// which 1.79 us per 32 of r at 1.71 of matrix instructions.  Narrow reductions are bound by their first loads and the epilogue.
+// are busy 88 % of the time, these 71 %), 32768 x 4096 x 1024 with bias and activation 272 us in a stream of
+// such passes (299 - 315 in profiles of ten); float 3200 x 1152 x 512 44 us, of which 1.79 us per 32 of r at 1.71 of matrix
+// instructions.  Narrow reductions are bound by their first loads and the epilogue.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <algorithm>
