@@ -348,3 +348,56 @@ def test_which_side_of_the_kink_the_backward_pass_takes(channels, pack):
   assert not bool((other & ~near).any())
   if channels > 100:
     assert bool(other.any())                        # (it does happen: the two passes are not one function's)
+
+
+# ---- which gradients are asked for; the widest maps -------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize('shape,groups', [((8, 64, 64, 64), 32), ((3, 40, 40, 105), 5), ((4, 4, 4, 256), 8), ((1, 4, 4, 256), 8)])
+@pytest.mark.parametrize('pack', [False, True])
+def test_each_gradient_alone_is_what_it_is_among_all(shape, groups, pack):
+  from sg2im_amd import functional as HF
+  g = torch.Generator(device='cuda').manual_seed(9)
+  r = lambda *s: torch.randn(*s, device='cuda', generator=g)  # noqa: E731
+  C = shape[-1]
+  values, dy = (r(*shape), 1 + 0.1 * r(C), 0.1 * r(C)), r(*shape)
+
+  def grads(wanted):
+    leaves = [t.clone().requires_grad_(k in wanted) for k, t in enumerate(values)]
+    y = HF.GroupNormAct.apply(*leaves, groups, 0.2, 1e-5, pack)
+    return torch.autograd.grad(y, [leaves[k] for k in wanted], dy)
+  every = grads((0, 1, 2))
+  for wanted in ((0,), (1,), (2,), (1, 2), (0, 2), (0, 1)):
+    for k, got in zip(wanted, grads(wanted)):
+      assert torch.equal(got, every[k]), (wanted, k)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('shape,groups', [((2, 1, 1, 1 << 20), 1), ((2, 1, 1, 1 << 20), 1 << 18), ((1, 3, 1, 1000003), 1), ((1, 5, 7, 40000), 40000),
+                                          ((1, 1, 1, 1 << 24), 64), ((1, 1 << 22, 1, 3), 1)])
+def test_the_widest_and_the_longest_maps(shape, groups, dtype, monkeypatch):
+  """(float32 additions in a row per thread: rows / 1024 chunks / the pixel lanes, below 64 here)"""
+  from sg2im_amd import functional as HF
+  from tests import test_groupnorm_linear_ckpt8 as base
+  monkeypatch.setattr(base, 'T', 64)
+  r = base.gen(61)
+  C = shape[-1]
+  x0, w0, b0, dy = (2 * r(*shape) + 1).to(dtype), (1 + 0.2 * r(C)).to(dtype), (0.2 * r(C)).to(dtype), r(*shape).to(dtype)
+  half = base.half_step(dtype)
+  for pack in (False, True):
+    x, w, b = (t.clone().requires_grad_(True) for t in (x0, w0, b0))
+    y = HF.GroupNormAct.apply(x, w, b, groups, 0.2, 1e-5, pack)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    seen = x0
+    if pack:
+      seen = base.eight(x0)[0] if C < 100000 else unpacked(x0)
+    f = base.gn_reference(x0, seen, w0, b0, groups, 0.2, 1e-5, dy)
+    for name, got in (('y', y), ('dx', dx), ('dw', dw), ('db', db)):
+      base.check(got, f[name], f[name + '_tol'] + half * f[name].abs(), name)
+
+
+def unpacked(x):
+  """(the definition in base.eight goes block by block: too many here, and pack8 is held to it elsewhere)"""
+  from sg2im_amd import ops
+  return ops.unpack8(ops.pack8(x), F32)

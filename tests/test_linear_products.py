@@ -207,3 +207,26 @@ def test_training_pass(bf16, gated, bias, dx, dw, size, checkpoint8):
     exactly(grads['dweight'], product(dz.t(), x.detach()), 'dweight')
   if bias:
     exactly(grads['dbias'], dz.sum(0), 'dbias')
+
+
+# the widest operands (2^22 columns), with ones and minus ones: sums stay below 2^24
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('size', [(3, 1 << 22, 2), (2, 3, 1 << 22), (1, (1 << 22) - 3, 1), (5, 1, (1 << 22) - 1)])
+def test_the_widest_layers(size, dtype):
+  from sg2im_amd import functional as HF
+  rows, k, n = size
+  g = torch.Generator(device='cuda').manual_seed(k + n)
+  r = lambda *s: (torch.randint(0, 2, s, device='cuda', generator=g) * 2 - 1).to(dtype)  # noqa: E731
+  for slope, checkpoint8 in ((SLOPE, False), (1.0, True)):
+    x, w, b, res = [t.requires_grad_(True) for t in (r(rows, k), r(n, k), r(n), r(rows, n))]
+    y = HF.LinearResidual.apply(x, w, b, res, slope, checkpoint8)
+    z = x.detach().to(F64) @ w.detach().to(F64).t() + b.detach().to(F64)
+    exactly(y.detach(), torch.where(z > 0, z, z * slope) + res.detach().to(F64), 'y')
+    dy = r(rows, n)
+    dz = dy.to(F64) * torch.where(z > 0, 1.0, slope)
+    dx, dw, db, dres = torch.autograd.grad(y, (x, w, b, res), dy)
+    exactly(dx, dz @ w.detach().to(F64), 'dx')
+    exactly(dw, dz.t() @ x.detach().to(F64), 'dweight')
+    exactly(db, dz.sum(0), 'dbias')
+    exactly(dres, dy, 'dresidual')
